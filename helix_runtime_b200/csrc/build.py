@@ -44,9 +44,14 @@ SOURCES = (
     "hx_attention.cu",
     "hx_attention_mma.cu",
     "hx_attention_tc.cu",
+    "hx_tree_attention.cu",
+    "hx_tree_attention_tc.cu",
+    "hx_verify.cu",
+    "hx_cache_rows.cu",
     "hx_sampling.cu",
 )
-HEADERS = ("hx_common.cuh", "hx_scan.cuh", "hx_mma.cuh", "hx_tcgen05.cuh", "hx_tensor_map.cuh", "hx_no_alloc.h")
+HEADERS = ("hx_common.cuh", "hx_scan.cuh", "hx_mma.cuh", "hx_tcgen05.cuh", "hx_tensor_map.cuh",
+           "hx_tree_attention.cuh", "hx_no_alloc.h")
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",

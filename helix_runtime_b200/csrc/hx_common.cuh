@@ -30,6 +30,7 @@ enum HxDeviceFlag : int {
   HX_FLAG_WAIT_TIMEOUT = 4,   // a bounded mbarrier wait gave up
   HX_FLAG_NONFINITE = 8,      // sampling saw a non-finite logit
   HX_FLAG_BAD_POSITION = 16,  // a token's position lies outside the position table
+  HX_FLAG_BAD_MOVE = 32,      // a move of cached rows or pages would overwrite what another one needs
 };
 
 void hx_set_error(const char* format, ...);

@@ -1,0 +1,573 @@
+// Attention of a tree of drafted tokens over the paged cache.
+//
+// A request brings `nodes` drafted tokens to a step.  Token n's key and value lie in the request's
+// pages at place context + n (whatever position it was rotated for); it attends to the context
+// cached keys and to the drafted tokens its bit mask names, usually itself and its ancestors in the
+// tree:
+//     o_n = sum_j w_nj v_j / sum_j w_nj,   w_nj = exp(scale q_n . k_j),   j cached or named.
+// A token that sees nothing (no cached key, no bit) gets zeros.
+//
+// The causal kernels take one position per token and everything in front of it; here the order of
+// the drafted keys says nothing, and all tokens of a request read the same cached keys.  So a
+// CTA takes the tokens of a request (and the query heads that share a key/value head) as rows of
+// one tile and reads every key once for all of them; a long context is cut over CTAs (see
+// hx_tree_attention.cuh).  Three kernels:
+//   * hx_tree_attention_tc.cu: bfloat16, heads of 64 to 128, pages of 16, 32 or 64 keys;
+//   * tree_tile_kernel: any other page size, float32 or bfloat16, heads up to 256 in steps of 4.
+//     32 rows by 64 keys at a time on the CUDA cores, all in float32;
+//   * tree_row_kernel: what is left (heads up to 1,024, even), a row a warp.
+#include "hx_tree_attention.cuh"
+
+#include <mutex>
+
+namespace {
+
+// ------------------------------------------------------------------ 32 rows x 64 keys
+
+constexpr int TILE_ROWS = 32, TILE_KEYS = 64, TILE_WARPS = 4, ROWS_A_WARP = TILE_ROWS / TILE_WARPS;
+constexpr int TILE_LEAST = 2;      // key tiles of the shortest run
+
+template <int D_MAX>
+struct TileConfig {
+  // queries [32][D], keys [D / 4][64][4], values [64][D + 4], probabilities [32][64]
+  static constexpr int floats(int d) {
+    return TILE_ROWS * d + TILE_KEYS * d + TILE_KEYS * (d + 4) + TILE_ROWS * TILE_KEYS;
+  }
+  static constexpr int kCtas = floats(D_MAX) * 4 <= 110 * 1024 ? 2 : 1;
+};
+
+// Four consecutive coordinates of a cached row, wherever the cache's pieces put them.
+template <typename T> __device__ __forceinline__ float4 load_four(const T* p);
+template <> __device__ __forceinline__ float4 load_four<float>(const float* p) {
+  return *reinterpret_cast<const float4*>(p);
+}
+template <> __device__ __forceinline__ float4 load_four<__nv_bfloat16>(const __nv_bfloat16* p) {
+  const uint2 raw = *reinterpret_cast<const uint2*>(p);
+  const __nv_bfloat162 low = *reinterpret_cast<const __nv_bfloat162*>(&raw.x);
+  const __nv_bfloat162 high = *reinterpret_cast<const __nv_bfloat162*>(&raw.y);
+  return make_float4(__bfloat162float(low.x), __bfloat162float(low.y), __bfloat162float(high.x),
+                     __bfloat162float(high.y));
+}
+
+// Scores: a warp has 8 rows, a lane 2 keys; a key's four coordinates are read once for 8 rows, a
+// row's are broadcast.  Values: a lane has 4 (8, above 128) coordinates of the same 8 rows.  Per SM the
+// shared-memory reads of both products take about as long as their multiply-adds, which is the bound.
+template <typename T, int D_MAX>
+__global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tree_tile_kernel(
+    const TreeArgs a) {
+  extern __shared__ float4 tile_shared[];
+  constexpr int OUT_PIECES = (D_MAX + 127) / 128;
+  hx_pdl_prologue();
+  const int D = a.head_dim, D4 = D / 4;
+  float* q_rows = reinterpret_cast<float*>(tile_shared);
+  float* keys = q_rows + TILE_ROWS * D;
+  float* values = keys + TILE_KEYS * D;
+  float* probabilities = values + TILE_KEYS * (D + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TreeRun run = tree_run<TILE_KEYS>(a, blockIdx.x, gridDim.x, TILE_LEAST);
+  if (run.count == 0) return;
+  TreeCursor c;
+  long long item_begin;
+  tree_locate<TILE_KEYS>(a, run.begin, c, item_begin);
+  const int chunk = hx_cache_chunk(sizeof(T), D);
+  const T* q = static_cast<const T*>(a.q);
+  const T* k_cache = static_cast<const T*>(a.k_cache);
+  const T* v_cache = static_cast<const T*>(a.v_cache);
+  const float scale_log2 = a.scale * HX_LOG2E;
+
+  for (int left = run.count; left > 0;) {
+    const int count = min(c.tiles - c.tile, left);
+    const TreeRows rows(a, c);
+    const int rows_here = rows.count, kv_head = rows.kv_head;
+    const int last_key = c.context + c.nodes - 1;
+    const int* table = a.block_tables + static_cast<size_t>(a.request_table_row[c.request]) * a.table_stride;
+    __syncthreads();
+    for (int i = threadIdx.x; i < TILE_ROWS * D4; i += blockDim.x) {
+      const int row = i / D4, d4 = i - row * D4;
+      float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (row < rows_here)
+        value = load_four<T>(q + static_cast<size_t>(c.q_begin + rows.token0 + row / rows.heads) * a.ldq +
+                             static_cast<size_t>(rows.head0 + row % rows.heads) * D + 4 * d4);
+      reinterpret_cast<float4*>(q_rows)[row * D4 + d4] = value;
+    }
+    float row_max[ROWS_A_WARP], row_sum[ROWS_A_WARP];
+    float4 acc[ROWS_A_WARP][OUT_PIECES];
+#pragma unroll
+    for (int i = 0; i < ROWS_A_WARP; ++i) {
+      row_max[i] = -INFINITY;
+      row_sum[i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < OUT_PIECES; ++j) acc[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    const bool live = warp * ROWS_A_WARP < rows_here;      // this warp has rows
+    for (int t = 0; t < count; ++t) {
+      const int key0 = (c.tile + t) * TILE_KEYS;
+      __syncthreads();      // the last tile has been read (and the queries are written)
+      // ---- keys and values of the tile; a key that does not exist or has no page is zeros
+      for (int i = threadIdx.x; i < TILE_KEYS * D4; i += blockDim.x) {
+        const int d4 = i / TILE_KEYS, key = i - d4 * TILE_KEYS;
+        float4 kv = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vv = kv;
+        if (key0 + key <= last_key) {
+          const int index = (key0 + key) / a.page_size;
+          const int page = index < a.table_stride ? table[index] : -1;
+          if (page < 0 || page >= a.num_pages) {
+            if (d4 == 0) atomicOr(a.status, HX_FLAG_BAD_PAGE);
+          } else {
+            const size_t at = hx_cache_offset(page, kv_head, (key0 + key) % a.page_size, 4 * d4, a.kv_heads,
+                                              a.page_size, D, chunk);
+            kv = load_four<T>(k_cache + at);
+            vv = load_four<T>(v_cache + at);
+          }
+        }
+        reinterpret_cast<float4*>(keys)[d4 * TILE_KEYS + key] = kv;
+        *reinterpret_cast<float4*>(values + key * (D + 4) + 4 * d4) = vv;
+      }
+      __syncthreads();
+      if (!live) continue;
+      // ---- scores of 8 rows against keys `lane` and `lane + 32`
+      float s[ROWS_A_WARP][2];
+#pragma unroll
+      for (int i = 0; i < ROWS_A_WARP; ++i) s[i][0] = s[i][1] = 0.0f;
+      const float4* my_q = reinterpret_cast<const float4*>(q_rows) + warp * ROWS_A_WARP * D4;
+#pragma unroll 2
+      for (int d4 = 0; d4 < D4; ++d4) {
+        const float4 k0 = reinterpret_cast<const float4*>(keys)[d4 * TILE_KEYS + lane];
+        const float4 k1 = reinterpret_cast<const float4*>(keys)[d4 * TILE_KEYS + lane + 32];
+#pragma unroll
+        for (int i = 0; i < ROWS_A_WARP; ++i) {
+          const float4 qi = my_q[i * D4 + d4];
+          s[i][0] = fmaf(qi.x, k0.x, s[i][0]);
+          s[i][1] = fmaf(qi.x, k1.x, s[i][1]);
+          s[i][0] = fmaf(qi.y, k0.y, s[i][0]);
+          s[i][1] = fmaf(qi.y, k1.y, s[i][1]);
+          s[i][0] = fmaf(qi.z, k0.z, s[i][0]);
+          s[i][1] = fmaf(qi.z, k1.z, s[i][1]);
+          s[i][0] = fmaf(qi.w, k0.w, s[i][0]);
+          s[i][1] = fmaf(qi.w, k1.w, s[i][1]);
+        }
+      }
+      // ---- the running maximum and sum of every row
+#pragma unroll
+      for (int i = 0; i < ROWS_A_WARP; ++i) {
+        const int row = warp * ROWS_A_WARP + i;
+        unsigned long long mask = ~0ull;
+        if (key0 + TILE_KEYS > c.context)
+          mask = row < rows_here ? tree_mask(a, c, rows.token0 + row / rows.heads, key0) : 0ull;
+        const float s0 = (mask >> lane) & 1 ? s[i][0] * scale_log2 : -INFINITY;
+        const float s1 = (mask >> (lane + 32)) & 1 ? s[i][1] * scale_log2 : -INFINITY;
+        float top = fmaxf(s0, s1);
+#pragma unroll
+        for (int offset = 16; offset > 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+        const float new_max = fmaxf(row_max[i], top);
+        const float against = new_max == -INFINITY ? 0.0f : new_max;
+        const float p0 = exp2f(s0 - against), p1 = exp2f(s1 - against);
+        const float correction = exp2f(row_max[i] - against);
+        float sum = p0 + p1;
+#pragma unroll
+        for (int offset = 16; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+        row_sum[i] = fmaf(row_sum[i], correction, sum);
+        row_max[i] = new_max;
+        probabilities[row * TILE_KEYS + lane] = p0;
+        probabilities[row * TILE_KEYS + lane + 32] = p1;
+#pragma unroll
+        for (int j = 0; j < OUT_PIECES; ++j) {
+          acc[i][j].x *= correction;
+          acc[i][j].y *= correction;
+          acc[i][j].z *= correction;
+          acc[i][j].w *= correction;
+        }
+      }
+      __syncwarp();
+      // ---- the weighted values: coordinates 4 lane .. of 8 rows, four keys at a time
+      const float4* my_p = reinterpret_cast<const float4*>(probabilities) + warp * ROWS_A_WARP * (TILE_KEYS / 4);
+      // (a drafted key that a row does not see adds nothing to it, not even an infinity times zero)
+      const bool drafted = key0 + TILE_KEYS > c.context;
+      const int keys_here = min(TILE_KEYS, last_key + 1 - key0);
+      for (int key4 = 0; key4 * 4 < keys_here; ++key4) {
+        float4 v[4][OUT_PIECES];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < OUT_PIECES; ++j) {
+            const int d = 4 * lane + 128 * j;
+            if (d < D) v[k][j] = *reinterpret_cast<const float4*>(values + (4 * key4 + k) * (D + 4) + d);
+          }
+#pragma unroll
+        for (int i = 0; i < ROWS_A_WARP; ++i) {
+          const float4 p = my_p[i * (TILE_KEYS / 4) + key4];
+          const float w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < OUT_PIECES; ++j) {
+              if (drafted && w[k] == 0.0f) continue;
+              acc[i][j].x = fmaf(w[k], v[k][j].x, acc[i][j].x);
+              acc[i][j].y = fmaf(w[k], v[k][j].y, acc[i][j].y);
+              acc[i][j].z = fmaf(w[k], v[k][j].z, acc[i][j].z);
+              acc[i][j].w = fmaf(w[k], v[k][j].w, acc[i][j].w);
+            }
+        }
+      }
+    }
+    // ---- the rows, or this CTA's part of them
+    if (live) {
+      const bool whole = c.tile == 0 && count == c.tiles;
+      float* part = a.partial + (2ll * blockIdx.x + (c.tile == 0 ? 1 : 0)) * tree_part_floats<TILE_ROWS>(D);
+#pragma unroll
+      for (int i = 0; i < ROWS_A_WARP; ++i) {
+        const int row = warp * ROWS_A_WARP + i;
+        if (row >= rows_here) break;
+        const float inverse = row_sum[i] > 0.0f ? 1.0f / row_sum[i] : 0.0f;
+        T* out = static_cast<T*>(a.out) + static_cast<size_t>(c.q_begin + rows.token0 + row / rows.heads) * a.ldo +
+                 static_cast<size_t>(rows.head0 + row % rows.heads) * D;
+#pragma unroll
+        for (int j = 0; j < OUT_PIECES; ++j) {
+          const int d = 4 * lane + 128 * j;
+          if (d >= D) continue;
+          const float4 v = acc[i][j];
+          if (whole) {
+            out[d] = hx_from_float<T>(v.x * inverse);
+            out[d + 1] = hx_from_float<T>(v.y * inverse);
+            out[d + 2] = hx_from_float<T>(v.z * inverse);
+            out[d + 3] = hx_from_float<T>(v.w * inverse);
+          } else {
+            *reinterpret_cast<float4*>(part + (static_cast<size_t>(d / 4) * TILE_ROWS + row) * 4) = v;
+          }
+        }
+        if (!whole && lane == 0) {
+          part[static_cast<size_t>(D) * TILE_ROWS + row] = row_max[i];
+          part[static_cast<size_t>(D + 1) * TILE_ROWS + row] = row_sum[i];
+        }
+      }
+    }
+    left -= count;
+    if (left > 0) tree_next_item<TILE_KEYS>(a, c);
+  }
+}
+
+// ------------------------------------------------------------------ a row a warp
+
+constexpr int ROW_WARPS = 4, ROW_KEYS = 64, ROW_MAX_DIM = 1024, ROW_CTAS = 4, ROW_LEAST = 2;
+
+// Lane j owns keys j and j + 32 of a tile for the scores and pairs of coordinates 2 lane + 64 i for
+// the values.  No shared keys: for head sizes that no model here has, right rather than fast.
+template <typename T>
+__global__ __launch_bounds__(ROW_WARPS * 32) void tree_row_kernel(const TreeArgs a) {
+  __shared__ float q_shared[ROW_WARPS][ROW_MAX_DIM];
+  constexpr int PAIRS = ROW_MAX_DIM / 64;
+  hx_pdl_prologue();
+  const int D = a.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TreeRun run = tree_run<ROW_KEYS>(a, blockIdx.x, gridDim.x, ROW_LEAST);
+  if (run.count == 0) return;
+  TreeCursor c;
+  long long item_begin;
+  tree_locate<ROW_KEYS>(a, run.begin, c, item_begin);
+  const int chunk = hx_cache_chunk(sizeof(T), D);
+  const T* k_cache = static_cast<const T*>(a.k_cache);
+  const T* v_cache = static_cast<const T*>(a.v_cache);
+  const float scale_log2 = a.scale * HX_LOG2E;
+  for (int left = run.count; left > 0;) {
+    const int count = min(c.tiles - c.tile, left);
+    const TreeRows rows(a, c);
+    const int rows_here = rows.count, kv_head = rows.kv_head;
+    const int last_key = c.context + c.nodes - 1;
+    const int* table = a.block_tables + static_cast<size_t>(a.request_table_row[c.request]) * a.table_stride;
+    const int row = warp;
+    if (row < rows_here) {
+      const int token = rows.token0 + row / rows.heads, head = rows.head0 + row % rows.heads;
+      const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(c.q_begin + token) * a.ldq +
+                   static_cast<size_t>(head) * D;
+      float* qs = q_shared[warp];
+      __syncwarp();
+      for (int d = lane; d < D; d += 32) qs[d] = hx_to_float<T>(q[d]);
+      __syncwarp();
+      float acc[PAIRS][2];
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) acc[i][0] = acc[i][1] = 0.0f;
+      float row_max = -INFINITY, row_sum = 0.0f;
+      for (int t = 0; t < count; ++t) {
+        const int key0 = (c.tile + t) * ROW_KEYS;
+        const unsigned long long mask = tree_mask(a, c, token, key0);
+        for (int half = 0; half < 2; ++half) {
+          const int key = key0 + 32 * half + lane;
+          int page = -1;
+          if (key <= last_key) {
+            const int index = key / a.page_size;
+            page = index < a.table_stride ? table[index] : -1;
+            if (page < 0 || page >= a.num_pages) {
+              atomicOr(a.status, HX_FLAG_BAD_PAGE);
+              page = -1;
+            }
+          }
+          float score = -INFINITY;
+          if (page >= 0 && ((mask >> (32 * half + lane)) & 1)) {
+            float dot = 0.0f;
+            for (int d = 0; d < D; d += 2) {
+              const T* k = k_cache + hx_cache_offset(page, kv_head, key % a.page_size, d, a.kv_heads,
+                                                     a.page_size, D, chunk);
+              dot = fmaf(qs[d], hx_to_float<T>(k[0]), dot);
+              dot = fmaf(qs[d + 1], hx_to_float<T>(k[1]), dot);
+            }
+            score = dot * scale_log2;
+          }
+          const unsigned seen = __ballot_sync(0xffffffffu, score != -INFINITY);
+          if (seen == 0u) continue;
+          float top = score;
+#pragma unroll
+          for (int offset = 16; offset > 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+          const float new_max = fmaxf(row_max, top);
+          const float correction = exp2f(row_max - new_max);
+          const float p = score == -INFINITY ? 0.0f : exp2f(score - new_max);
+          float sum = p;
+#pragma unroll
+          for (int offset = 16; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+          row_sum = fmaf(row_sum, correction, sum);
+          row_max = new_max;
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) {
+            acc[i][0] *= correction;
+            acc[i][1] *= correction;
+          }
+          for (unsigned rest = seen; rest != 0u; rest &= rest - 1) {
+            const int j = __ffs(rest) - 1;
+            const float w = __shfl_sync(0xffffffffu, p, j);
+            const int v_page = __shfl_sync(0xffffffffu, page, j);
+            const int slot = (key0 + 32 * half + j) % a.page_size;
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+              const int d = 2 * lane + 64 * i;
+              if (d >= D) continue;
+              const T* v = v_cache + hx_cache_offset(v_page, kv_head, slot, d, a.kv_heads, a.page_size, D, chunk);
+              acc[i][0] = fmaf(w, hx_to_float<T>(v[0]), acc[i][0]);
+              acc[i][1] = fmaf(w, hx_to_float<T>(v[1]), acc[i][1]);
+            }
+          }
+        }
+      }
+      const bool whole = c.tile == 0 && count == c.tiles;
+      const float inverse = row_sum > 0.0f ? 1.0f / row_sum : 0.0f;
+      T* out = static_cast<T*>(a.out) + static_cast<size_t>(c.q_begin + token) * a.ldo +
+               static_cast<size_t>(head) * D;
+      float* part = a.partial + (2ll * blockIdx.x + (c.tile == 0 ? 1 : 0)) * tree_part_floats<ROW_WARPS>(D);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const int d = 2 * lane + 64 * i;
+        if (d >= D) continue;
+        if (whole) {
+          out[d] = hx_from_float<T>(acc[i][0] * inverse);
+          out[d + 1] = hx_from_float<T>(acc[i][1] * inverse);
+        } else {
+          *reinterpret_cast<float2*>(part + (static_cast<size_t>(d / 2) * ROW_WARPS + row) * 2) =
+              make_float2(acc[i][0], acc[i][1]);
+        }
+      }
+      if (!whole && lane == 0) {
+        part[static_cast<size_t>(D) * ROW_WARPS + row] = row_max;
+        part[static_cast<size_t>(D + 1) * ROW_WARPS + row] = row_sum;
+      }
+    }
+    left -= count;
+    if (left > 0) tree_next_item<ROW_KEYS>(a, c);
+  }
+}
+
+// ------------------------------------------------------------------ joining parts
+
+constexpr int JOIN_THREADS = 128;
+constexpr int JOIN_LOADS = 4;      // parts whose loads are in flight together
+
+// Block (x, y): the item that begins in the run of CTA x and goes on behind it, if there is one,
+// and the y-th share of its rows' coordinates.  The parts: the one CTA x left in its place 1, and those the
+// CTAs behind it left in their place 0, in that order.  The run of x is empty or the item ends
+// inside it: nothing to do.
+template <typename T, int ROWS, int KEYS, int VEC>
+__global__ __launch_bounds__(JOIN_THREADS) void tree_join_kernel(const TreeArgs a, int ctas, int least) {
+  // the runs are found from the step's description, which was there before the kernel in front
+  hx_pdl_trigger();
+  const int owner = blockIdx.x;
+  const TreeRun run = tree_run<KEYS>(a, owner, ctas, least);
+  TreeCursor c;
+  long long item_begin = 0;
+  bool mine = false;
+  int parts = 0;
+  if (run.count > 0) {
+    tree_locate<KEYS>(a, run.begin + run.count - 1, c, item_begin);
+    mine = item_begin >= run.begin && item_begin + c.tiles > run.begin + run.count;
+    if (mine) parts = static_cast<int>((item_begin + c.tiles - 1) / run.per_cta) - owner + 1;
+  }
+  hx_pdl_wait();
+  if (!mine) return;
+  const int D = a.head_dim;
+  const TreeRows rows(a, c);
+  const int rows_here = rows.count;
+  const long long stride = tree_part_floats<ROWS>(D);
+  const float* first = a.partial + (2ll * owner + 1) * stride;
+  const float* others = a.partial + 2ll * (owner + 1) * stride;
+  auto part_of = [&](int index) { return index == 0 ? first : others + 2ll * (index - 1) * stride; };
+  const int pieces = D / VEC;
+  for (int i = blockIdx.y * JOIN_THREADS + threadIdx.x; i < rows_here * pieces; i += gridDim.y * JOIN_THREADS) {
+    const int piece = i / rows_here, row = i - piece * rows_here;
+    float total_max = -INFINITY, total_sum = 0.0f, acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+    for (int base = 0; base < parts; base += JOIN_LOADS) {
+      float m[JOIN_LOADS], l[JOIN_LOADS], o[JOIN_LOADS][VEC];
+#pragma unroll
+      for (int u = 0; u < JOIN_LOADS; ++u) {
+        m[u] = -INFINITY;
+        l[u] = 0.0f;
+        if (base + u < parts) {
+          const float* part = part_of(base + u);
+          m[u] = __ldcg(part + static_cast<size_t>(D) * ROWS + row);
+          l[u] = __ldcg(part + static_cast<size_t>(D + 1) * ROWS + row);
+          const float* at = part + (static_cast<size_t>(piece) * ROWS + row) * VEC;
+          if constexpr (VEC == 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(at));
+            o[u][0] = v.x; o[u][1] = v.y; o[u][2] = v.z; o[u][3] = v.w;
+          } else {
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(at));
+            o[u][0] = v.x; o[u][1] = v.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < JOIN_LOADS; ++u) {
+        if (m[u] == -INFINITY) continue;      // no part, or one whose row saw nothing
+        const float new_max = fmaxf(total_max, m[u]);
+        const float keep = exp2f(total_max - new_max), take = exp2f(m[u] - new_max);
+        total_max = new_max;
+        total_sum = fmaf(total_sum, keep, l[u] * take);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = fmaf(acc[e], keep, o[u][e] * take);
+      }
+    }
+    const float inverse = total_sum > 0.0f ? 1.0f / total_sum : 0.0f;
+    T* out = static_cast<T*>(a.out) + static_cast<size_t>(c.q_begin + rows.token0 + row / rows.heads) * a.ldo +
+             static_cast<size_t>(rows.head0 + row % rows.heads) * D + piece * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) out[e] = hx_from_float<T>(acc[e] * inverse);
+  }
+}
+
+int tile_ctas_an_sm(int head_dim) { return head_dim <= 128 ? 2 : 1; }
+
+template <typename T, int D_MAX>
+int launch_tile(const TreeArgs& a, int ctas, cudaStream_t stream) {
+  const int bytes = TileConfig<D_MAX>::floats(a.head_dim) * 4;
+  static std::once_flag once;
+  static bool reserved = false;
+  std::call_once(once, [] {
+    reserved = cudaFuncSetAttribute(tree_tile_kernel<T, D_MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    TileConfig<D_MAX>::floats(D_MAX) * 4) == cudaSuccess;
+    if (!reserved) cudaGetLastError();
+  });
+  HX_REQUIRE(reserved, "hx_tree_attention: cannot reserve shared memory");
+  hx_launch(tree_tile_kernel<T, D_MAX>, ctas, TILE_WARPS * 32, bytes, stream, a);
+  HX_CHECK_LAUNCH("hx_tree_attention");
+  return HX_OK;
+}
+
+// Which kernel: the tensor cores', the tile kernel, or the row kernel.
+enum TreeKernel { TREE_TC, TREE_TILE, TREE_ROW };
+TreeKernel kernel_for(int dtype, int head_dim, int page_size) {
+  if (dtype == HX_BF16 && hx_tree_tc_takes(head_dim, page_size)) return TREE_TC;
+  if (head_dim % 4 == 0 && head_dim <= 256) return TREE_TILE;
+  return TREE_ROW;
+}
+
+}  // namespace
+
+int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int least, int rows, int keys, int vec,
+                 cudaStream_t stream) {
+  // shares of an item's coordinates: 16 of them, so that a block has a few pieces a thread at most
+  const int shares = rows >= 128 ? 16 : rows >= 32 ? 8 : 2;
+  const dim3 grid(ctas, shares);
+  const bool half = dtype == HX_BF16;
+  if (rows == 128 && keys == 64 && vec == 4 && half)
+    hx_launch(tree_join_kernel<__nv_bfloat16, 128, 64, 4>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+  else if (rows == TILE_ROWS && half)
+    hx_launch(tree_join_kernel<__nv_bfloat16, TILE_ROWS, TILE_KEYS, 4>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+  else if (rows == TILE_ROWS)
+    hx_launch(tree_join_kernel<float, TILE_ROWS, TILE_KEYS, 4>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+  else if (half)
+    hx_launch(tree_join_kernel<__nv_bfloat16, ROW_WARPS, ROW_KEYS, 2>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+  else
+    hx_launch(tree_join_kernel<float, ROW_WARPS, ROW_KEYS, 2>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+  HX_CHECK_LAUNCH("hx_tree_attention");
+  return HX_OK;
+}
+
+// Floats of scratch that hx_tree_attention needs for these sizes, whatever the step brings; negative:
+// there is no kernel for them.
+HX_API long long hx_tree_attention_scratch_floats(int dtype, int heads, int kv_heads, int head_dim,
+                                                  int page_size) {
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 || head_dim % 2 != 0 ||
+      head_dim > ROW_MAX_DIM || page_size <= 0 || (dtype != HX_F32 && dtype != HX_BF16))
+    return -1;
+  const int sms = hx_device_sm_count();
+  if (sms <= 0) return -1;
+  switch (kernel_for(dtype, head_dim, page_size)) {
+    case TREE_TC: return hx_tree_tc_floats(head_dim);
+    case TREE_TILE: return 2ll * sms * tile_ctas_an_sm(head_dim) * tree_part_floats<TILE_ROWS>(head_dim);
+    default: return 2ll * sms * ROW_CTAS * tree_part_floats<ROW_WARPS>(head_dim);
+  }
+}
+
+// out[t, h D .. (h + 1) D) for every token t of the requests; see the head of this file.  visible:
+// [tokens, ld_visible] of 64-bit words, `words` of them a token, bit j of word w: the token sees
+// drafted token 64 w + j of its request.  partial: hx_tree_attention_scratch_floats() floats.  Rows of
+// `out` behind request_start[requests] are left as they are.
+HX_API int hx_tree_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int dtype,
+                             const long long* visible, int ld_visible, int words,
+                             const int* request_start, const int* request_context,
+                             const int* request_table_row, const int* block_tables, int table_stride,
+                             void* out, int ldo, float* partial, int requests, int heads, int kv_heads,
+                             int head_dim, int page_size, int num_pages, float scale, int* status,
+                             cudaStream_t stream) {
+  HX_REQUIRE(dtype == HX_F32 || dtype == HX_BF16, "hx_tree_attention: unknown dtype %d", dtype);
+  HX_REQUIRE(requests >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && page_size > 0,
+             "hx_tree_attention: bad sizes");
+  HX_REQUIRE(head_dim > 0 && head_dim % 2 == 0 && head_dim <= ROW_MAX_DIM,
+             "hx_tree_attention: head_dim %d (even, at most %d)", head_dim, ROW_MAX_DIM);
+  HX_REQUIRE(words > 0 && ld_visible >= words, "hx_tree_attention: a token has at least one word of 64 bits");
+  HX_REQUIRE(num_pages > 0 && table_stride > 0 && static_cast<long long>(num_pages) * kv_heads < (1ll << 31),
+             "hx_tree_attention: bad cache geometry");
+  HX_REQUIRE(scale > 0.0f, "hx_tree_attention: the scale must be positive");
+  HX_REQUIRE(status != nullptr && partial != nullptr, "hx_tree_attention: status word or scratch missing");
+  const int size = dtype == HX_BF16 ? 2 : 4;
+  const int piece = hx_cache_chunk(size, head_dim) * size;      // bytes the cache is read in
+  auto aligned = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; };
+  HX_REQUIRE(aligned(k_cache, piece) && aligned(v_cache, piece) && aligned(partial, 16) && aligned(visible, 8),
+             "hx_tree_attention: cache, scratch or masks are not aligned");
+  if (requests == 0) return HX_OK;
+  TreeArgs a{q, ldq, k_cache, v_cache, visible, ld_visible, words, request_start, request_context,
+             request_table_row, block_tables, table_stride, out, ldo, partial, requests, heads, kv_heads,
+             head_dim, page_size, num_pages, scale, status, 1, 1, 1};
+  const TreeKernel kernel = kernel_for(dtype, head_dim, page_size);
+  const int sms = hx_device_sm_count();
+  HX_REQUIRE(sms > 0, "hx_tree_attention: the device cannot be asked");
+  if (kernel == TREE_TC) {
+    HX_REQUIRE(ldq % 8 == 0 && ldo % 8 == 0 && aligned(q, 16) && aligned(out, 16),
+               "hx_tree_attention: q and out must be 16-byte aligned, row strides multiples of 8");
+    return hx_tree_tc_launch(a, stream);
+  }
+  if (kernel == TREE_TILE) {
+    HX_REQUIRE(ldq % 4 == 0 && aligned(q, 4 * size), "hx_tree_attention: q must be aligned to four elements");
+    tree_fill_rows(a, TILE_ROWS);
+    const int ctas = sms * tile_ctas_an_sm(head_dim);
+    int rc;
+    if (dtype == HX_BF16)
+      rc = head_dim <= 128 ? launch_tile<__nv_bfloat16, 128>(a, ctas, stream)
+                           : launch_tile<__nv_bfloat16, 256>(a, ctas, stream);
+    else
+      rc = head_dim <= 128 ? launch_tile<float, 128>(a, ctas, stream) : launch_tile<float, 256>(a, ctas, stream);
+    if (rc != HX_OK) return rc;
+    return hx_tree_join(a, dtype, ctas, TILE_LEAST, TILE_ROWS, TILE_KEYS, 4, stream);
+  }
+  tree_fill_rows(a, ROW_WARPS);
+  const int ctas = sms * ROW_CTAS;
+  if (dtype == HX_BF16) hx_launch(tree_row_kernel<__nv_bfloat16>, ctas, ROW_WARPS * 32, 0, stream, a);
+  else hx_launch(tree_row_kernel<float>, ctas, ROW_WARPS * 32, 0, stream, a);
+  HX_CHECK_LAUNCH("hx_tree_attention");
+  return hx_tree_join(a, dtype, ctas, ROW_LEAST, ROW_WARPS, ROW_KEYS, 2, stream);
+}

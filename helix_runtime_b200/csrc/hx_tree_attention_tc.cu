@@ -1,0 +1,663 @@
+// Tree attention on the 5th-generation tensor cores (tcgen05), bfloat16 storage; what it computes and
+// how the work is cut into runs is told in hx_tree_attention.cu and hx_tree_attention.cuh.
+//
+// A tile of 128 rows (the M of a product) holds the drafted tokens of a request, each with the
+// query heads of one key/value head; the item walks its keys 64 at a time.  Warp roles:
+//   warp 0      asks for keys and values: values a whole (page, head) block a copy, keys piece by
+//               piece (16 bytes of all slots of a page), two copies a lane, which lays them out as
+//               [piece][64 keys][16 bytes] whatever the page size: one stride from 8 keys to the
+//               next, so that one product covers the tile;
+//   warp 1      one lane issues S = Q K^T into one of two score buffers in tensor memory;
+//   warp 2      one lane issues O += P V;
+//   warp 3      loads the queries of an item, as soon as the item before has read its own;
+//   warps 4-7   softmax: thread r owns row r.  P goes back over the scores as two bfloat16 terms
+//               (P = hi + lo, 16 bits of each probability, so that the softmax stays a float32
+//               quantity as far as the result can tell); the reference of the exponentials is
+//               raised when a tile exceeds it by more than 2^8, O stays in tensor memory.
+// Keys and values keep flowing across items: the rings go by TURNS, the key tiles of the CTA's run in
+// order.  Two CTAs share an SM and fill each other's gaps.
+//
+// Masks matter in the tiles that hold drafted keys, the last one or two of an item.  There values
+// are looked at, too: a drafted value that is not finite would reach rows that do not see it (0 x
+// infinity), so it is taken as zero in the product and added, as what it is, to the rows that do see it.
+//
+// Every wait is bounded; a wait that runs out sets a status bit, the CTA lets its copies land, frees its
+// tensor memory and returns.
+#include "hx_tcgen05.cuh"
+#include "hx_tree_attention.cuh"
+
+#include <mutex>
+
+namespace {
+
+constexpr int BLOCK_M = 128, BLOCK_N = 64;
+constexpr int WARP_PAGES = 0, WARP_SCORES = 1, WARP_OUTPUT = 2, WARP_QUERIES = 3;      // and 4 to 7: softmax
+constexpr int THREADS = 256;
+constexpr int GROUP_STRIDE = 128;             // bytes from one 8-row core matrix to the next row group
+constexpr int CHUNK_STRIDE = BLOCK_M * 16;    // bytes from one 16-byte column of Q to the next
+constexpr int KEY_STRIDE = BLOCK_N * 16;      // ... and of the keys
+constexpr float RAISE_MAXIMUM_BY = 8.0f;      // log2 units a tile must exceed a row's reference by
+constexpr int CTAS_AN_SM = 2;
+constexpr int LEAST = 2;                      // key tiles of the shortest run
+
+template <int D>
+struct TreeTcConfig {
+  static constexpr int kKeyStages = 3, kValueStages = 2;
+  static constexpr int kQBytes = BLOCK_M * D * 2;
+  static constexpr int kHalfBytes = BLOCK_N * D * 2;          // keys (or values) of a tile
+  static constexpr int kBarrierBytes = 256;
+  static constexpr int kSmemBytes = kQBytes + (kKeyStages + kValueStages) * kHalfBytes + 128 + kBarrierBytes;
+  static constexpr int kLowTermColumn = BLOCK_N / 2;          // P: hi in columns [0, 32), lo after
+  static constexpr int kOutputColumn = 2 * BLOCK_N;
+  static constexpr int kTmemColumns = 256;
+  static_assert(2 * BLOCK_N + D <= kTmemColumns, "tensor memory of a CTA");
+  static_assert(CTAS_AN_SM * (kSmemBytes + 1024) <= 228 * 1024, "an SM has 228 KB of shared memory");
+};
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two float32 operations in one instruction, and the largest of three: the softmax is bound by the
+// instructions it issues.
+__device__ __forceinline__ uint64_t pair_of(float low, float high) {
+  uint64_t pair;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(pair) : "f"(low), "f"(high));
+  return pair;
+}
+__device__ __forceinline__ void halves_of(uint64_t pair, float& low, float& high) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(low), "=f"(high) : "l"(pair));
+}
+__device__ __forceinline__ uint64_t pair_fma(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ float max_of_3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
+  const __nv_bfloat162 pair = __floats2bfloat162_rn(low, high);
+  return *reinterpret_cast<const uint32_t*>(&pair);
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+      ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+// A bfloat16 whose exponent is all ones: an infinity or not a number.
+__device__ __forceinline__ bool not_finite(uint32_t bits16) { return (bits16 & 0x7f80u) == 0x7f80u; }
+
+// What is not finite among the drafted values that a row sees in the segment [c.tile, c.tile + count) is
+// added to the row as stored: whatever their weight, the sum is not finite either.
+template <int D>
+__device__ __noinline__ void add_not_finite(const TreeArgs& a, const TreeCursor& c, int count, int token, int row,
+                                            __nv_bfloat16* out, float* part) {
+  const int first = max(c.context, c.tile * BLOCK_N);
+  const int end = min(c.context + c.nodes, (c.tile + count) * BLOCK_N);
+  const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v_cache);
+  for (int key = first; key < end; ++key) {
+    if (!(tree_mask(a, c, token, key / BLOCK_N * BLOCK_N) >> (key % BLOCK_N) & 1)) continue;
+    const int index = key / a.page_size;
+    if (index >= a.table_stride) continue;
+    const int page = a.block_tables[static_cast<size_t>(a.request_table_row[c.request]) * a.table_stride + index];
+    if (page < 0 || page >= a.num_pages) continue;
+    for (int d = 0; d < D; ++d) {
+      const float x = __bfloat162float(v[hx_cache_offset(page, c.kv_head(a), key % a.page_size, d, a.kv_heads,
+                                                         a.page_size, D, 8)]);
+      if (isfinite(x)) continue;
+      if (out != nullptr) out[d] = __float2bfloat16_rn(__bfloat162float(out[d]) + x);
+      else part[(static_cast<size_t>(d / 4) * BLOCK_M + row) * 4 + d % 4] += x;
+    }
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(const TreeArgs a) {
+  using Config = TreeTcConfig<D>;
+  constexpr int K_STAGES = Config::kKeyStages, V_STAGES = Config::kValueStages;
+  constexpr int PIECES = D / 8;
+  hx_pdl_trigger();
+
+  // the run is found from the step's description, which was there before the kernel in front
+  const TreeRun run = tree_run<BLOCK_N>(a, blockIdx.x, gridDim.x, LEAST);
+  if (run.count == 0) {      // before any barrier or allocation: the whole CTA leaves
+    hx_pdl_wait();
+    return;
+  }
+  TreeCursor at;
+  long long item_begin;
+  tree_locate<BLOCK_N>(a, run.begin, at, item_begin);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  uint8_t* q_tile = smem;
+  uint8_t* k_stages = q_tile + Config::kQBytes;
+  uint8_t* v_stages = k_stages + K_STAGES * Config::kHalfBytes;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(v_stages + V_STAGES * Config::kHalfBytes);
+  uint64_t* k_done = k_full + K_STAGES;        // its scores have read them
+  uint64_t* v_full = k_done + K_STAGES;
+  uint64_t* v_done = v_full + V_STAGES;
+  uint64_t* s_full = v_done + V_STAGES;        // [2] scores of turn t in buffer t % 2
+  uint64_t* p_full = s_full + 2;               // [2] its probabilities are in place
+  uint64_t* o_full = p_full + 2;               // [2] its output product is done
+  uint64_t* q_ready = o_full + 2;              // the queries of a segment are in shared memory
+  uint64_t* q_done = q_ready + 1;              // the last score product of a segment has read them
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_done + 1);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  volatile int* poisoned = failed + 1;         // the last segment with a drafted value that is not finite
+  static_assert((2 * K_STAGES + 2 * V_STAGES + 8) * 8 + 12 <= Config::kBarrierBytes, "the place of barriers and flags");
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int page_size = a.page_size;
+  const int pages_per_tile = BLOCK_N / page_size;
+  const uint32_t page_bytes = static_cast<uint32_t>(page_size) * D * 2;
+  const uint32_t piece_stride = static_cast<uint32_t>(page_size) * 16;   // next 16-byte piece of a key
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < K_STAGES; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_done[s], 1);
+    }
+    for (int s = 0; s < V_STAGES; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_done[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&s_full[b], 1);
+      mbar_init(&p_full[b], 4);   // one arrival per softmax warp
+      mbar_init(&o_full[b], 1);
+    }
+    mbar_init(q_ready, 1);
+    mbar_init(q_done, 1);
+    *failed = 0;
+    *poisoned = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == WARP_SCORES) tmem_alloc(tmem_holder, Config::kTmemColumns);
+  hx_pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+
+  // One lane waits and looks at the failure flag, all lanes get the same answer.
+  auto wait_for = [&](uint64_t* bar, uint32_t parity) {
+    int state = 0;      // 0: go on, 1: this wait ran out, 2: somebody else failed
+    if (lane == 0) state = *failed ? 2 : (mbar_wait(bar, parity & 1u) ? 0 : 1);
+    state = __shfl_sync(0xffffffffu, state, 0);
+    if (state == 1 && lane == 0) {
+      atomicOr(a.status, HX_FLAG_WAIT_TIMEOUT);
+      *failed = 1;
+    }
+    return state == 0;
+  };
+
+  if (warp == WARP_PAGES) {
+    // ------------------------------------------------------------ page requests
+    // Turn t asks for the keys of turn t and for the values of turn t - 1, which are wanted later.
+    // Lane p < pages_per_tile holds the block (of bytes into the layer's cache) of the turn's page p,
+    // -1 where there is none.
+    TreeCursor c = at;
+    int asked = 0;                      // key tiles whose values' copies are on their way
+    int keys_asked = 0;
+    auto block_of = [&]() {
+      long long block = -1;
+      if (lane < pages_per_tile) {
+        const int index = c.tile * pages_per_tile + lane;
+        if (index * page_size < c.context + c.nodes) {
+          const int page = index < a.table_stride
+                               ? a.block_tables[static_cast<size_t>(a.request_table_row[c.request]) * a.table_stride + index]
+                               : -1;
+          if (page >= 0 && page < a.num_pages)
+            block = (static_cast<long long>(page) * a.kv_heads + c.kv_head(a)) * page_bytes;
+          else
+            atomicOr(a.status, HX_FLAG_BAD_PAGE);
+        }
+      }
+      return block;
+    };
+    long long block = block_of(), value_block = -1;
+    const uint8_t* k_cache = static_cast<const uint8_t*>(a.k_cache);
+    const uint8_t* v_cache = static_cast<const uint8_t*>(a.v_cache);
+    for (int turn = 0; turn <= run.count; ++turn) {
+      long long next_block = -1;
+      if (turn + 1 < run.count) {      // the next turn's pages, in flight during the waits
+        if (++c.tile == c.tiles) tree_next_item<BLOCK_N>(a, c);
+        next_block = block_of();
+      }
+      if (turn < run.count) {
+        const int stage = turn % K_STAGES;
+        if (!wait_for(&k_done[stage], static_cast<uint32_t>(turn / K_STAGES) + 1u)) break;
+        const unsigned there = __ballot_sync(0xffffffffu, block >= 0);
+        if (lane == 0) mbar_expect_tx(&k_full[stage], __popc(there) * page_bytes);
+        __syncwarp();
+        const uint32_t target = smem_u32(k_stages + stage * Config::kHalfBytes);
+        if (page_size == BLOCK_N) {      // a page's block is laid out as the product wants it
+          if (lane == 0 && there != 0u) bulk_copy(target, k_cache + block, page_bytes, &k_full[stage]);
+        } else {                         // (2 or 4 pages: a lane's copies are all of one page)
+          const int p = lane % pages_per_tile;
+          const long long from = __shfl_sync(0xffffffffu, block, p);
+          for (int piece = lane / pages_per_tile; piece < PIECES && from >= 0; piece += 32 / pages_per_tile)
+            bulk_copy(target + piece * KEY_STRIDE + p * piece_stride, k_cache + from + piece * piece_stride,
+                      piece_stride, &k_full[stage]);
+          __syncwarp();
+        }
+        ++keys_asked;
+      }
+      if (turn > 0) {
+        const int stage = (turn - 1) % V_STAGES;
+        if (!wait_for(&v_done[stage], static_cast<uint32_t>((turn - 1) / V_STAGES) + 1u)) break;
+        const unsigned there = __ballot_sync(0xffffffffu, value_block >= 0);
+        if (lane == 0) mbar_expect_tx(&v_full[stage], __popc(there) * page_bytes);
+        __syncwarp();
+        if (value_block >= 0)
+          bulk_copy(smem_u32(v_stages + stage * Config::kHalfBytes) + lane * page_bytes, v_cache + value_block,
+                    page_bytes, &v_full[stage]);
+        ++asked;
+      }
+      value_block = block;
+      block = next_block;
+    }
+    // a CTA does not leave while copies into its shared memory are in flight
+    if (*failed) {
+      for (int t = max(0, keys_asked - K_STAGES); t < keys_asked; ++t)
+        if (lane == 0) mbar_wait(&k_full[t % K_STAGES], static_cast<uint32_t>(t / K_STAGES) & 1u);
+      for (int t = max(0, asked - V_STAGES); t < asked; ++t)
+        if (lane == 0) mbar_wait(&v_full[t % V_STAGES], static_cast<uint32_t>(t / V_STAGES) & 1u);
+      __syncwarp();
+    }
+  } else if (warp == WARP_QUERIES) {
+    // ------------------------------------------------------------------ queries
+    // [D / 8 pieces][16 row groups][8 rows][16 bytes]; rows behind the last keep what lay there (a row's
+    // scores concern no other row)
+    // (q_done has a phase a segment: a barrier that completes one a turn would have to be waited for
+    // turn by turn, a parity says nothing about phases further back)
+    TreeCursor c = at;
+    int segment = 0;
+    for (int left = run.count; left > 0; ++segment) {
+      const int count = min(c.tiles - c.tile, left);
+      if (segment > 0 && !wait_for(q_done, static_cast<uint32_t>(segment - 1))) break;
+      const TreeRows rows(a, c);
+      const int rows_here = rows.count;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
+                               static_cast<size_t>(c.q_begin + rows.token0) * a.ldq + static_cast<size_t>(rows.head0) * D;
+      // neighbouring lanes take eight rows' same piece; eight loads of a lane are in flight
+      constexpr int LOADS = 8;
+      const int items = (rows_here + 7) / 8 * PIECES * 8;
+      for (int base = 0; base < items; base += 32 * LOADS) {
+        uint4 value[LOADS];
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+          const int i = base + u * 32 + lane;
+          const int block = i >> 3, row_group = block / PIECES, piece = block - row_group * PIECES;
+          const int row = row_group * 8 + (i & 7);
+          value[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (i < items && row < rows_here) {
+            const int token = row / rows.heads;
+            value[u] = *reinterpret_cast<const uint4*>(q + static_cast<size_t>(token) * a.ldq +
+                                                       static_cast<size_t>(row - token * rows.heads) * D + piece * 8);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+          const int i = base + u * 32 + lane;
+          const int block = i >> 3, row_group = block / PIECES, piece = block - row_group * PIECES;
+          if (i < items)
+            *reinterpret_cast<uint4*>(q_tile + piece * CHUNK_STRIDE + row_group * GROUP_STRIDE + (i & 7) * 16) = value[u];
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+      left -= count;
+      if (left > 0) tree_next_item<BLOCK_N>(a, c);
+    }
+  } else if (warp == WARP_SCORES) {
+    // ------------------------------------------------------------ score products
+    if (hx_elect_one()) {
+      constexpr uint32_t idesc = make_idesc(BLOCK_M, BLOCK_N);
+      const uint64_t desc_q = make_smem_desc_plain(smem_u32(q_tile), CHUNK_STRIDE, GROUP_STRIDE);
+      const uint64_t desc_k0 = make_smem_desc_plain(smem_u32(k_stages), KEY_STRIDE, GROUP_STRIDE);
+      TreeCursor c = at;
+      int turn = 0, segment = 0;
+      for (int left = run.count; left > 0 && !*failed; ++segment) {
+        const int count = min(c.tiles - c.tile, left);
+        bool ok = mbar_wait(q_ready, static_cast<uint32_t>(segment) & 1u);
+        for (int t = 0; t < count && ok && !*failed; ++t, ++turn) {
+          const int b = turn & 1, stage = turn % K_STAGES;
+          // (the buffer held the probabilities of two turns ago, which the output product must have read)
+          ok = mbar_wait(&k_full[stage], static_cast<uint32_t>(turn / K_STAGES) & 1u) &&
+               (turn < 2 || mbar_wait(&o_full[b], static_cast<uint32_t>(turn / 2 - 1) & 1u));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t desc_k = desc_k0 + stage * (Config::kHalfBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem_base + b * BLOCK_N, desc_q + k * ((2 * CHUNK_STRIDE) >> 4),
+                      desc_k + k * ((2 * KEY_STRIDE) >> 4), idesc, k > 0 ? 1u : 0u);
+          umma_commit(&s_full[b]);
+          umma_commit(&k_done[stage]);
+          if (t == count - 1) umma_commit(q_done);
+        }
+        if (!ok) {
+          atomicOr(a.status, HX_FLAG_WAIT_TIMEOUT);
+          *failed = 1;
+        }
+        left -= count;
+        if (left > 0) tree_next_item<BLOCK_N>(a, c);
+      }
+    }
+  } else if (warp == WARP_OUTPUT) {
+    // ----------------------------------------------------------- output products
+    if (hx_elect_one()) {
+      constexpr uint32_t idesc = make_idesc_b_mn_major(BLOCK_M, D);
+      // values: MN-major, the next 8 keys are 128 bytes on, the next 8 coordinates one piece on
+      const uint64_t desc_v0 = make_smem_desc_plain(smem_u32(v_stages), GROUP_STRIDE, piece_stride);
+      uint32_t value_step[BLOCK_N / 16];
+#pragma unroll
+      for (int g = 0; g < BLOCK_N / 16; ++g)
+        value_step[g] = ((g * 16 / page_size) * page_bytes + (g * 16 % page_size) * 16) >> 4;
+      const uint32_t target = tmem_base + Config::kOutputColumn;
+      TreeCursor c = at;
+      int turn = 0;
+      for (int left = run.count; left > 0 && !*failed;) {
+        const int count = min(c.tiles - c.tile, left);
+        for (int t = 0; t < count && !*failed; ++t, ++turn) {
+          const int b = turn & 1, stage = turn % V_STAGES;
+          // (the first probabilities of a segment come when the rows of the one before have left)
+          if (!mbar_wait(&p_full[b], static_cast<uint32_t>(turn / 2) & 1u) ||
+              !mbar_wait(&v_full[stage], static_cast<uint32_t>(turn / V_STAGES) & 1u)) {
+            atomicOr(a.status, HX_FLAG_WAIT_TIMEOUT);
+            *failed = 1;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t desc_v = desc_v0 + stage * (Config::kHalfBytes >> 4);
+          const uint32_t p_hi = tmem_base + b * BLOCK_N, p_lo = p_hi + Config::kLowTermColumn;
+#pragma unroll
+          for (int g = 0; g < BLOCK_N / 16; ++g) {
+            umma_bf16_a_tmem(target, p_hi + g * 8, desc_v + value_step[g], idesc, (t > 0 || g > 0) ? 1u : 0u);
+            umma_bf16_a_tmem(target, p_lo + g * 8, desc_v + value_step[g], idesc, 1u);
+          }
+          umma_commit(&v_done[stage]);
+          umma_commit(&o_full[b]);
+        }
+        left -= count;
+        if (left > 0) tree_next_item<BLOCK_N>(a, c);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    const int quarter = warp & 3;      // tensor-memory lanes [32 * quarter, 32 * quarter + 32)
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t output_base = lane_base + Config::kOutputColumn;
+    const float scale_log2 = a.scale * HX_LOG2E;      // positive: it does not change which score is largest
+    const uint64_t factor_pair = pair_of(scale_log2, scale_log2), minus_one = pair_of(-1.0f, -1.0f);
+    TreeCursor c = at;
+    int turn = 0, segment = 0;
+    bool ok = true;
+    for (int left = run.count; left > 0 && ok; ++segment) {
+      const int count = min(c.tiles - c.tile, left);
+      const TreeRows rows(a, c);
+      const int rows_here = rows.count;
+      const int my_token = rows.token0 + min(row, rows_here - 1) / rows.heads;      // (rows behind the last: any)
+      const int my_head = rows.head0 + row % rows.heads;
+      const bool live = quarter * 32 < rows_here;                         // the warp has rows
+      const int last_key = c.context + c.nodes - 1;
+      float row_max = -INFINITY;      // the reference of this row's exponentials, in log2 units
+      float row_sum = 0.0f;
+      for (int t = 0; t < count && ok; ++t, ++turn) {
+        const int b = turn & 1;
+        ok = wait_for(&s_full[b], static_cast<uint32_t>(turn / 2));
+        if (!ok) break;
+        const int key0 = (c.tile + t) * BLOCK_N;
+        const bool drafted = key0 + BLOCK_N > c.context;
+        if (live) {
+          tc_fence_after();
+          const uint32_t score_base = lane_base + b * BLOCK_N;
+          float p[BLOCK_N];
+          {
+            uint32_t r[4][16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_load16_issue(score_base + i * 16, r[i]);
+            tmem_load_wait();
+#pragma unroll
+            for (int i = 0; i < BLOCK_N; ++i) p[i] = __uint_as_float(r[i / 16][i % 16]);
+          }
+          if (drafted) {
+            const unsigned long long mask = tree_mask(a, c, my_token, key0);
+            const uint32_t low = static_cast<uint32_t>(mask), high = static_cast<uint32_t>(mask >> 32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (!((low >> i) & 1)) p[i] = -INFINITY;
+              if (!((high >> i) & 1)) p[i + 32] = -INFINITY;
+            }
+          }
+          float part_max[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) part_max[u] = max_of_3(p[u], p[u + 4], p[u + 8]);
+#pragma unroll
+          for (int i = 12; i + 8 <= BLOCK_N; i += 8)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) part_max[u] = max_of_3(part_max[u], p[i + u], p[i + 4 + u]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) part_max[u] = fmaxf(part_max[u], p[BLOCK_N - 4 + u]);
+          const float tile_max = scale_log2 * fmaxf(max_of_3(part_max[0], part_max[1], part_max[2]), part_max[3]);
+          // a row that has seen nothing yet keeps -inf as its reference and zeros as its probabilities
+          const float old_max = row_max;
+          // (each row by itself, so that what another row sees does not reach this one, not even by rounding)
+          const bool exceeds = row < rows_here && tile_max > old_max + RAISE_MAXIMUM_BY;
+          const bool raised = t > 0 && __any_sync(0xffffffffu, exceeds);
+          if (t == 0 || exceeds) row_max = tile_max;
+          if (raised) {
+            // what O holds was taken against the old reference; the product of the last turn must have landed
+            const float correction = !exceeds ? 1.0f : old_max == -INFINITY ? 0.0f : fast_exp2(old_max - row_max);
+            row_sum *= correction;
+            ok = wait_for(&o_full[(turn - 1) & 1], static_cast<uint32_t>((turn - 1) / 2));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int d0 = 0; d0 < D; d0 += 32) {
+              const bool both = d0 + 16 < D;
+              uint32_t r0[16], r1[16];
+              tmem_load16_issue(output_base + d0, r0);
+              if (both) tmem_load16_issue(output_base + d0 + 16, r1);
+              tmem_load_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                r0[i] = __float_as_uint(__uint_as_float(r0[i]) * correction);
+                if (both) r1[i] = __float_as_uint(__uint_as_float(r1[i]) * correction);
+              }
+              tmem_store16_raw(output_base + d0, r0);
+              if (both) tmem_store16_raw(output_base + d0 + 16, r1);
+            }
+          }
+          uint64_t part_sum[4] = {0, 0, 0, 0};
+          const float reference = row_max == -INFINITY ? 0.0f : row_max;
+          const uint64_t reference_pair = pair_of(-reference, -reference);
+#pragma unroll
+          for (int i = 0; i < BLOCK_N; i += 2) {
+            float x0, x1;
+            halves_of(pair_fma(pair_of(p[i], p[i + 1]), factor_pair, reference_pair), x0, x1);
+            p[i] = fast_exp2(x0);
+            p[i + 1] = fast_exp2(x1);
+            part_sum[(i / 2) % 4] = pair_add(part_sum[(i / 2) % 4], pair_of(p[i], p[i + 1]));
+          }
+          {
+            float low, high;
+            halves_of(pair_add(pair_add(part_sum[0], part_sum[1]), pair_add(part_sum[2], part_sum[3])), low, high);
+            row_sum += low + high;
+          }
+          // P = hi + lo over the scores just read, two keys per column, the earlier key in the lower half
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float p0 = p[half * 32 + 2 * i], p1 = p[half * 32 + 2 * i + 1];
+              hi[i] = pack_bf16(p0, p1);
+              float rest0, rest1;
+              halves_of(pair_fma(pair_of(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)),
+                                 minus_one, pair_of(p0, p1)), rest0, rest1);
+              lo[i] = pack_bf16(rest0, rest1);
+            }
+            tmem_store16_raw(score_base + half * 16, hi);
+            tmem_store16_raw(score_base + Config::kLowTermColumn + half * 16, lo);
+          }
+          tmem_store_wait();
+        }
+        if (drafted) {
+          // values behind the last key (whatever an earlier tile left there) and drafted values that
+          // are not finite become zeros
+          ok = wait_for(&v_full[turn % V_STAGES], static_cast<uint32_t>(turn / V_STAGES));
+          if (!ok) break;
+          uint8_t* v_half = v_stages + (turn % V_STAGES) * Config::kHalfBytes;
+          const int first_stale = last_key + 1 - key0, first_drafted = max(c.context - key0, 0);
+          bool found = false;
+          for (int i = row; i < BLOCK_N * PIECES; i += 128) {
+            const int piece = i / BLOCK_N, key = i - piece * BLOCK_N;
+            if (key < first_drafted) continue;
+            uint4* place = reinterpret_cast<uint4*>(v_half + (key / page_size) * page_bytes +
+                                                    (piece * page_size + key % page_size) * 16);
+            if (key >= first_stale) {
+              *place = make_uint4(0u, 0u, 0u, 0u);
+              continue;
+            }
+            uint4 value = *place;
+            uint32_t* halves = reinterpret_cast<uint32_t*>(&value);
+            bool bad = false;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              if (not_finite(halves[h])) { halves[h] &= 0xffff0000u; bad = true; }
+              if (not_finite(halves[h] >> 16)) { halves[h] &= 0x0000ffffu; bad = true; }
+            }
+            if (bad) {
+              *place = value;
+              found = true;
+            }
+          }
+          if (found) *poisoned = segment;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[b]);
+      }
+      if (!ok) break;
+
+      // ---- the segment's rows: finished, or this CTA's part of them
+      ok = wait_for(&o_full[(turn - 1) & 1], static_cast<uint32_t>((turn - 1) / 2));
+      if (!ok) break;
+      if (live) {
+        tc_fence_after();
+        const bool whole = c.tile == 0 && count == c.tiles;
+        const float inverse = row_sum > 0.0f ? 1.0f / row_sum : 0.0f;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(c.q_begin + my_token) * a.ldo +
+                             static_cast<size_t>(my_head) * D;
+        float* part = a.partial + (2ll * blockIdx.x + (c.tile == 0 ? 1 : 0)) * tree_part_floats<BLOCK_M>(D);
+#pragma unroll
+        for (int d0 = 0; d0 < D; d0 += 16) {
+          float o[16];
+          __syncwarp();
+          tmem_load16(output_base + d0, o);
+          if (row < rows_here) {
+            if (row_max == -INFINITY) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+            }
+            if (whole) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint4 packed;
+                packed.x = pack_bf16(o[8 * h] * inverse, o[8 * h + 1] * inverse);
+                packed.y = pack_bf16(o[8 * h + 2] * inverse, o[8 * h + 3] * inverse);
+                packed.z = pack_bf16(o[8 * h + 4] * inverse, o[8 * h + 5] * inverse);
+                packed.w = pack_bf16(o[8 * h + 6] * inverse, o[8 * h + 7] * inverse);
+                *reinterpret_cast<uint4*>(out + d0 + 8 * h) = packed;
+              }
+            } else {
+#pragma unroll
+              for (int h = 0; h < 4; ++h)
+                *reinterpret_cast<float4*>(part + (static_cast<size_t>(d0 / 4 + h) * BLOCK_M + row) * 4) =
+                    make_float4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
+            }
+          }
+        }
+        if (!whole && row < rows_here) {
+          part[static_cast<size_t>(D) * BLOCK_M + row] = row_max;
+          part[static_cast<size_t>(D + 1) * BLOCK_M + row] = row_sum;
+        }
+        // (told before the arrivals that the last output product waited for)
+        if (*poisoned == segment && row < rows_here)
+          add_not_finite<D>(a, c, count, my_token, row, whole ? out : nullptr, whole ? nullptr : part);
+        tc_fence_before();
+      }
+      left -= count;
+      if (left > 0) tree_next_item<BLOCK_N>(a, c);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == WARP_SCORES) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Config::kTmemColumns);
+  }
+}
+
+template <int D>
+int launch(const TreeArgs& a, int ctas, cudaStream_t stream) {
+  using Config = TreeTcConfig<D>;
+  static std::once_flag once;
+  static bool reserved = false;
+  std::call_once(once, [] {
+    reserved = cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    Config::kSmemBytes) == cudaSuccess;
+    if (!reserved) cudaGetLastError();
+  });
+  HX_REQUIRE(reserved, "hx_tree_attention: cannot reserve %d bytes of shared memory", Config::kSmemBytes);
+  hx_launch(tree_attention_tc_kernel<D>, ctas, THREADS, Config::kSmemBytes, stream, a);
+  HX_CHECK_LAUNCH("hx_tree_attention");
+  return HX_OK;
+}
+
+}  // namespace
+
+bool hx_tree_tc_takes(int head_dim, int page_size) {
+  return head_dim >= 64 && head_dim <= 128 && head_dim % 16 == 0 &&
+         (page_size == 16 || page_size == 32 || page_size == 64);
+}
+
+long long hx_tree_tc_floats(int head_dim) {
+  return 2ll * hx_device_sm_count() * CTAS_AN_SM * tree_part_floats<BLOCK_M>(head_dim);
+}
+
+int hx_tree_tc_launch(TreeArgs a, cudaStream_t stream) {
+  tree_fill_rows(a, BLOCK_M);
+  const int ctas = hx_device_sm_count() * CTAS_AN_SM;
+  int rc;
+  switch (a.head_dim) {
+    case 64: rc = launch<64>(a, ctas, stream); break;
+    case 80: rc = launch<80>(a, ctas, stream); break;
+    case 96: rc = launch<96>(a, ctas, stream); break;
+    case 112: rc = launch<112>(a, ctas, stream); break;
+    default: rc = launch<128>(a, ctas, stream); break;
+  }
+  if (rc != HX_OK) return rc;
+  return hx_tree_join(a, HX_BF16, ctas, LEAST, BLOCK_M, BLOCK_N, 4, stream);
+}

@@ -24,6 +24,27 @@ from ..ops import library as ops
 from ..parts.base import StepContext, Workspace
 
 
+def ancestor_words(parents: Sequence[int], words: int = 0) -> np.ndarray:
+    """The masks of a tree of drafted tokens (``parents``: each one's number, smaller than its
+    child's; -1 for token 0), int64 ``[tokens, words]`` as
+    :func:`helix_runtime_b200.ops.library.tree_attention` reads them: bit ``j`` of word ``w`` of a
+    token's row is set where token ``64 w + j`` is itself or an ancestor.  ``words`` 0: as many as
+    the tokens need."""
+    count = len(parents)
+    words = words or max(1, -(-count // 64))
+    if count > 64 * words:
+        raise ValueError(f"{count} tokens need {-(-count // 64)} words of 64 bits")
+    masks = np.zeros((count, words), dtype=np.uint64)
+    for token, parent in enumerate(parents):
+        if not (parent == -1 if token == 0 else 0 <= parent < token):
+            raise ValueError(f"token {token} of a tree has the parent {parent}: token 0 has -1, every "
+                             "other one that comes before it")
+        if token:
+            masks[token] = masks[parent]
+        masks[token, token // 64] |= np.uint64(1) << np.uint64(token % 64)
+    return masks.view(np.int64)
+
+
 @dataclasses.dataclass
 class StepEntry:
     request: Hashable
@@ -238,7 +259,9 @@ class StepFunction:
                                         (ops.FLAG_WAIT_TIMEOUT, "a bounded kernel wait ran out"),
                                         (ops.FLAG_NONFINITE, "non-finite logits"),
                                         (ops.FLAG_BAD_POSITION,
-                                         "a position outside the position table"))
+                                         "a position outside the position table"),
+                                        (ops.FLAG_BAD_MOVE,
+                                         "a move in the cache over what another needs"))
                  if flags & bit]
         return "the step's kernels reported: " + "; ".join(names)
 

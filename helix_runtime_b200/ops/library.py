@@ -36,6 +36,7 @@ FLAG_BAD_PAGE = 2
 FLAG_WAIT_TIMEOUT = 4
 FLAG_NONFINITE = 8
 FLAG_BAD_POSITION = 16
+FLAG_BAD_MOVE = 32
 
 _c_int = ctypes.c_int
 _c_ptr = ctypes.c_void_p
@@ -387,6 +388,24 @@ def _declare(library: ctypes.CDLL) -> None:
                  "hx_matrix_lstm_state_floats", "hx_matrix_lstm_gates", "hx_matrix_lstm",
                  "hx_state_chunks_supports", "hx_state_chunks"):
         getattr(library, name).restype = _c_int
+    library.hx_tree_attention_scratch_floats.argtypes = [_c_int] * 5
+    library.hx_tree_attention_scratch_floats.restype = _c_longlong
+    library.hx_tree_attention.argtypes = [
+        _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+        _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr,
+        _c_ptr]
+    library.hx_tree_attention.restype = _c_int
+    library.hx_copy_pages.argtypes = [_c_ptr, _c_int, _c_int, _c_longlong, _c_ptr, _c_ptr, _c_int, _c_ptr,
+                                      _c_ptr]
+    library.hx_copy_pages.restype = _c_int
+    library.hx_keep_rows.argtypes = [
+        _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr,
+        _c_int, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr]
+    library.hx_keep_rows.restype = _c_int
+    library.hx_verify_drafts.argtypes = [
+        _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,
+        _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr]
+    library.hx_verify_drafts.restype = _c_int
     for name in ("hx_embed", "hx_rmsnorm", "hx_swiglu", "hx_rope_append", "hx_gemm_simt",
                  "hx_gemm_tc", "hx_gemm_tc_supports", "hx_gemm_tc_token_tile",
                  "hx_paged_attention", "hx_argmax", "hx_sample", "hx_embed_scaled",
@@ -1010,6 +1029,157 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     else:
         _check(lib().hx_prefill_attention_windowed(*arguments, int(window), int(keep_first),
                                                    _ptr(status), _stream()))
+
+
+# ----------------------------------------------------------------- trees of drafted tokens
+
+def _need_each(dtype: torch.dtype, names: str, *tensors: torch.Tensor) -> None:
+    """Operands of one dtype on the current device, contiguous in their last dimension."""
+    device = torch.cuda.current_device() if torch.cuda.is_available() else -2
+    for index, tensor in enumerate(tensors):
+        if tensor.dtype != dtype or tensor.stride(-1) != 1 or tensor.get_device() != device:
+            raise KernelError(f"{names.split()[index]} must be {dtype}, contiguous in its last dimension and on "
+                              "the current CUDA device")
+
+
+def tree_attention_scratch(dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int,
+                           page_size: int) -> int:
+    """Floats of scratch that :func:`tree_attention` needs for these sizes, whatever a step brings."""
+    floats = int(lib().hx_tree_attention_scratch_floats(dtype_code(dtype), heads, kv_heads, head_dim,
+                                                        page_size))
+    if floats < 0:
+        raise KernelError(f"no tree attention of {heads} heads of {head_dim} on {kv_heads} with pages "
+                          f"of {page_size}")
+    return floats
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   visible: torch.Tensor, request_start: torch.Tensor, request_context: torch.Tensor,
+                   request_table_row: torch.Tensor, block_tables: torch.Tensor, out: torch.Tensor,
+                   partial: Optional[torch.Tensor], requests: int, heads: int, kv_heads: int,
+                   head_dim: int, page_size: int, num_pages: int, scale: float,
+                   status: torch.Tensor) -> None:
+    """Attention of drafted tokens: request ``r`` brings the tokens ``request_start[r]`` to
+    ``request_start[r + 1]``, whose keys and values lie in its pages at the places behind its
+    ``request_context[r]`` cached ones, in the order of the tokens.  A token sees every cached
+    key and the drafted ones that ``visible`` (int64 ``[tokens, words]``) names: bit ``j`` of word
+    ``w`` stands for token ``64 w + j`` of its request (see
+    :func:`helix_runtime_b200.engine.step.ancestor_words`).  A token that sees nothing gets zeros.
+    Rows of ``out`` behind the last request's are left as they are.  ``partial`` (float32,
+    :func:`tree_attention_scratch` elements) is made here when it is not given; a call uses it from
+    its launch to its end, so calls that may run at the same time need one each."""
+    code = dtype_code(q.dtype)
+    _need_each(q.dtype, "q k_cache v_cache out", q, k_cache, v_cache, out)
+    _need_each(torch.int64, "visible", visible)
+    _need_each(torch.int32, "request_start request_context request_table_row block_tables status", request_start,
+               request_context, request_table_row, block_tables, status)
+    if visible.dim() != 2 or q.dim() != 2 or out.dim() != 2 or block_tables.dim() != 2:
+        raise KernelError("visible is [tokens, words]; q, out and block_tables are matrices")
+    if (visible.shape[0] < min(q.shape[0], out.shape[0]) or request_start.shape[0] <= requests
+            or min(request_context.shape[0], request_table_row.shape[0]) < requests):
+        raise KernelError("every token has its words, and every request its start, end, context and table")
+    if min(q.shape[1], out.shape[1]) < heads * head_dim or \
+            min(k_cache.numel(), v_cache.numel()) < num_pages * kv_heads * page_size * head_dim:
+        raise KernelError("q and out hold the heads of a token in a row, the cache num_pages pages")
+    if partial is None:
+        partial = torch.empty(tree_attention_scratch(q.dtype, heads, kv_heads, head_dim, page_size),
+                              dtype=torch.float32, device=q.device)
+    else:
+        _need_each(torch.float32, "partial", partial)
+        if partial.numel() < lib().hx_tree_attention_scratch_floats(code, heads, kv_heads, head_dim, page_size):
+            raise KernelError("partial is smaller than tree_attention_scratch says")
+    _check(lib().hx_tree_attention(
+        q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), code, visible.data_ptr(),
+        visible.stride(0), visible.shape[1], request_start.data_ptr(), request_context.data_ptr(),
+        request_table_row.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), out.data_ptr(),
+        out.stride(0), partial.data_ptr(), requests, heads, kv_heads, head_dim, page_size, num_pages,
+        scale, status.data_ptr(), _stream()))
+
+
+def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], token_ids: torch.Tensor,
+                  parents: torch.Tensor, request_start: torch.Tensor, temperature: torch.Tensor,
+                  uniform: torch.Tensor, path: torch.Tensor, kept: torch.Tensor,
+                  next_tokens: torch.Tensor, requests: int, status: torch.Tensor,
+                  replacement: bool = False) -> None:
+    """Which drafted tokens stand, and the token that follows the last of them.
+
+    ``logits`` (float32 ``[tokens, vocab]``) are the target's for the tokens of a step whose
+    requests each brought a tree: token 0 is the last one the request was given, every other
+    (``token_ids``) a draft for what follows its parent (``parents``: its number in the request,
+    smaller than its own; -1 for token 0).  ``draft_logits`` (the same shape) row ``t``: what the
+    children of ``t`` were drawn from, in the order of their numbers, at the request's
+    ``temperature``; with ``replacement`` each from the whole distribution, without it each from
+    what the ones before it left.  None: drafts of no distribution (looked up, say).
+
+    ``uniform`` (float32 in [0, 1), one a token): a drafted token's decides whether it stands,
+    token 0's picks the next token.  The tokens are distributed as the target's own samples at
+    ``temperature`` (float32 ``[requests]``; 0: greedy, then a draft stands when it is the lowest
+    id among the maxima).  Out, all int32: ``path`` ``[requests, width]``, the numbers of the
+    tokens that stand, from 0 on, -1 behind them; ``kept`` how many they are; ``next_tokens``, -1
+    (and FLAG_NONFINITE) when logits on the way are not finite.  A path that is full ends the walk."""
+    _need_each(torch.float32, "logits temperature uniform", logits, temperature, uniform)
+    _need_each(torch.int32, "token_ids parents request_start path kept next_tokens status", token_ids, parents,
+               request_start, path, kept, next_tokens, status)
+    if draft_logits is not None:
+        _need_each(torch.float32, "draft_logits", draft_logits)
+        if draft_logits.shape != logits.shape:
+            raise KernelError("draft_logits has a row of the vocabulary for every row of logits")
+    tokens, vocab = logits.shape
+    if (min(token_ids.shape[0], parents.shape[0], uniform.shape[0]) < tokens or path.dim() != 2
+            or request_start.shape[0] <= requests
+            or min(temperature.shape[0], path.shape[0], kept.shape[0], next_tokens.shape[0]) < requests):
+        raise KernelError("verify_drafts: an operand is too short for the step's tokens and requests")
+    _check(lib().hx_verify_drafts(
+        logits.data_ptr(), logits.stride(0), None if draft_logits is None else draft_logits.data_ptr(),
+        0 if draft_logits is None else draft_logits.stride(0), vocab, token_ids.data_ptr(),
+        parents.data_ptr(), request_start.data_ptr(), temperature.data_ptr(), uniform.data_ptr(),
+        path.data_ptr(), path.stride(0), path.shape[1], kept.data_ptr(), next_tokens.data_ptr(), requests,
+        1 if replacement else 0, status.data_ptr(), _stream()))
+
+
+def _storage_sizes(storage: torch.Tensor):
+    """``[layers, 2, pages, kv_heads, page_size, head_dim]`` of a cache group's storage."""
+    if storage.dim() != 6 or storage.shape[1] != 2 or not storage.is_contiguous():
+        raise KernelError("storage is [layers, 2, pages, kv_heads, page_size, head_dim], contiguous")
+    _need_each(storage.dtype, "storage", storage)
+    return storage.shape
+
+
+def keep_rows(storage: torch.Tensor, block_tables: torch.Tensor, request_table_row: torch.Tensor,
+              request_context: torch.Tensor, path: torch.Tensor, kept: torch.Tensor, requests: int,
+              status: torch.Tensor) -> None:
+    """The cached rows of drafted tokens that stand move together, in all layers of a group of the
+    cache (``storage``: :attr:`helix_runtime_b200.cache.manager.CacheGroup.storage`): row ``k <
+    kept[r]`` of request ``r`` goes from place ``request_context[r] + path[r, k]`` to place
+    ``request_context[r] + k``; ``path`` as :func:`verify_drafts` leaves it, ascending.  A request
+    whose path does not ascend, is longer than a row of ``path`` (FLAG_BAD_MOVE) or leads outside its
+    pages (FLAG_BAD_PAGE) keeps its rows where they are.  Requests share no page they move rows in."""
+    layers, _, pages, kv_heads, page_size, head_dim = _storage_sizes(storage)
+    _need_each(torch.int32, "block_tables request_table_row request_context path kept status", block_tables,
+               request_table_row, request_context, path, kept, status)
+    if path.dim() != 2 or min(request_table_row.shape[0], request_context.shape[0], path.shape[0],
+                              kept.shape[0]) < requests:
+        raise KernelError("keep_rows: an operand is too short for the requests")
+    _check(lib().hx_keep_rows(
+        storage.data_ptr(), dtype_code(storage.dtype), 2 * layers, pages, kv_heads, page_size, head_dim,
+        block_tables.data_ptr(), block_tables.stride(0), request_table_row.data_ptr(),
+        request_context.data_ptr(), path.data_ptr(), path.stride(0), path.shape[1], kept.data_ptr(),
+        requests, status.data_ptr(), _stream()))
+
+
+def copy_pages(storage: torch.Tensor, source: torch.Tensor, target: torch.Tensor,
+               status: torch.Tensor) -> None:
+    """Page ``target[i]`` becomes a copy of page ``source[i]`` (int32 on the device), in all layers
+    of a group of the cache (``storage`` as in :func:`keep_rows`).  A pair with a page outside the
+    pool is left out (FLAG_BAD_PAGE), and so is one whose target another pair writes or reads
+    (FLAG_BAD_MOVE); a page copied onto itself stays."""
+    layers, _, pages, kv_heads, page_size, head_dim = _storage_sizes(storage)
+    _need_each(torch.int32, "source target status", source, target, status)
+    if source.shape != target.shape or source.dim() != 1:
+        raise KernelError("source and target are lists of pages of one length")
+    _check(lib().hx_copy_pages(
+        storage.data_ptr(), 2 * layers, pages, kv_heads * page_size * head_dim * storage.element_size(),
+        source.data_ptr(), target.data_ptr(), source.shape[0], status.data_ptr(), _stream()))
 
 
 # ------------------------------------------------------------ residual streams, biased sums

@@ -50,6 +50,7 @@ extern "C" {
 #define HX_STATUS_WAIT_TIMEOUT 4
 #define HX_STATUS_NONFINITE 8
 #define HX_STATUS_BAD_POSITION 16
+#define HX_STATUS_BAD_MOVE 32
 
 /* ---- library ---------------------------------------------------------------------------- */
 int hx_abi_version(void);
@@ -767,6 +768,36 @@ int hx_prefill_attention_tc_windowed(const void* q, int ldq, const void* k_cache
                                      int head_dim, int page_size, int num_pages, float scale,
                                      int min_query_len, int window, int keep_first, int* status,
                                      cudaStream_t stream);
+
+/* ---- trees of drafted tokens ------------------------------------------------------------ */
+/* floats of scratch hx_tree_attention needs, whatever the step brings; negative: no kernel */
+long long hx_tree_attention_scratch_floats(int dtype, int heads, int kv_heads, int head_dim,
+                                           int page_size);
+/* a request's drafted tokens over its cached keys and the drafted ones that a bit mask names;
+ * visible: [tokens, ld_visible] 64-bit words, `words` of them a token, bit j of word w = token
+ * 64 w + j of the request, whose key lies behind the request_context cached ones */
+int hx_tree_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int dtype,
+                      const long long* visible, int ld_visible, int words, const int* request_start,
+                      const int* request_context, const int* request_table_row,
+                      const int* block_tables, int table_stride, void* out, int ldo, float* partial,
+                      int requests, int heads, int kv_heads, int head_dim, int page_size,
+                      int num_pages, float scale, int* status, cudaStream_t stream);
+/* which drafted tokens stand against the target's logits, by the caller's uniform numbers, and the
+ * token that follows the last of them; path: the numbers of those that stand, -1 behind them */
+int hx_verify_drafts(const float* logits, int ld, const float* draft, int ld_draft, int vocab,
+                     const int* token_ids, const int* parents, const int* request_start,
+                     const float* temperature, const float* uniform, int* path, int ld_path, int width,
+                     int* kept, int* next_tokens, int requests, int put_back, int* status,
+                     cudaStream_t stream);
+/* row k < kept[r] of request r moves from place context + path[r][k] to place context + k, in
+ * every plane (a layer's keys, or its values) of the storage */
+int hx_keep_rows(void* storage, int dtype, int planes, int num_pages, int kv_heads, int page_size,
+                 int head_dim, const int* block_tables, int table_stride, const int* request_table_row,
+                 const int* request_context, const int* path, int ld_path, int width, const int* kept,
+                 int requests, int* status, cudaStream_t stream);
+/* page source[i] to page target[i], in every plane */
+int hx_copy_pages(void* storage, int planes, int num_pages, long long page_bytes, const int* source,
+                  const int* target, int pairs, int* status, cudaStream_t stream);
 
 /* ---- sampling --------------------------------------------------------------------------- */
 /* lowest id among the maxima; -1 and HX_STATUS_NONFINITE for a row with a non-finite logit */

@@ -1,0 +1,258 @@
+"""Attention of drafted tokens over the paged cache, against the plain form in 64 bits."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from helix_runtime_b200.ops import library as ops
+from plain_tree import Batch, ancestors, random_parents
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float32]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("contexts,nodes,heads,kv_heads,head_dim,page", [
+    ([5], [1], 1, 1, 64, 16),                                  # one token of one head
+    ([0], [1], 2, 2, 128, 16),                                 # no cached key
+    ([63, 64, 65, 127, 128], [1, 1, 1, 1, 1], 4, 4, 128, 16),  # keys end at and around a tile's border
+    ([100, 3], [5, 9], 4, 4, 128, 16),
+    ([700, 0, 65], [20, 1, 64], 4, 1, 128, 16),                # heads that share keys; 64 and 256 rows
+    ([700, 0, 65], [20, 1, 64], 4, 2, 112, 32),
+    ([300, 31], [40, 7], 2, 2, 64, 64),
+    ([300, 31], [140, 70], 4, 2, 96, 16),                      # more than two words of a mask
+    ([33, 10], [129, 2], 2, 2, 80, 16),                        # a second tile of one row
+    ([40], [9], 12, 4, 64, 32),                                # groups of three
+    ([50], [3], 96, 1, 64, 16),                                # one token a tile
+    ([50], [3], 260, 2, 64, 16),                               # a token's heads take two tiles
+    ([50, 7], [6, 3], 2, 1, 160, 16),                          # heads of other kernels
+    ([50, 7], [40, 3], 2, 1, 256, 32),
+    ([50, 70], [6, 33], 4, 2, 64, 8),                          # pages no tensor-core kernel takes
+    ([50, 70], [6, 3], 4, 2, 100, 7),
+    ([50, 70], [6, 3], 4, 2, 300, 8),
+    ([50, 70], [6, 3], 4, 4, 6, 1),
+    ([5000], [64], 8, 2, 128, 32),                             # one request over all CTAs
+])
+def test_sizes(dtype, contexts, nodes, heads, kv_heads, head_dim, page):
+    batch = Batch(1, contexts, nodes, heads, kv_heads, head_dim, page, dtype, row_pad=8)
+    batch.run(ops)
+    batch.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 64])
+def test_many_items_a_run(dtype, page):
+    """CTAs whose runs end items, hold whole ones and begin others."""
+    rng = np.random.default_rng(5)
+    contexts = [int(c) for c in rng.integers(0, 900, 20)]
+    nodes = [int(n) for n in rng.integers(1, 20, 20)]
+    nodes[7] = 0                       # a request without tokens
+    batch = Batch(2, contexts, nodes, 32, 32, 64, page, dtype)
+    batch.run(ops)
+    batch.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_short_items_many_a_run(dtype):
+    batch = Batch(3, [3] * 70, [1 + i % 5 for i in range(70)], 32, 32, 64, 16, dtype)
+    batch.run(ops)
+    batch.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("head_dim,page", [(64, 16), (64, 8), (6, 4)])
+def test_masks(dtype, head_dim, page):
+    """Tokens that see nothing, all, later tokens, none of the drafted ones, only the last."""
+    rng = np.random.default_rng(7)
+    count = 70
+    seen = [np.zeros((count, count), dtype=bool), rng.random((count, count)) < 0.3]
+    seen[0][3] = True
+    seen[0][5, count - 1] = True
+    seen[1][0] = False
+    for contexts in ([0, 0], [130, 0], [0, 61]):
+        batch = Batch(4, contexts, [count, count], 4, 4, head_dim, page, dtype, seen=seen)
+        batch.run(ops)
+        batch.check()
+        if contexts[0] == 0:
+            assert bool((batch.out[0, :4 * head_dim] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_words(dtype):
+    """More words than the tokens need (bits behind the last token name nothing), and fewer."""
+    for words in (1, 3):
+        seen = [np.ones((90, 90), dtype=bool), np.ones((20, 20), dtype=bool)]
+        batch = Batch(5, [40, 7], [90, 20], 2, 2, 64, 16, dtype, seen=seen, words=words)
+        if words == 3:
+            batch.visible[:] = -1
+        batch.run(ops)
+        batch.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("head_dim,page", [(128, 16), (128, 8), (6, 4)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_values_that_are_not_finite_reach_who_sees_them(dtype, head_dim, page, bad):
+    """A drafted key and value that are not finite change nothing for tokens that do not see them;
+    a value reaches, coordinate by coordinate, those that do."""
+    nodes, context = 12, 100
+    seen = [ancestors([-1, 0, 0, 1, 1, 2, 2, 3, 3, 5, 5, 6])]
+    clean = Batch(6, [context], [nodes], 2, 2, head_dim, page, dtype, seen=seen)
+    clean.run(ops)
+    batch = Batch(6, [context], [nodes], 2, 2, head_dim, page, dtype, seen=seen)
+    place = context + 2                     # token 2: its branch is 2, 5, 6, 9, 10, 11
+    page_id = int(batch.tables[batch.row[0], place // page])
+    rows = torch.zeros((2, page, head_dim), dtype=dtype)
+    rows[:, place % page, 1] = bad
+    from plain_tree import to_cache
+    hit = to_cache(rows, dtype).ne(0).to(batch.v.device)
+    batch.v[page_id][hit] = bad
+    batch.run(ops)
+    branch = [2, 5, 6, 9, 10, 11]
+    others = [n for n in range(nodes) if n not in branch]
+    got, want = batch.out[:nodes, :2 * head_dim], clean.out[:nodes, :2 * head_dim]
+    assert torch.equal(got[others], want[others])
+    columns = [1, head_dim + 1]
+    kept = [c for c in range(2 * head_dim) if c not in columns]
+    assert torch.equal(got[branch][:, kept], want[branch][:, kept])
+    reached = got[branch][:, columns]
+    assert bool((reached.isnan() if bad != bad else reached == bad).all())
+    batch.v.copy_(clean.v)
+    batch.k[page_id][hit] = bad
+    batch.run(ops)
+    assert torch.equal(batch.out[:nodes][others], clean.out[:nodes][others])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scratch_needs_nothing_and_is_reused(dtype):
+    floats = ops.tree_attention_scratch(dtype, 4, 4, 128, 16)
+    partial = torch.full((floats + 1,), float("nan"), device="cuda:0")
+    for seed, contexts, nodes in ((8, [700, 20], [30, 4]), (9, [64], [1]), (10, [5000, 90, 3], [7, 60, 1])):
+        batch = Batch(seed, contexts, nodes, 4, 4, 128, 16, dtype)
+        batch.run(ops, partial[:floats])
+        batch.check()
+    assert bool(partial[floats:].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pages_outside_the_pool_are_reported(dtype):
+    for index, wrong in ((0, -1), (3, 10 ** 6)):
+        batch = Batch(11, [50, 50], [4, 4], 2, 2, 64, 16, dtype, stale=0.0)
+        batch.tables[batch.row[0], index] = wrong
+        batch.run(ops)
+        assert int(batch.status.item()) == ops.FLAG_BAD_PAGE
+        expected, weighed, largest = batch.expected()
+        off = (batch.out[4:8, :128].double().cpu() - expected[4:]).abs()
+        assert bool((off <= batch.tolerance(expected, weighed, largest)[4:]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nothing_to_do(dtype):
+    batch = Batch(12, [9], [0], 2, 2, 64, 16, dtype)
+    batch.run(ops)
+    assert bool((batch.out == 7.0).all())
+    batch.requests = 0
+    batch.run(ops)
+    assert bool((batch.out == 7.0).all()) and int(batch.status.item()) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_graph_is_replayed_over_other_trees(dtype):
+    """A recorded call reads lengths, masks and tables when it is replayed."""
+    args = ([400, 90], [17, 30], 4, 4, 128, 16, dtype)
+    batch = Batch(13, *args)
+    partial = torch.empty(ops.tree_attention_scratch(dtype, 4, 4, 128, 16), device="cuda:0")
+    batch.run(ops, partial)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch.run(ops, partial)
+    other = Batch(14, [33, 401], [30, 16], *args[2:])
+    for name in ("q", "out", "visible", "start", "context", "row", "status"):
+        mine, theirs = getattr(batch, name), getattr(other, name)
+        mine[:theirs.shape[0]].copy_(theirs)
+    batch.out.fill_(7.0)
+    pages = min(batch.num_pages, other.num_pages)
+    assert other.num_pages <= batch.num_pages and other.tables.shape[1] <= batch.tables.shape[1]
+    batch.k[:pages].copy_(other.k[:pages])
+    batch.v[:pages].copy_(other.v[:pages])
+    batch.tables.fill_(-1)
+    batch.tables[:, :other.tables.shape[1]].copy_(other.tables)
+    graph.replay()
+    torch.cuda.synchronize()
+    other.check(batch.out[:other.out.shape[0]])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_other_stream(dtype):
+    batch = Batch(15, [400, 90], [17, 30], 4, 4, 128, 16, dtype)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        batch.run(ops)
+    stream.synchronize()
+    batch.check()
+
+
+def test_offsets_beyond_32_bits():
+    """Pages behind the first 2^31 elements of a layer's keys and values."""
+    small = Batch(16, [200, 30], [9, 20], 32, 32, 128, 64, torch.bfloat16, stale=0.0)
+    pages = (1 << 31) // (32 * 64 * 128) + small.num_pages + 1
+    shift = pages - small.num_pages
+    for name in ("k", "v"):
+        wide = torch.empty((pages, *getattr(small, name).shape[1:]), dtype=torch.bfloat16, device="cuda:0")
+        wide[shift:] = getattr(small, name)
+        setattr(small, name, wide)
+    small.tables = torch.where(small.tables >= 0, small.tables + shift, small.tables)
+    small.num_pages = pages
+    small.run(ops)
+    small.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_chain_is_what_causal_attention_computes(dtype):
+    """Drafts in a row: the causal kernel over the same pages."""
+    contexts, nodes = [77, 300], [6, 9]
+    seen = [np.tril(np.ones((n, n), dtype=bool)) for n in nodes]
+    batch = Batch(17, contexts, nodes, 4, 2, 128, 16, dtype, seen=seen, stale=0.0)
+    batch.run(ops)
+    tokens = sum(nodes)
+    positions = torch.tensor([c + j for c, n in zip(contexts, nodes) for j in range(n)], dtype=torch.int32,
+                             device="cuda:0")
+    request = torch.tensor([r for r, n in enumerate(nodes) for _ in range(n)], dtype=torch.int32, device="cuda:0")
+    causal = torch.zeros((tokens, 4 * 128), dtype=dtype, device="cuda:0")
+    ops.paged_attention(batch.q, batch.k, batch.v, positions, request, batch.row, batch.tables, causal, None,
+                        tokens, 4, 2, 128, 16, batch.num_pages, 0, batch.scale, 256, 2, batch.status)
+    expected, weighed, largest = batch.expected()
+    allowed = 2 * batch.tolerance(expected, weighed, largest)
+    assert bool(((batch.out[:tokens, :512] - causal).double().cpu().abs() <= allowed).all())
+    batch.check()
+
+
+def test_refusals():
+    batch = Batch(18, [50], [4], 2, 2, 64, 16, torch.bfloat16)
+    base = dict(vars(batch))
+
+    def refused(**changes):
+        for name, value in {**base, **changes}.items():
+            setattr(batch, name, value)
+        with pytest.raises(ops.KernelError):
+            batch.run(ops)
+        assert bool((base["out"] == 7.0).all())
+
+    refused(head_dim=63)
+    refused(head_dim=1026)
+    refused(kv_heads=3)
+    refused(page_size=0)
+    refused(num_pages=0)
+    refused(scale=0.0)
+    refused(scale=-1.0)
+    refused(heads=0)
+    refused(visible=batch.visible.to(torch.int32))
+    refused(visible=batch.visible[:2])
+    refused(start=batch.start[:1])
+    refused(k=batch.k.float())
+    refused(q=batch.q.double())
+    refused(q=torch.zeros((7, 130), dtype=torch.bfloat16, device="cuda:0")[:, 1:129])      # not aligned
