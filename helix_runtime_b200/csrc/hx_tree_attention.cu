@@ -12,7 +12,7 @@
 // CTA takes the tokens of a request (and the query heads that share a key/value head) as rows of
 // one tile and reads every key once for all of them; a long context is cut over CTAs (see
 // hx_tree_attention.cuh).  Three kernels:
-//   * hx_tree_attention_tc.cu: bfloat16, heads of 64 to 128, pages of 16, 32 or 64 keys;
+//   * hx_tree_attention_tc.cu: bfloat16, heads of 64 to 128, pages of 8, 16, 32 or 64 keys;
 //   * tree_tile_kernel: any other page size, float32 or bfloat16, heads up to 256 in steps of 4.
 //     32 rows by 64 keys at a time on the CUDA cores, all in float32;
 //   * tree_row_kernel: what is left (heads up to 1,024, even), a row a warp.
@@ -65,10 +65,13 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
   float* probabilities = values + TILE_KEYS * (D + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TreeRun run = tree_run<TILE_KEYS>(a, blockIdx.x, gridDim.x, TILE_LEAST);
-  if (run.count == 0) return;
   TreeCursor c;
-  long long item_begin;
-  tree_locate<TILE_KEYS>(a, run.begin, c, item_begin);
+  if (run.count > 0) {
+    tree_locate<TILE_KEYS>(a, run.begin, c);
+  } else {
+    if (threadIdx.x == 0) tree_tell_cut<TILE_ROWS, TILE_KEYS>(a, run, c, 0, blockIdx.x, gridDim.x);
+    return;
+  }
   const int chunk = hx_cache_chunk(sizeof(T), D);
   const T* q = static_cast<const T*>(a.q);
   const T* k_cache = static_cast<const T*>(a.k_cache);
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
     // ---- the rows, or this CTA's part of them
     if (live) {
       const bool whole = c.tile == 0 && count == c.tiles;
-      float* part = a.partial + (2ll * blockIdx.x + (c.tile == 0 ? 1 : 0)) * tree_part_floats<TILE_ROWS>(D);
+      float* part = tree_part<TILE_ROWS>(a, blockIdx.x, c.tile == 0);
 #pragma unroll
       for (int i = 0; i < ROWS_A_WARP; ++i) {
         const int row = warp * ROWS_A_WARP + i;
@@ -242,6 +245,7 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
     }
     left -= count;
     if (left > 0) tree_next_item<TILE_KEYS>(a, c);
+    else if (threadIdx.x == 0) tree_tell_cut<TILE_ROWS, TILE_KEYS>(a, run, c, count, blockIdx.x, gridDim.x);
   }
 }
 
@@ -258,10 +262,13 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void tree_row_kernel(const TreeArgs
   hx_pdl_prologue();
   const int D = a.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TreeRun run = tree_run<ROW_KEYS>(a, blockIdx.x, gridDim.x, ROW_LEAST);
-  if (run.count == 0) return;
   TreeCursor c;
-  long long item_begin;
-  tree_locate<ROW_KEYS>(a, run.begin, c, item_begin);
+  if (run.count > 0) {
+    tree_locate<ROW_KEYS>(a, run.begin, c);
+  } else {
+    if (threadIdx.x == 0) tree_tell_cut<ROW_WARPS, ROW_KEYS>(a, run, c, 0, blockIdx.x, gridDim.x);
+    return;
+  }
   const int chunk = hx_cache_chunk(sizeof(T), D);
   const T* k_cache = static_cast<const T*>(a.k_cache);
   const T* v_cache = static_cast<const T*>(a.v_cache);
@@ -348,7 +355,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void tree_row_kernel(const TreeArgs
       const float inverse = row_sum > 0.0f ? 1.0f / row_sum : 0.0f;
       T* out = static_cast<T*>(a.out) + static_cast<size_t>(c.q_begin + token) * a.ldo +
                static_cast<size_t>(head) * D;
-      float* part = a.partial + (2ll * blockIdx.x + (c.tile == 0 ? 1 : 0)) * tree_part_floats<ROW_WARPS>(D);
+      float* part = tree_part<ROW_WARPS>(a, blockIdx.x, c.tile == 0);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
         const int d = 2 * lane + 64 * i;
@@ -368,59 +375,44 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void tree_row_kernel(const TreeArgs
     }
     left -= count;
     if (left > 0) tree_next_item<ROW_KEYS>(a, c);
+    else if (threadIdx.x == 0) tree_tell_cut<ROW_WARPS, ROW_KEYS>(a, run, c, count, blockIdx.x, gridDim.x);
   }
 }
 
 // ------------------------------------------------------------------ joining parts
 
-constexpr int JOIN_THREADS = 128;
-constexpr int JOIN_LOADS = 4;      // parts whose loads are in flight together
+constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_LOADS = 8;      // parts whose loads are in flight together
 
-// Block (x, y): the item that begins in the run of CTA x and goes on behind it, if there is one,
-// and the y-th share of its rows' coordinates.  The parts: the one CTA x left in its place 1, and those the
-// CTAs behind it left in their place 0, in that order.  The run of x is empty or the item ends
-// inside it: nothing to do.
-template <typename T, int ROWS, int KEYS, int VEC>
-__global__ __launch_bounds__(JOIN_THREADS) void tree_join_kernel(const TreeArgs a, int ctas, int least) {
-  // the runs are found from the step's description, which was there before the kernel in front
-  hx_pdl_trigger();
-  const int owner = blockIdx.x;
-  const TreeRun run = tree_run<KEYS>(a, owner, ctas, least);
-  TreeCursor c;
-  long long item_begin = 0;
-  bool mine = false;
-  int parts = 0;
-  if (run.count > 0) {
-    tree_locate<KEYS>(a, run.begin + run.count - 1, c, item_begin);
-    mine = item_begin >= run.begin && item_begin + c.tiles > run.begin + run.count;
-    if (mine) parts = static_cast<int>((item_begin + c.tiles - 1) / run.per_cta) - owner + 1;
-  }
-  hx_pdl_wait();
-  if (!mine) return;
-  const int D = a.head_dim;
-  const TreeRows rows(a, c);
-  const int rows_here = rows.count;
+// Block (x, y): the y-th share of the coordinates of the item that begins in the run of CTA x and goes
+// on behind it, if there is one.  Its parts: what CTA x left in its place 1, and what the CTAs behind it
+// left in their place 0, joined in that order.
+template <typename T, int ROWS, int VEC>
+__global__ __launch_bounds__(JOIN_THREADS) void tree_join_kernel(const TreeArgs a) {
+  hx_pdl_prologue();
+  const int owner = blockIdx.x, ctas = gridDim.x, D = a.head_dim;
+  const TreeCut cut = *tree_cut<ROWS>(a, owner, ctas);
+  if (cut.parts == 0) return;
   const long long stride = tree_part_floats<ROWS>(D);
   const float* first = a.partial + (2ll * owner + 1) * stride;
   const float* others = a.partial + 2ll * (owner + 1) * stride;
   auto part_of = [&](int index) { return index == 0 ? first : others + 2ll * (index - 1) * stride; };
   const int pieces = D / VEC;
-  for (int i = blockIdx.y * JOIN_THREADS + threadIdx.x; i < rows_here * pieces; i += gridDim.y * JOIN_THREADS) {
-    const int piece = i / rows_here, row = i - piece * rows_here;
+  for (int i = blockIdx.y * JOIN_THREADS + threadIdx.x; i < cut.rows * pieces; i += gridDim.y * JOIN_THREADS) {
+    const int piece = i / cut.rows, row = i - piece * cut.rows;
     float total_max = -INFINITY, total_sum = 0.0f, acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
-    for (int base = 0; base < parts; base += JOIN_LOADS) {
+    for (int base = 0; base < cut.parts; base += JOIN_LOADS) {
       float m[JOIN_LOADS], l[JOIN_LOADS], o[JOIN_LOADS][VEC];
 #pragma unroll
       for (int u = 0; u < JOIN_LOADS; ++u) {
         m[u] = -INFINITY;
-        l[u] = 0.0f;
-        if (base + u < parts) {
+        if (base + u < cut.parts) {
           const float* part = part_of(base + u);
-          m[u] = __ldcg(part + static_cast<size_t>(D) * ROWS + row);
-          l[u] = __ldcg(part + static_cast<size_t>(D + 1) * ROWS + row);
-          const float* at = part + (static_cast<size_t>(piece) * ROWS + row) * VEC;
+          m[u] = __ldcg(part + D * ROWS + row);
+          l[u] = __ldcg(part + (D + 1) * ROWS + row);
+          const float* at = part + (piece * ROWS + row) * VEC;
           if constexpr (VEC == 4) {
             const float4 v = __ldcg(reinterpret_cast<const float4*>(at));
             o[u][0] = v.x; o[u][1] = v.y; o[u][2] = v.z; o[u][3] = v.w;
@@ -442,8 +434,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void tree_join_kernel(const TreeArgs 
       }
     }
     const float inverse = total_sum > 0.0f ? 1.0f / total_sum : 0.0f;
-    T* out = static_cast<T*>(a.out) + static_cast<size_t>(c.q_begin + rows.token0 + row / rows.heads) * a.ldo +
-             static_cast<size_t>(rows.head0 + row % rows.heads) * D + piece * VEC;
+    T* out = static_cast<T*>(a.out) + static_cast<size_t>(cut.token + row / cut.heads) * a.ldo +
+             static_cast<size_t>(cut.head0 + row % cut.heads) * D + piece * VEC;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) out[e] = hx_from_float<T>(acc[e] * inverse);
   }
@@ -477,22 +469,20 @@ TreeKernel kernel_for(int dtype, int head_dim, int page_size) {
 
 }  // namespace
 
-int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int least, int rows, int keys, int vec,
-                 cudaStream_t stream) {
-  // shares of an item's coordinates: 16 of them, so that a block has a few pieces a thread at most
-  const int shares = rows >= 128 ? 16 : rows >= 32 ? 8 : 2;
-  const dim3 grid(ctas, shares);
+int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int rows, cudaStream_t stream) {
+  // shares of an item: of 128 rows, two pieces of coordinates a thread
+  const dim3 grid(ctas, rows >= 128 ? 8 : rows >= 32 ? 4 : 1);
   const bool half = dtype == HX_BF16;
-  if (rows == 128 && keys == 64 && vec == 4 && half)
-    hx_launch(tree_join_kernel<__nv_bfloat16, 128, 64, 4>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+  if (rows == 128)
+    hx_launch(tree_join_kernel<__nv_bfloat16, 128, 4>, grid, JOIN_THREADS, 0, stream, a);
   else if (rows == TILE_ROWS && half)
-    hx_launch(tree_join_kernel<__nv_bfloat16, TILE_ROWS, TILE_KEYS, 4>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+    hx_launch(tree_join_kernel<__nv_bfloat16, TILE_ROWS, 4>, grid, JOIN_THREADS, 0, stream, a);
   else if (rows == TILE_ROWS)
-    hx_launch(tree_join_kernel<float, TILE_ROWS, TILE_KEYS, 4>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+    hx_launch(tree_join_kernel<float, TILE_ROWS, 4>, grid, JOIN_THREADS, 0, stream, a);
   else if (half)
-    hx_launch(tree_join_kernel<__nv_bfloat16, ROW_WARPS, ROW_KEYS, 2>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+    hx_launch(tree_join_kernel<__nv_bfloat16, ROW_WARPS, 2>, grid, JOIN_THREADS, 0, stream, a);
   else
-    hx_launch(tree_join_kernel<float, ROW_WARPS, ROW_KEYS, 2>, grid, JOIN_THREADS, 0, stream, a, ctas, least);
+    hx_launch(tree_join_kernel<float, ROW_WARPS, 2>, grid, JOIN_THREADS, 0, stream, a);
   HX_CHECK_LAUNCH("hx_tree_attention");
   return HX_OK;
 }
@@ -508,8 +498,8 @@ HX_API long long hx_tree_attention_scratch_floats(int dtype, int heads, int kv_h
   if (sms <= 0) return -1;
   switch (kernel_for(dtype, head_dim, page_size)) {
     case TREE_TC: return hx_tree_tc_floats(head_dim);
-    case TREE_TILE: return 2ll * sms * tile_ctas_an_sm(head_dim) * tree_part_floats<TILE_ROWS>(head_dim);
-    default: return 2ll * sms * ROW_CTAS * tree_part_floats<ROW_WARPS>(head_dim);
+    case TREE_TILE: return tree_scratch_floats<TILE_ROWS>(head_dim, sms * tile_ctas_an_sm(head_dim));
+    default: return tree_scratch_floats<ROW_WARPS>(head_dim, sms * ROW_CTAS);
   }
 }
 
@@ -562,12 +552,12 @@ HX_API int hx_tree_attention(const void* q, int ldq, const void* k_cache, const 
     else
       rc = head_dim <= 128 ? launch_tile<float, 128>(a, ctas, stream) : launch_tile<float, 256>(a, ctas, stream);
     if (rc != HX_OK) return rc;
-    return hx_tree_join(a, dtype, ctas, TILE_LEAST, TILE_ROWS, TILE_KEYS, 4, stream);
+    return hx_tree_join(a, dtype, ctas, TILE_ROWS, stream);
   }
   tree_fill_rows(a, ROW_WARPS);
   const int ctas = sms * ROW_CTAS;
   if (dtype == HX_BF16) hx_launch(tree_row_kernel<__nv_bfloat16>, ctas, ROW_WARPS * 32, 0, stream, a);
   else hx_launch(tree_row_kernel<float>, ctas, ROW_WARPS * 32, 0, stream, a);
   HX_CHECK_LAUNCH("hx_tree_attention");
-  return hx_tree_join(a, dtype, ctas, ROW_LEAST, ROW_WARPS, ROW_KEYS, 2, stream);
+  return hx_tree_join(a, dtype, ctas, ROW_WARPS, stream);
 }

@@ -99,11 +99,9 @@ __device__ __forceinline__ long long tree_total(const TreeArgs& a) {
   return mine;
 }
 
-// The item and key tile at place `at` of the list (0 <= at < total); `item_begin`: the place of the
-// item's first tile.  Called by a converged warp.
+// The item and key tile at place `at` of the list (0 <= at < total).  Called by a converged warp.
 template <int KEYS>
-__device__ __forceinline__ void tree_locate(const TreeArgs& a, long long at, TreeCursor& c,
-                                            long long& item_begin) {
+__device__ __forceinline__ void tree_locate(const TreeArgs& a, long long at, TreeCursor& c) {
   const int lane = threadIdx.x & 31;
   long long before = 0;
   int found = -1;
@@ -132,7 +130,6 @@ __device__ __forceinline__ void tree_locate(const TreeArgs& a, long long at, Tre
   const long long inside = at - before;
   c.item = static_cast<int>(inside / c.tiles);
   c.tile = static_cast<int>(inside - static_cast<long long>(c.item) * c.tiles);
-  item_begin = at - c.tile;
 }
 
 // On to the next item (there is one: callers count the tiles that are left to them).
@@ -154,6 +151,15 @@ __device__ __forceinline__ void tree_next_item(const TreeArgs& a, TreeCursor& c)
 struct TreeRun {
   long long begin, per_cta, total;
   int count;
+};
+
+// What the join needs to know of the item that begins in a CTA's run and goes on behind it; a CTA
+// without one says parts = 0.
+struct TreeCut {
+  int parts;                    // this CTA's and those of the CTAs behind it
+  int token, head0, heads;      // the row of `out` and the head of row 0, heads a token
+  int rows;
+  int unused[3];
 };
 template <int KEYS>
 __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int cta, int ctas, int least) {
@@ -203,12 +209,41 @@ template <int ROWS>
 __host__ __device__ constexpr long long tree_part_floats(int head_dim) {
   return static_cast<long long>(ROWS) * (head_dim + 2);
 }
+// The scratch: two parts a CTA, behind them what each says about its cut item.
+template <int ROWS>
+__host__ __device__ constexpr long long tree_scratch_floats(int head_dim, int ctas) {
+  return ctas * (2 * tree_part_floats<ROWS>(head_dim) + static_cast<long long>(sizeof(TreeCut) / 4));
+}
+template <int ROWS>
+__device__ __forceinline__ TreeCut* tree_cut(const TreeArgs& a, int cta, int ctas) {
+  return reinterpret_cast<TreeCut*>(a.partial + ctas * 2 * tree_part_floats<ROWS>(a.head_dim)) + cta;
+}
+template <int ROWS>
+__device__ __forceinline__ float* tree_part(const TreeArgs& a, int cta, bool item_begins) {
+  return a.partial + (2ll * cta + (item_begins ? 1 : 0)) * tree_part_floats<ROWS>(a.head_dim);
+}
+
+// One thread says what the CTA's run leaves to the join: looked at from the run's last key tile.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void tree_tell_cut(const TreeArgs& a, const TreeRun& run, const TreeCursor& last,
+                                              int last_count, int cta, int ctas) {
+  TreeCut cut = {};
+  if (run.count > 0 && last.tile == 0 && last_count < last.tiles) {
+    const TreeRows rows(a, last);
+    const long long item_end = run.begin + run.count - last_count + last.tiles;
+    cut.parts = static_cast<int>((item_end - 1) / run.per_cta) - cta + 1;
+    cut.token = last.q_begin + rows.token0;
+    cut.head0 = rows.head0;
+    cut.heads = rows.heads;
+    cut.rows = rows.count;
+  }
+  *tree_cut<ROWS>(a, cta, ctas) = cut;
+}
 
 }  // namespace
 
-// Joins the parts that `ctas` CTAs left, on the same stream behind them.
-int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int least, int rows, int keys, int vec,
-                 cudaStream_t stream);
+// Joins the parts that `ctas` CTAs of tiles of `rows` rows left, on the same stream behind them.
+int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int rows, cudaStream_t stream);
 
 // The tcgen05 kernel (bfloat16): whether it takes these sizes, its scratch, its launch.
 bool hx_tree_tc_takes(int head_dim, int page_size);

@@ -3,10 +3,7 @@
 //
 // A tile of 128 rows (the M of a product) holds the drafted tokens of a request, each with the
 // query heads of one key/value head; the item walks its keys 64 at a time.  Warp roles:
-//   warp 0      asks for keys and values: values a whole (page, head) block a copy, keys piece by
-//               piece (16 bytes of all slots of a page), two copies a lane, which lays them out as
-//               [piece][64 keys][16 bytes] whatever the page size: one stride from 8 keys to the
-//               next, so that one product covers the tile;
+//   warp 0      asks for keys and values, a whole (page, head) block a copy (see below);
 //   warp 1      one lane issues S = Q K^T into one of two score buffers in tensor memory;
 //   warp 2      one lane issues O += P V;
 //   warp 3      loads the queries of an item, as soon as the item before has read its own;
@@ -17,12 +14,22 @@
 // Keys and values keep flowing across items: the rings go by TURNS, the key tiles of the CTA's run in
 // order.  Two CTAs share an SM and fill each other's gaps.
 //
+// Operands as they land.  A block of the cache is [piece][slot][16 bytes], so eight slots of a piece
+// are a core matrix (8 rows x 16 bytes) of an operand that is not swizzled.  What a product's descriptor
+// wants is one stride from eight keys to the next eight.  Pages of 64: 128 bytes.  Pages of 32: two
+// products of 32 keys.  Pages of 8: the stride is the block's size.  Pages of 16: the first eight
+// slots of the four pages lie a block apart, and so do the second eight: two products of 32 keys,
+// whose scores stand in that order, column 32 a + 8 p + s for key 16 p + 8 a + s.  The output product
+// takes 16 columns at a time, eight keys each of two pages, again a block apart.  (Copying keys piece by
+// piece into one stride instead took a copy of 256 bytes 80 cycles of the warp that asks, 6,500 cycles a tile.)
+//
 // Masks matter in the tiles that hold drafted keys, the last one or two of an item.  There values
 // are looked at, too: a drafted value that is not finite would reach rows that do not see it (0 x
 // infinity), so it is taken as zero in the product and added, as what it is, to the rows that do see it.
 //
 // Every wait is bounded; a wait that runs out sets a status bit, the CTA lets its copies land, frees its
 // tensor memory and returns.
+#include "hx_mma.cuh"
 #include "hx_tcgen05.cuh"
 #include "hx_tree_attention.cuh"
 
@@ -35,7 +42,6 @@ constexpr int WARP_PAGES = 0, WARP_SCORES = 1, WARP_OUTPUT = 2, WARP_QUERIES = 3
 constexpr int THREADS = 256;
 constexpr int GROUP_STRIDE = 128;             // bytes from one 8-row core matrix to the next row group
 constexpr int CHUNK_STRIDE = BLOCK_M * 16;    // bytes from one 16-byte column of Q to the next
-constexpr int KEY_STRIDE = BLOCK_N * 16;      // ... and of the keys
 constexpr float RAISE_MAXIMUM_BY = 8.0f;      // log2 units a tile must exceed a row's reference by
 constexpr int CTAS_AN_SM = 2;
 constexpr int LEAST = 2;                      // key tiles of the shortest run
@@ -101,7 +107,7 @@ __device__ __forceinline__ bool not_finite(uint32_t bits16) { return (bits16 & 0
 // What is not finite among the drafted values that a row sees in the segment [c.tile, c.tile + count) is
 // added to the row as stored: whatever their weight, the sum is not finite either.
 template <int D>
-__device__ __noinline__ void add_not_finite(const TreeArgs& a, const TreeCursor& c, int count, int token, int row,
+__device__ __noinline__ void add_not_finite(const TreeArgs& a, TreeCursor c, int count, int token, int row,
                                             __nv_bfloat16* out, float* part) {
   const int first = max(c.context, c.tile * BLOCK_N);
   const int end = min(c.context + c.nodes, (c.tile + count) * BLOCK_N);
@@ -123,7 +129,8 @@ __device__ __noinline__ void add_not_finite(const TreeArgs& a, const TreeCursor&
 }
 
 template <int D>
-__global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
+    const __grid_constant__ TreeArgs a) {
   using Config = TreeTcConfig<D>;
   constexpr int K_STAGES = Config::kKeyStages, V_STAGES = Config::kValueStages;
   constexpr int PIECES = D / 8;
@@ -131,13 +138,13 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
 
   // the run is found from the step's description, which was there before the kernel in front
   const TreeRun run = tree_run<BLOCK_N>(a, blockIdx.x, gridDim.x, LEAST);
+  TreeCursor at;
   if (run.count == 0) {      // before any barrier or allocation: the whole CTA leaves
     hx_pdl_wait();
+    if (threadIdx.x == 0) tree_tell_cut<BLOCK_M, BLOCK_N>(a, run, at, 0, blockIdx.x, gridDim.x);
     return;
   }
-  TreeCursor at;
-  long long item_begin;
-  tree_locate<BLOCK_N>(a, run.begin, at, item_begin);
+  tree_locate<BLOCK_N>(a, run.begin, at);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -189,6 +196,8 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   }
   if (warp == WARP_SCORES) tmem_alloc(tmem_holder, Config::kTmemColumns);
   hx_pdl_wait();
+  // (nothing to join unless the softmax gets to the end of the run and says otherwise)
+  if (threadIdx.x == 0) *tree_cut<BLOCK_M>(a, blockIdx.x, gridDim.x) = TreeCut{};
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -208,70 +217,85 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
 
   if (warp == WARP_PAGES) {
     // ------------------------------------------------------------ page requests
+    auto request_values = [&](int turn, long long block) {
+      const int stage = turn % V_STAGES;
+      if (!wait_for(&v_done[stage], static_cast<uint32_t>(turn / V_STAGES) + 1u)) return false;
+      const unsigned there = __ballot_sync(0xffffffffu, block >= 0);
+      if (lane == 0) mbar_expect_tx(&v_full[stage], __popc(there) * page_bytes);
+      __syncwarp();
+      if (block >= 0)
+        bulk_copy(smem_u32(v_stages + stage * Config::kHalfBytes) + lane * page_bytes,
+                  static_cast<const uint8_t*>(a.v_cache) + block, page_bytes, &v_full[stage]);
+      return true;
+    };
     // Turn t asks for the keys of turn t and for the values of turn t - 1, which are wanted later.
     // Lane p < pages_per_tile holds the block (of bytes into the layer's cache) of the turn's page p,
-    // -1 where there is none.
+    // -1 where there is none.  Page numbers are read 32 at a time, the next 32 while these are used, and the
+    // first of the next item while this one's are (a read at each turn held the copies up: 2,400 cycles a tile).
     TreeCursor c = at;
-    int asked = 0;                      // key tiles whose values' copies are on their way
-    int keys_asked = 0;
-    auto block_of = [&]() {
-      long long block = -1;
-      if (lane < pages_per_tile) {
-        const int index = c.tile * pages_per_tile + lane;
-        if (index * page_size < c.context + c.nodes) {
-          const int page = index < a.table_stride
-                               ? a.block_tables[static_cast<size_t>(a.request_table_row[c.request]) * a.table_stride + index]
-                               : -1;
-          if (page >= 0 && page < a.num_pages)
-            block = (static_cast<long long>(page) * a.kv_heads + c.kv_head(a)) * page_bytes;
-          else
-            atomicOr(a.status, HX_FLAG_BAD_PAGE);
-        }
-      }
-      return block;
+    int asked = 0, keys_asked = 0;      // key tiles whose copies are on their way
+    auto table_of = [&](const TreeCursor& of) {
+      return a.block_tables + static_cast<size_t>(a.request_table_row[of.request]) * a.table_stride;
     };
-    long long block = block_of(), value_block = -1;
+    auto pages_from = [&](const int* table, const TreeCursor& of, int first) {
+      const int index = first + lane;
+      return index < a.table_stride && index * page_size < of.context + of.nodes ? table[index] : -1;
+    };
     const uint8_t* k_cache = static_cast<const uint8_t*>(a.k_cache);
-    const uint8_t* v_cache = static_cast<const uint8_t*>(a.v_cache);
-    for (int turn = 0; turn <= run.count; ++turn) {
-      long long next_block = -1;
-      if (turn + 1 < run.count) {      // the next turn's pages, in flight during the waits
-        if (++c.tile == c.tiles) tree_next_item<BLOCK_N>(a, c);
-        next_block = block_of();
+    const int* table = table_of(c);
+    int pages = pages_from(table, c, c.tile * pages_per_tile / 32 * 32);
+    long long value_block = -1;
+    int turn = 0, left = run.count;
+    bool going = true;
+    while (left > 0 && going) {
+      const int count = min(c.tiles - c.tile, left);
+      TreeCursor next = c;
+      const int* next_table = table;
+      int next_item_pages = -1;
+      if (left > count) {
+        tree_next_item<BLOCK_N>(a, next);
+        if (next.request != c.request) next_table = table_of(next);
+        next_item_pages = pages_from(next_table, next, 0);
       }
-      if (turn < run.count) {
+      int window = c.tile * pages_per_tile / 32 * 32;
+      int next_pages = pages_from(table, c, window + 32);
+      const long long kv_head = c.kv_head(a);
+      for (int t = 0; t < count; ++t, ++turn) {
+        const int index = (c.tile + t) * pages_per_tile;      // of the tile's first page
+        if (index - window >= 32) {
+          window += 32;
+          pages = next_pages;
+          next_pages = pages_from(table, c, window + 32);
+        }
+        const int page = __shfl_sync(0xffffffffu, pages, (index - window + lane) & 31);
+        long long block = -1;
+        if (lane < pages_per_tile && (index + lane) * page_size < c.context + c.nodes) {
+          if (page >= 0 && page < a.num_pages) block = (page * static_cast<long long>(a.kv_heads) + kv_head) * page_bytes;
+          else atomicOr(a.status, HX_FLAG_BAD_PAGE);
+        }
         const int stage = turn % K_STAGES;
-        if (!wait_for(&k_done[stage], static_cast<uint32_t>(turn / K_STAGES) + 1u)) break;
+        going = wait_for(&k_done[stage], static_cast<uint32_t>(turn / K_STAGES) + 1u);
+        if (!going) break;
         const unsigned there = __ballot_sync(0xffffffffu, block >= 0);
         if (lane == 0) mbar_expect_tx(&k_full[stage], __popc(there) * page_bytes);
         __syncwarp();
-        const uint32_t target = smem_u32(k_stages + stage * Config::kHalfBytes);
-        if (page_size == BLOCK_N) {      // a page's block is laid out as the product wants it
-          if (lane == 0 && there != 0u) bulk_copy(target, k_cache + block, page_bytes, &k_full[stage]);
-        } else {                         // (2 or 4 pages: a lane's copies are all of one page)
-          const int p = lane % pages_per_tile;
-          const long long from = __shfl_sync(0xffffffffu, block, p);
-          for (int piece = lane / pages_per_tile; piece < PIECES && from >= 0; piece += 32 / pages_per_tile)
-            bulk_copy(target + piece * KEY_STRIDE + p * piece_stride, k_cache + from + piece * piece_stride,
-                      piece_stride, &k_full[stage]);
-          __syncwarp();
-        }
+        if (block >= 0)
+          bulk_copy(smem_u32(k_stages + stage * Config::kHalfBytes) + lane * page_bytes, k_cache + block, page_bytes,
+                    &k_full[stage]);
         ++keys_asked;
+        if (turn > 0) {
+          going = request_values(turn - 1, value_block);
+          if (!going) break;
+          ++asked;
+        }
+        value_block = block;
       }
-      if (turn > 0) {
-        const int stage = (turn - 1) % V_STAGES;
-        if (!wait_for(&v_done[stage], static_cast<uint32_t>((turn - 1) / V_STAGES) + 1u)) break;
-        const unsigned there = __ballot_sync(0xffffffffu, value_block >= 0);
-        if (lane == 0) mbar_expect_tx(&v_full[stage], __popc(there) * page_bytes);
-        __syncwarp();
-        if (value_block >= 0)
-          bulk_copy(smem_u32(v_stages + stage * Config::kHalfBytes) + lane * page_bytes, v_cache + value_block,
-                    page_bytes, &v_full[stage]);
-        ++asked;
-      }
-      value_block = block;
-      block = next_block;
+      left -= count;
+      c = next;
+      table = next_table;
+      pages = next_item_pages;
     }
+    if (going && request_values(turn - 1, value_block)) ++asked;
     // a CTA does not leave while copies into its shared memory are in flight
     if (*failed) {
       for (int t = max(0, keys_asked - K_STAGES); t < keys_asked; ++t)
@@ -295,31 +319,19 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       const int rows_here = rows.count;
       const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
                                static_cast<size_t>(c.q_begin + rows.token0) * a.ldq + static_cast<size_t>(rows.head0) * D;
-      // neighbouring lanes take eight rows' same piece; eight loads of a lane are in flight
-      constexpr int LOADS = 8;
+      // (asynchronous copies: all of a lane's are in flight together, without registers.  Eight at a time
+      // through registers took 25,000 cycles for 128 rows)
       const int items = (rows_here + 7) / 8 * PIECES * 8;
-      for (int base = 0; base < items; base += 32 * LOADS) {
-        uint4 value[LOADS];
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-          const int i = base + u * 32 + lane;
-          const int block = i >> 3, row_group = block / PIECES, piece = block - row_group * PIECES;
-          const int row = row_group * 8 + (i & 7);
-          value[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (i < items && row < rows_here) {
-            const int token = row / rows.heads;
-            value[u] = *reinterpret_cast<const uint4*>(q + static_cast<size_t>(token) * a.ldq +
-                                                       static_cast<size_t>(row - token * rows.heads) * D + piece * 8);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-          const int i = base + u * 32 + lane;
-          const int block = i >> 3, row_group = block / PIECES, piece = block - row_group * PIECES;
-          if (i < items)
-            *reinterpret_cast<uint4*>(q_tile + piece * CHUNK_STRIDE + row_group * GROUP_STRIDE + (i & 7) * 16) = value[u];
-        }
+      for (int i = lane; i < items; i += 32) {
+        const int block = i >> 3, row_group = block / PIECES, piece = block - row_group * PIECES;
+        const int row = row_group * 8 + (i & 7), token = row / rows.heads;
+        const bool there = row < rows_here;
+        hx_cp_async_16(smem_u32(q_tile + piece * CHUNK_STRIDE + row_group * GROUP_STRIDE + (i & 7) * 16),
+                       there ? q + static_cast<size_t>(token) * a.ldq + static_cast<size_t>(row - token * rows.heads) * D + piece * 8
+                             : q, there ? 16 : 0);
       }
+      hx_cp_async_commit();
+      hx_cp_async_wait<0>();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
@@ -329,9 +341,14 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   } else if (warp == WARP_SCORES) {
     // ------------------------------------------------------------ score products
     if (hx_elect_one()) {
-      constexpr uint32_t idesc = make_idesc(BLOCK_M, BLOCK_N);
+      // pages of 16 and 32: two products of 32 keys, the second `apart` bytes on
+      const bool halves = page_size == 16 || page_size == 32;
+      const uint32_t idesc = halves ? make_idesc(BLOCK_M, BLOCK_N / 2) : make_idesc(BLOCK_M, BLOCK_N);
+      const uint32_t apart = (page_size == 16 ? GROUP_STRIDE : page_bytes) >> 4;
+      const uint32_t key_step = (2 * piece_stride) >> 4;      // 16 coordinates on
       const uint64_t desc_q = make_smem_desc_plain(smem_u32(q_tile), CHUNK_STRIDE, GROUP_STRIDE);
-      const uint64_t desc_k0 = make_smem_desc_plain(smem_u32(k_stages), KEY_STRIDE, GROUP_STRIDE);
+      const uint64_t desc_k0 =
+          make_smem_desc_plain(smem_u32(k_stages), piece_stride, page_size >= 32 ? GROUP_STRIDE : page_bytes);
       TreeCursor c = at;
       int turn = 0, segment = 0;
       for (int left = run.count; left > 0 && !*failed; ++segment) {
@@ -347,8 +364,14 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
           const uint64_t desc_k = desc_k0 + stage * (Config::kHalfBytes >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem_base + b * BLOCK_N, desc_q + k * ((2 * CHUNK_STRIDE) >> 4),
-                      desc_k + k * ((2 * KEY_STRIDE) >> 4), idesc, k > 0 ? 1u : 0u);
+            umma_bf16(tmem_base + b * BLOCK_N, desc_q + k * ((2 * CHUNK_STRIDE) >> 4), desc_k + k * key_step, idesc,
+                      k > 0 ? 1u : 0u);
+          if (halves) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              umma_bf16(tmem_base + b * BLOCK_N + BLOCK_N / 2, desc_q + k * ((2 * CHUNK_STRIDE) >> 4),
+                        desc_k + apart + k * key_step, idesc, k > 0 ? 1u : 0u);
+          }
           umma_commit(&s_full[b]);
           umma_commit(&k_done[stage]);
           if (t == count - 1) umma_commit(q_done);
@@ -365,12 +388,14 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
     // ----------------------------------------------------------- output products
     if (hx_elect_one()) {
       constexpr uint32_t idesc = make_idesc_b_mn_major(BLOCK_M, D);
-      // values: MN-major, the next 8 keys are 128 bytes on, the next 8 coordinates one piece on
-      const uint64_t desc_v0 = make_smem_desc_plain(smem_u32(v_stages), GROUP_STRIDE, piece_stride);
+      // values: MN-major, the next 8 keys are 128 bytes or a block on, the next 8 coordinates one piece on
+      const uint64_t desc_v0 =
+          make_smem_desc_plain(smem_u32(v_stages), page_size >= 32 ? GROUP_STRIDE : page_bytes, piece_stride);
       uint32_t value_step[BLOCK_N / 16];
 #pragma unroll
       for (int g = 0; g < BLOCK_N / 16; ++g)
-        value_step[g] = ((g * 16 / page_size) * page_bytes + (g * 16 % page_size) * 16) >> 4;
+        value_step[g] = (page_size == 16 ? 2 * (g & 1) * page_bytes + (g >> 1) * GROUP_STRIDE
+                                         : (g * 16 / page_size) * page_bytes + (g * 16 % page_size) * 16) >> 4;
       const uint32_t target = tmem_base + Config::kOutputColumn;
       TreeCursor c = at;
       int turn = 0;
@@ -441,7 +466,12 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
           }
           if (drafted) {
             const unsigned long long mask = tree_mask(a, c, my_token, key0);
-            const uint32_t low = static_cast<uint32_t>(mask), high = static_cast<uint32_t>(mask >> 32);
+            uint32_t low = static_cast<uint32_t>(mask), high = static_cast<uint32_t>(mask >> 32);
+            if (page_size == 16) {      // the order of the columns
+              const uint32_t even = __byte_perm(low, high, 0x6420);
+              high = __byte_perm(low, high, 0x7531);
+              low = even;
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               if (!((low >> i) & 1)) p[i] = -INFINITY;
@@ -569,7 +599,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
         const float inverse = row_sum > 0.0f ? 1.0f / row_sum : 0.0f;
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(c.q_begin + my_token) * a.ldo +
                              static_cast<size_t>(my_head) * D;
-        float* part = a.partial + (2ll * blockIdx.x + (c.tile == 0 ? 1 : 0)) * tree_part_floats<BLOCK_M>(D);
+        float* part = tree_part<BLOCK_M>(a, blockIdx.x, c.tile == 0);
 #pragma unroll
         for (int d0 = 0; d0 < D; d0 += 16) {
           float o[16];
@@ -609,6 +639,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       }
       left -= count;
       if (left > 0) tree_next_item<BLOCK_N>(a, c);
+      else if (row == 0) tree_tell_cut<BLOCK_M, BLOCK_N>(a, run, c, count, blockIdx.x, gridDim.x);
     }
   }
 
@@ -640,11 +671,11 @@ int launch(const TreeArgs& a, int ctas, cudaStream_t stream) {
 
 bool hx_tree_tc_takes(int head_dim, int page_size) {
   return head_dim >= 64 && head_dim <= 128 && head_dim % 16 == 0 &&
-         (page_size == 16 || page_size == 32 || page_size == 64);
+         (page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64);
 }
 
 long long hx_tree_tc_floats(int head_dim) {
-  return 2ll * hx_device_sm_count() * CTAS_AN_SM * tree_part_floats<BLOCK_M>(head_dim);
+  return tree_scratch_floats<BLOCK_M>(head_dim, hx_device_sm_count() * CTAS_AN_SM);
 }
 
 int hx_tree_tc_launch(TreeArgs a, cudaStream_t stream) {
@@ -659,5 +690,5 @@ int hx_tree_tc_launch(TreeArgs a, cudaStream_t stream) {
     default: rc = launch<128>(a, ctas, stream); break;
   }
   if (rc != HX_OK) return rc;
-  return hx_tree_join(a, HX_BF16, ctas, LEAST, BLOCK_M, BLOCK_N, 4, stream);
+  return hx_tree_join(a, HX_BF16, ctas, BLOCK_M, stream);
 }

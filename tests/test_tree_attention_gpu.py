@@ -29,7 +29,8 @@ DTYPES = [torch.bfloat16, torch.float32]
     ([50], [3], 260, 2, 64, 16),                               # a token's heads take two tiles
     ([50, 7], [6, 3], 2, 1, 160, 16),                          # heads of other kernels
     ([50, 7], [40, 3], 2, 1, 256, 32),
-    ([50, 70], [6, 33], 4, 2, 64, 8),                          # pages no tensor-core kernel takes
+    ([50, 700], [6, 33], 4, 2, 64, 8),
+    ([50, 70], [6, 33], 4, 2, 64, 24),                         # pages no tensor-core kernel takes
     ([50, 70], [6, 3], 4, 2, 100, 7),
     ([50, 70], [6, 3], 4, 2, 300, 8),
     ([50, 70], [6, 3], 4, 4, 6, 1),
