@@ -45,6 +45,7 @@ SOURCES = (
     "hx_attention_mma.cu",
     "hx_attention_tc.cu",
     "hx_tree_attention.cu",
+    "hx_tree_attention_stream.cu",
     "hx_tree_attention_tc.cu",
     "hx_verify.cu",
     "hx_cache_rows.cu",

@@ -12,7 +12,8 @@
 // CTA takes the tokens of a request (and the query heads that share a key/value head) as rows of
 // one tile and reads every key once for all of them; a long context is cut over CTAs (see
 // hx_tree_attention.cuh).  Three kernels:
-//   * hx_tree_attention_tc.cu: bfloat16, heads of 64 to 128, pages of 8, 16, 32 or 64 keys;
+//   * hx_tree_attention_stream.cu: bfloat16, heads of 64 to 128, pages of 8, 16 or 32 keys, few rows;
+//   * hx_tree_attention_tc.cu: the same with many rows, and pages of 64;
 //   * tree_tile_kernel: any other page size, float32 or bfloat16, heads up to 256 in steps of 4.
 //     32 rows by 64 keys at a time on the CUDA cores, all in float32;
 //   * tree_row_kernel: what is left (heads up to 1,024, even), a row a warp.
@@ -65,13 +66,10 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
   float* probabilities = values + TILE_KEYS * (D + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TreeRun run = tree_run<TILE_KEYS>(a, blockIdx.x, gridDim.x, TILE_LEAST);
+  if (threadIdx.x == 0) tree_tell_none<TILE_ROWS>(a);
+  if (run.count == 0) return;
   TreeCursor c;
-  if (run.count > 0) {
-    tree_locate<TILE_KEYS>(a, run.begin, c);
-  } else {
-    if (threadIdx.x == 0) tree_tell_cut<TILE_ROWS, TILE_KEYS>(a, run, c, 0, blockIdx.x, gridDim.x);
-    return;
-  }
+  tree_locate<TILE_KEYS>(a, run.begin, c);
   const int chunk = hx_cache_chunk(sizeof(T), D);
   const T* q = static_cast<const T*>(a.q);
   const T* k_cache = static_cast<const T*>(a.k_cache);
@@ -245,7 +243,7 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
     }
     left -= count;
     if (left > 0) tree_next_item<TILE_KEYS>(a, c);
-    else if (threadIdx.x == 0) tree_tell_cut<TILE_ROWS, TILE_KEYS>(a, run, c, count, blockIdx.x, gridDim.x);
+    else if (threadIdx.x == 0) tree_tell_cut<TILE_ROWS>(a, run, c, count);
   }
 }
 
@@ -262,13 +260,10 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void tree_row_kernel(const TreeArgs
   hx_pdl_prologue();
   const int D = a.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TreeRun run = tree_run<ROW_KEYS>(a, blockIdx.x, gridDim.x, ROW_LEAST);
+  if (threadIdx.x == 0) tree_tell_none<ROW_WARPS>(a);
+  if (run.count == 0) return;
   TreeCursor c;
-  if (run.count > 0) {
-    tree_locate<ROW_KEYS>(a, run.begin, c);
-  } else {
-    if (threadIdx.x == 0) tree_tell_cut<ROW_WARPS, ROW_KEYS>(a, run, c, 0, blockIdx.x, gridDim.x);
-    return;
-  }
+  tree_locate<ROW_KEYS>(a, run.begin, c);
   const int chunk = hx_cache_chunk(sizeof(T), D);
   const T* k_cache = static_cast<const T*>(a.k_cache);
   const T* v_cache = static_cast<const T*>(a.v_cache);
@@ -375,69 +370,173 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void tree_row_kernel(const TreeArgs
     }
     left -= count;
     if (left > 0) tree_next_item<ROW_KEYS>(a, c);
-    else if (threadIdx.x == 0) tree_tell_cut<ROW_WARPS, ROW_KEYS>(a, run, c, count, blockIdx.x, gridDim.x);
+    else if (threadIdx.x == 0) tree_tell_cut<ROW_WARPS>(a, run, c, count);
   }
 }
 
 // ------------------------------------------------------------------ joining parts
 
-constexpr int JOIN_THREADS = 256;
-constexpr int JOIN_LOADS = 8;      // parts whose loads are in flight together
+constexpr int JOIN_WARPS = 8, JOIN_THREADS = 32 * JOIN_WARPS;
+constexpr int JOIN_ALONE = 4;      // parts that a thread joins by itself
+constexpr int JOIN_CTAS = 3;       // an SM
 
-// Block (x, y): the y-th share of the coordinates of the item that begins in the run of CTA x and goes
-// on behind it, if there is one.  Its parts: what CTA x left in its place 1, and what the CTAs behind it
-// left in their place 0, joined in that order.
-template <typename T, int ROWS, int VEC>
-__global__ __launch_bounds__(JOIN_THREADS) void tree_join_kernel(const TreeArgs a) {
-  hx_pdl_prologue();
-  const int owner = blockIdx.x, ctas = gridDim.x, D = a.head_dim;
-  const TreeCut cut = *tree_cut<ROWS>(a, owner, ctas);
-  if (cut.parts == 0) return;
+// COUNT coordinates of a row out of some parts: sums against the largest of their maxima.
+template <int COUNT>
+struct Joined {
+  float top = -INFINITY, sum = 0.0f, acc[COUNT] = {};
+  __device__ __forceinline__ void add(float m, float l, const float (&o)[COUNT]) {
+    if (m == -INFINITY) return;      // no part, or one whose row saw nothing
+    const float new_top = fmaxf(top, m);
+    const float keep = exp2f(top - new_top), take = exp2f(m - new_top);
+    top = new_top;
+    sum = fmaf(sum, keep, l * take);
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) acc[e] = fmaf(acc[e], keep, o[e] * take);
+  }
+};
+
+// Parts [begin, end) of a row's coordinates from COUNT * group on; the loads of LOADS parts are in
+// flight together.  A piece (VEC coordinates) behind the last is the last one again.
+template <int ROWS, int VEC, int COUNT, int LOADS>
+__device__ __forceinline__ Joined<COUNT> join_parts(const TreeArgs& a, int owner, int begin, int end, int row,
+                                                    int group) {
+  const int D = a.head_dim;
   const long long stride = tree_part_floats<ROWS>(D);
-  const float* first = a.partial + (2ll * owner + 1) * stride;
-  const float* others = a.partial + 2ll * (owner + 1) * stride;
-  auto part_of = [&](int index) { return index == 0 ? first : others + 2ll * (index - 1) * stride; };
-  const int pieces = D / VEC;
-  for (int i = blockIdx.y * JOIN_THREADS + threadIdx.x; i < cut.rows * pieces; i += gridDim.y * JOIN_THREADS) {
-    const int piece = i / cut.rows, row = i - piece * cut.rows;
-    float total_max = -INFINITY, total_sum = 0.0f, acc[VEC];
+  Joined<COUNT> joined;
+  for (int base = begin; base < end; base += LOADS) {
+    float m[LOADS], l[LOADS], o[LOADS][COUNT];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
-    for (int base = 0; base < cut.parts; base += JOIN_LOADS) {
-      float m[JOIN_LOADS], l[JOIN_LOADS], o[JOIN_LOADS][VEC];
+    for (int u = 0; u < LOADS; ++u) {
+      m[u] = -INFINITY;
+      if (base + u < end) {
+        const int index = base + u;
+        const float* part = a.partial + (index == 0 ? 2ll * owner + 1 : 2ll * (owner + index)) * stride;
+        m[u] = __ldcg(part + D * ROWS + row);
+        l[u] = __ldcg(part + (D + 1) * ROWS + row);
 #pragma unroll
-      for (int u = 0; u < JOIN_LOADS; ++u) {
-        m[u] = -INFINITY;
-        if (base + u < cut.parts) {
-          const float* part = part_of(base + u);
-          m[u] = __ldcg(part + D * ROWS + row);
-          l[u] = __ldcg(part + (D + 1) * ROWS + row);
-          const float* at = part + (piece * ROWS + row) * VEC;
+        for (int p = 0; p < COUNT / VEC; ++p) {
+          const float* at = part + (min(group * (COUNT / VEC) + p, D / VEC - 1) * ROWS + row) * VEC;
           if constexpr (VEC == 4) {
             const float4 v = __ldcg(reinterpret_cast<const float4*>(at));
-            o[u][0] = v.x; o[u][1] = v.y; o[u][2] = v.z; o[u][3] = v.w;
+            o[u][4 * p] = v.x; o[u][4 * p + 1] = v.y; o[u][4 * p + 2] = v.z; o[u][4 * p + 3] = v.w;
           } else {
             const float2 v = __ldcg(reinterpret_cast<const float2*>(at));
-            o[u][0] = v.x; o[u][1] = v.y;
+            o[u][2 * p] = v.x; o[u][2 * p + 1] = v.y;
           }
         }
       }
-#pragma unroll
-      for (int u = 0; u < JOIN_LOADS; ++u) {
-        if (m[u] == -INFINITY) continue;      // no part, or one whose row saw nothing
-        const float new_max = fmaxf(total_max, m[u]);
-        const float keep = exp2f(total_max - new_max), take = exp2f(m[u] - new_max);
-        total_max = new_max;
-        total_sum = fmaf(total_sum, keep, l[u] * take);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] = fmaf(acc[e], keep, o[u][e] * take);
-      }
     }
-    const float inverse = total_sum > 0.0f ? 1.0f / total_sum : 0.0f;
-    T* out = static_cast<T*>(a.out) + static_cast<size_t>(cut.token + row / cut.heads) * a.ldo +
-             static_cast<size_t>(cut.head0 + row % cut.heads) * D + piece * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) out[e] = hx_from_float<T>(acc[e] * inverse);
+    for (int u = 0; u < LOADS; ++u) joined.add(m[u], l[u], o[u]);
+  }
+  return joined;
+}
+
+template <typename T, int COUNT>
+__device__ __forceinline__ void store_joined(const TreeArgs& a, const TreeCut& cut, int row, int group,
+                                             const Joined<COUNT>& joined) {
+  const float inverse = joined.sum > 0.0f ? 1.0f / joined.sum : 0.0f;
+  T* out = static_cast<T*>(a.out) + static_cast<size_t>(cut.token + row / cut.heads) * a.ldo +
+           static_cast<size_t>(cut.head0 + row % cut.heads) * a.head_dim + group * COUNT;
+  const int here = a.head_dim - group * COUNT;
+  // (where whole vectors fit: the tensor cores' kernels see to it that rows are aligned)
+  if (sizeof(T) == 2 && COUNT % 4 == 0 && a.head_dim % COUNT == 0 &&
+      (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+#pragma unroll
+    for (int e = 0; e + 3 < COUNT; e += 4) {
+      const __nv_bfloat162 low = __floats2bfloat162_rn(joined.acc[e] * inverse, joined.acc[e + 1] * inverse);
+      const __nv_bfloat162 high = __floats2bfloat162_rn(joined.acc[e + 2] * inverse, joined.acc[e + 3] * inverse);
+      *reinterpret_cast<uint2*>(out + e) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&low), *reinterpret_cast<const uint32_t*>(&high));
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < COUNT; ++e)
+    if (e < here) out[e] = hx_from_float<T>(joined.acc[e] * inverse);
+}
+
+// Every block makes a list of the cut items and the blocks share them out.  An item of few parts (there
+// are many such items): a thread joins them all, for 16 coordinates of a row, so that maxima and weights
+// are read once for them.  One of more (a long context of few requests): the warps of a block take runs
+// of the parts, a thread 4 coordinates.  Neighbouring lanes have neighbouring rows.  Always joined in
+// ascending order of the keys.
+template <typename T, int ROWS, int VEC>
+__global__ __launch_bounds__(JOIN_THREADS, JOIN_CTAS) void tree_join_kernel(const TreeArgs a, int ctas) {
+  constexpr int ALONE = 16, SHARED = 4;          // coordinates of a thread
+  __shared__ short list[TREE_MOST_CTAS];         // items of few parts from the front, of many from the back
+  __shared__ short parts_of[TREE_MOST_CTAS];
+  __shared__ TreeCut cuts[TREE_MOST_CTAS];
+  __shared__ int few_of[JOIN_WARPS], many_of[JOIN_WARPS];
+  __shared__ float met[JOIN_WARPS][SHARED + 2][32];
+  hx_pdl_prologue();
+  const int D = a.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int few = 0, many = 0;
+  for (int base = 0; base < ctas; base += JOIN_THREADS) {
+    const int owner = base + threadIdx.x;
+    int parts = 0;
+    if (owner < ctas) {      // (a cut that is none may be anything)
+      parts = __ldcg(tree_cut_parts<ROWS>(a, ctas) + owner);
+      const int4 cut = __ldcg(reinterpret_cast<const int4*>(tree_cuts<ROWS>(a, ctas) + owner));
+      cuts[owner] = TreeCut{cut.x, cut.y, cut.z, cut.w};
+      parts_of[owner] = static_cast<short>(parts);
+    }
+    const unsigned is_few = __ballot_sync(0xffffffffu, parts > 0 && parts <= JOIN_ALONE);
+    const unsigned is_many = __ballot_sync(0xffffffffu, parts > JOIN_ALONE);
+    if (lane == 0) {
+      few_of[warp] = __popc(is_few);
+      many_of[warp] = __popc(is_many);
+    }
+    __syncthreads();
+    const unsigned below = (1u << lane) - 1;
+    int my_few = few + __popc(is_few & below), my_many = many + __popc(is_many & below);
+    for (int w = 0; w < JOIN_WARPS; ++w) {
+      if (w < warp) my_few += few_of[w], my_many += many_of[w];
+      few += few_of[w];
+      many += many_of[w];
+    }
+    if ((is_few >> lane) & 1) list[my_few] = static_cast<short>(owner);
+    if ((is_many >> lane) & 1) list[TREE_MOST_CTAS - 1 - my_many] = static_cast<short>(owner);
+    __syncthreads();
+  }
+  const int slots = ROWS * ((D + ALONE - 1) / ALONE);      // of an item
+  for (int s = blockIdx.x * JOIN_THREADS + threadIdx.x; s < few * slots; s += gridDim.x * JOIN_THREADS) {
+    const int owner = list[s / slots], at = s % slots, group = at / ROWS, row = at % ROWS;
+    const TreeCut cut = cuts[owner];
+    if (row < cut.rows)
+      store_joined<T, ALONE>(a, cut, row, group,
+                             join_parts<ROWS, VEC, ALONE, 2>(a, owner, 0, parts_of[owner], row, group));
+  }
+  constexpr int LANE_ROWS = ROWS < 32 ? ROWS : 32, LANE_GROUPS = 32 / LANE_ROWS;      // of a warp
+  const int groups = (D + SHARED - 1) / SHARED;
+  const int units = (ROWS / LANE_ROWS) * ((groups + LANE_GROUPS - 1) / LANE_GROUPS);
+  for (int u = blockIdx.x; u < many * units; u += gridDim.x) {
+    const int owner = list[TREE_MOST_CTAS - 1 - u / units], parts = parts_of[owner], unit = u % units;
+    const TreeCut cut = cuts[owner];
+    const int row = unit % (ROWS / LANE_ROWS) * LANE_ROWS + lane % LANE_ROWS;
+    const int group = unit / (ROWS / LANE_ROWS) * LANE_GROUPS + lane / LANE_ROWS;
+    const bool mine = row < cut.rows && group < groups;
+    Joined<SHARED> joined;
+    if (mine)
+      joined = join_parts<ROWS, VEC, SHARED, 8>(a, owner, parts * warp / JOIN_WARPS, parts * (warp + 1) / JOIN_WARPS,
+                                                row, group);
+    met[warp][0][lane] = joined.top;
+    met[warp][1][lane] = joined.sum;
+#pragma unroll
+    for (int e = 0; e < SHARED; ++e) met[warp][2 + e][lane] = joined.acc[e];
+    __syncthreads();
+    if (warp == 0 && mine) {
+      Joined<SHARED> total;
+#pragma unroll
+      for (int w = 0; w < JOIN_WARPS; ++w) {
+        float o[SHARED];
+#pragma unroll
+        for (int e = 0; e < SHARED; ++e) o[e] = met[w][2 + e][lane];
+        total.add(met[w][0][lane], met[w][1][lane], o);
+      }
+      store_joined<T, SHARED>(a, cut, row, group, total);
+    }
+    __syncthreads();
   }
 }
 
@@ -459,6 +558,9 @@ int launch_tile(const TreeArgs& a, int ctas, cudaStream_t stream) {
   return HX_OK;
 }
 
+// Where the streaming kernel still beats the tcgen05 one (see STREAM figures in hx_tree_attention_stream.cu).
+constexpr int STREAM_MOST_ROWS = 32;
+
 // Which kernel: the tensor cores', the tile kernel, or the row kernel.
 enum TreeKernel { TREE_TC, TREE_TILE, TREE_ROW };
 TreeKernel kernel_for(int dtype, int head_dim, int page_size) {
@@ -469,20 +571,18 @@ TreeKernel kernel_for(int dtype, int head_dim, int page_size) {
 
 }  // namespace
 
-int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int rows, cudaStream_t stream) {
-  // shares of an item: of 128 rows, two pieces of coordinates a thread
-  const dim3 grid(ctas, rows >= 128 ? 8 : rows >= 32 ? 4 : 1);
+int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int rows, int vec, cudaStream_t stream) {
+  HX_REQUIRE(ctas <= TREE_MOST_CTAS, "hx_tree_attention: a grid of %d CTAs", ctas);
+  const int grid = hx_device_sm_count() * JOIN_CTAS;
   const bool half = dtype == HX_BF16;
-  if (rows == 128)
-    hx_launch(tree_join_kernel<__nv_bfloat16, 128, 4>, grid, JOIN_THREADS, 0, stream, a);
-  else if (rows == TILE_ROWS && half)
-    hx_launch(tree_join_kernel<__nv_bfloat16, TILE_ROWS, 4>, grid, JOIN_THREADS, 0, stream, a);
-  else if (rows == TILE_ROWS)
-    hx_launch(tree_join_kernel<float, TILE_ROWS, 4>, grid, JOIN_THREADS, 0, stream, a);
-  else if (half)
-    hx_launch(tree_join_kernel<__nv_bfloat16, ROW_WARPS, 2>, grid, JOIN_THREADS, 0, stream, a);
-  else
-    hx_launch(tree_join_kernel<float, ROW_WARPS, 2>, grid, JOIN_THREADS, 0, stream, a);
+  auto run = [&](auto kernel) { hx_launch(kernel, grid, JOIN_THREADS, 0, stream, a, ctas); };
+  if (half && rows == 128) run(tree_join_kernel<__nv_bfloat16, 128, 4>);
+  else if (half && rows == 32 && vec == 2) run(tree_join_kernel<__nv_bfloat16, 32, 2>);
+  else if (half && rows == 16) run(tree_join_kernel<__nv_bfloat16, 16, 2>);
+  else if (half && rows == TILE_ROWS) run(tree_join_kernel<__nv_bfloat16, TILE_ROWS, 4>);
+  else if (rows == TILE_ROWS) run(tree_join_kernel<float, TILE_ROWS, 4>);
+  else if (half) run(tree_join_kernel<__nv_bfloat16, ROW_WARPS, 2>);
+  else run(tree_join_kernel<float, ROW_WARPS, 2>);
   HX_CHECK_LAUNCH("hx_tree_attention");
   return HX_OK;
 }
@@ -497,7 +597,11 @@ HX_API long long hx_tree_attention_scratch_floats(int dtype, int heads, int kv_h
   const int sms = hx_device_sm_count();
   if (sms <= 0) return -1;
   switch (kernel_for(dtype, head_dim, page_size)) {
-    case TREE_TC: return hx_tree_tc_floats(head_dim);
+    case TREE_TC: {      // (or the streaming kernel, as the trees are)
+      const long long tc = hx_tree_tc_floats(head_dim);
+      const long long stream = hx_tree_stream_takes(head_dim, page_size) ? hx_tree_stream_floats(head_dim) : 0;
+      return tc > stream ? tc : stream;
+    }
     case TREE_TILE: return tree_scratch_floats<TILE_ROWS>(head_dim, sms * tile_ctas_an_sm(head_dim));
     default: return tree_scratch_floats<ROW_WARPS>(head_dim, sms * ROW_CTAS);
   }
@@ -505,15 +609,16 @@ HX_API long long hx_tree_attention_scratch_floats(int dtype, int heads, int kv_h
 
 // out[t, h D .. (h + 1) D) for every token t of the requests; see the head of this file.  visible:
 // [tokens, ld_visible] of 64-bit words, `words` of them a token, bit j of word w: the token sees
-// drafted token 64 w + j of its request.  partial: hx_tree_attention_scratch_floats() floats.  Rows of
+// drafted token 64 w + j of its request.  max_nodes: the most tokens a request brings, which a kernel
+// is chosen by (any number gives the right result; 0: not known).  partial: hx_tree_attention_scratch_floats() floats.  Rows of
 // `out` behind request_start[requests] are left as they are.
 HX_API int hx_tree_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int dtype,
                              const long long* visible, int ld_visible, int words,
                              const int* request_start, const int* request_context,
                              const int* request_table_row, const int* block_tables, int table_stride,
                              void* out, int ldo, float* partial, int requests, int heads, int kv_heads,
-                             int head_dim, int page_size, int num_pages, float scale, int* status,
-                             cudaStream_t stream) {
+                             int head_dim, int page_size, int num_pages, float scale, int max_nodes,
+                             int* status, cudaStream_t stream) {
   HX_REQUIRE(dtype == HX_F32 || dtype == HX_BF16, "hx_tree_attention: unknown dtype %d", dtype);
   HX_REQUIRE(requests >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && page_size > 0,
              "hx_tree_attention: bad sizes");
@@ -539,6 +644,9 @@ HX_API int hx_tree_attention(const void* q, int ldq, const void* k_cache, const 
   if (kernel == TREE_TC) {
     HX_REQUIRE(ldq % 8 == 0 && ldo % 8 == 0 && aligned(q, 16) && aligned(out, 16),
                "hx_tree_attention: q and out must be 16-byte aligned, row strides multiples of 8");
+    const long long rows = static_cast<long long>(max_nodes) * (heads / kv_heads);
+    if (hx_tree_stream_takes(head_dim, page_size) && rows > 0 && rows <= STREAM_MOST_ROWS)
+      return hx_tree_stream_launch(a, static_cast<int>(rows), stream);
     return hx_tree_tc_launch(a, stream);
   }
   if (kernel == TREE_TILE) {
@@ -552,12 +660,12 @@ HX_API int hx_tree_attention(const void* q, int ldq, const void* k_cache, const 
     else
       rc = head_dim <= 128 ? launch_tile<float, 128>(a, ctas, stream) : launch_tile<float, 256>(a, ctas, stream);
     if (rc != HX_OK) return rc;
-    return hx_tree_join(a, dtype, ctas, TILE_ROWS, stream);
+    return hx_tree_join(a, dtype, ctas, TILE_ROWS, 4, stream);
   }
   tree_fill_rows(a, ROW_WARPS);
   const int ctas = sms * ROW_CTAS;
   if (dtype == HX_BF16) hx_launch(tree_row_kernel<__nv_bfloat16>, ctas, ROW_WARPS * 32, 0, stream, a);
   else hx_launch(tree_row_kernel<float>, ctas, ROW_WARPS * 32, 0, stream, a);
   HX_CHECK_LAUNCH("hx_tree_attention");
-  return hx_tree_join(a, dtype, ctas, ROW_WARPS, stream);
+  return hx_tree_join(a, dtype, ctas, ROW_WARPS, 2, stream);
 }

@@ -153,14 +153,12 @@ struct TreeRun {
   int count;
 };
 
-// What the join needs to know of the item that begins in a CTA's run and goes on behind it; a CTA
-// without one says parts = 0.
-struct TreeCut {
-  int parts;                    // this CTA's and those of the CTAs behind it
-  int token, head0, heads;      // the row of `out` and the head of row 0, heads a token
-  int rows;
-  int unused[3];
+// What the join needs to know of the item that begins in a CTA's run and goes on behind it.
+struct alignas(16) TreeCut {
+  int token, head0;      // the row of `out` and the head of row 0
+  int heads, rows;       // heads a token, rows
 };
+constexpr int TREE_MOST_CTAS = 1024;
 template <int KEYS>
 __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int cta, int ctas, int least) {
   TreeRun run;
@@ -209,43 +207,55 @@ template <int ROWS>
 __host__ __device__ constexpr long long tree_part_floats(int head_dim) {
   return static_cast<long long>(ROWS) * (head_dim + 2);
 }
-// The scratch: two parts a CTA, behind them what each says about its cut item.
+// The scratch: two parts a CTA, behind them what each says about its cut item and, last, how many parts
+// that item has (0: there is none).
 template <int ROWS>
 __host__ __device__ constexpr long long tree_scratch_floats(int head_dim, int ctas) {
-  return ctas * (2 * tree_part_floats<ROWS>(head_dim) + static_cast<long long>(sizeof(TreeCut) / 4));
+  return ctas * (2 * tree_part_floats<ROWS>(head_dim) + static_cast<long long>(sizeof(TreeCut) / 4) + 1);
 }
 template <int ROWS>
-__device__ __forceinline__ TreeCut* tree_cut(const TreeArgs& a, int cta, int ctas) {
-  return reinterpret_cast<TreeCut*>(a.partial + ctas * 2 * tree_part_floats<ROWS>(a.head_dim)) + cta;
+__device__ __forceinline__ TreeCut* tree_cuts(const TreeArgs& a, int ctas) {
+  return reinterpret_cast<TreeCut*>(a.partial + ctas * 2 * tree_part_floats<ROWS>(a.head_dim));
+}
+template <int ROWS>
+__device__ __forceinline__ int* tree_cut_parts(const TreeArgs& a, int ctas) {
+  return reinterpret_cast<int*>(tree_cuts<ROWS>(a, ctas) + ctas);
 }
 template <int ROWS>
 __device__ __forceinline__ float* tree_part(const TreeArgs& a, int cta, bool item_begins) {
   return a.partial + (2ll * cta + (item_begins ? 1 : 0)) * tree_part_floats<ROWS>(a.head_dim);
 }
 
-// One thread says what the CTA's run leaves to the join: looked at from the run's last key tile.
-template <int ROWS, int KEYS>
+// One thread says that the CTA's run leaves nothing to the join: first of all, so that it holds
+// whatever comes between, ...
+template <int ROWS>
+__device__ __forceinline__ void tree_tell_none(const TreeArgs& a) {
+  tree_cut_parts<ROWS>(a, gridDim.x)[blockIdx.x] = 0;
+}
+// ... and at the run's end what it does leave, looked at from the last segment.
+template <int ROWS>
 __device__ __forceinline__ void tree_tell_cut(const TreeArgs& a, const TreeRun& run, const TreeCursor& last,
-                                              int last_count, int cta, int ctas) {
-  TreeCut cut = {};
-  if (run.count > 0 && last.tile == 0 && last_count < last.tiles) {
-    const TreeRows rows(a, last);
-    const long long item_end = run.begin + run.count - last_count + last.tiles;
-    cut.parts = static_cast<int>((item_end - 1) / run.per_cta) - cta + 1;
-    cut.token = last.q_begin + rows.token0;
-    cut.head0 = rows.head0;
-    cut.heads = rows.heads;
-    cut.rows = rows.count;
-  }
-  *tree_cut<ROWS>(a, cta, ctas) = cut;
+                                              int last_count) {
+  if (last.tile != 0 || last_count == last.tiles) return;
+  const TreeRows rows(a, last);
+  const long long item_end = run.begin + run.count - last_count + last.tiles;
+  tree_cuts<ROWS>(a, gridDim.x)[blockIdx.x] = TreeCut{last.q_begin + rows.token0, rows.head0, rows.heads, rows.count};
+  tree_cut_parts<ROWS>(a, gridDim.x)[blockIdx.x] =
+      static_cast<int>((item_end - 1) / run.per_cta) - static_cast<int>(blockIdx.x) + 1;
 }
 
 }  // namespace
 
-// Joins the parts that `ctas` CTAs of tiles of `rows` rows left, on the same stream behind them.
-int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int rows, cudaStream_t stream);
+// Joins the parts that `ctas` CTAs of tiles of `rows` rows left (`vec` coordinates side by side), on the
+// same stream behind them.
+int hx_tree_join(const TreeArgs& a, int dtype, int ctas, int rows, int vec, cudaStream_t stream);
 
 // The tcgen05 kernel (bfloat16): whether it takes these sizes, its scratch, its launch.
 bool hx_tree_tc_takes(int head_dim, int page_size);
 long long hx_tree_tc_floats(int head_dim);
 int hx_tree_tc_launch(TreeArgs a, cudaStream_t stream);
+
+// The streaming kernel (bfloat16), tiles of 16 or 32 rows; `rows`: of the largest tree.
+bool hx_tree_stream_takes(int head_dim, int page_size);
+long long hx_tree_stream_floats(int head_dim);
+int hx_tree_stream_launch(TreeArgs a, int rows, cudaStream_t stream);

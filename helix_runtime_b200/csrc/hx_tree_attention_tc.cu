@@ -141,7 +141,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   TreeCursor at;
   if (run.count == 0) {      // before any barrier or allocation: the whole CTA leaves
     hx_pdl_wait();
-    if (threadIdx.x == 0) tree_tell_cut<BLOCK_M, BLOCK_N>(a, run, at, 0, blockIdx.x, gridDim.x);
+    if (threadIdx.x == 0) tree_tell_none<BLOCK_M>(a);
     return;
   }
   tree_locate<BLOCK_N>(a, run.begin, at);
@@ -196,8 +196,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   }
   if (warp == WARP_SCORES) tmem_alloc(tmem_holder, Config::kTmemColumns);
   hx_pdl_wait();
-  // (nothing to join unless the softmax gets to the end of the run and says otherwise)
-  if (threadIdx.x == 0) *tree_cut<BLOCK_M>(a, blockIdx.x, gridDim.x) = TreeCut{};
+  if (threadIdx.x == 0) tree_tell_none<BLOCK_M>(a);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -639,7 +638,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       }
       left -= count;
       if (left > 0) tree_next_item<BLOCK_N>(a, c);
-      else if (row == 0) tree_tell_cut<BLOCK_M, BLOCK_N>(a, run, c, count, blockIdx.x, gridDim.x);
+      else if (row == 0) tree_tell_cut<BLOCK_M>(a, run, c, count);
     }
   }
 
@@ -658,7 +657,9 @@ int launch(const TreeArgs& a, int ctas, cudaStream_t stream) {
   static bool reserved = false;
   std::call_once(once, [] {
     reserved = cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    Config::kSmemBytes) == cudaSuccess;
+                                    Config::kSmemBytes) == cudaSuccess &&
+               cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared) == cudaSuccess;
     if (!reserved) cudaGetLastError();
   });
   HX_REQUIRE(reserved, "hx_tree_attention: cannot reserve %d bytes of shared memory", Config::kSmemBytes);
@@ -690,5 +691,5 @@ int hx_tree_tc_launch(TreeArgs a, cudaStream_t stream) {
     default: rc = launch<128>(a, ctas, stream); break;
   }
   if (rc != HX_OK) return rc;
-  return hx_tree_join(a, HX_BF16, ctas, BLOCK_M, stream);
+  return hx_tree_join(a, HX_BF16, ctas, BLOCK_M, 4, stream);
 }

@@ -392,8 +392,8 @@ def _declare(library: ctypes.CDLL) -> None:
     library.hx_tree_attention_scratch_floats.restype = _c_longlong
     library.hx_tree_attention.argtypes = [
         _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-        _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr,
-        _c_ptr]
+        _c_int, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int,
+        _c_ptr, _c_ptr]
     library.hx_tree_attention.restype = _c_int
     library.hx_copy_pages.argtypes = [_c_ptr, _c_int, _c_int, _c_longlong, _c_ptr, _c_ptr, _c_int, _c_ptr,
                                       _c_ptr]
@@ -1033,23 +1033,37 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
 # ----------------------------------------------------------------- trees of drafted tokens
 
-def _need_each(dtype: torch.dtype, names: str, *tensors: torch.Tensor) -> None:
+def _need_each(device: int, dtype: torch.dtype, names: str, *tensors: torch.Tensor) -> None:
     """Operands of one dtype on the current device, contiguous in their last dimension."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -2
-    for index, tensor in enumerate(tensors):
-        if tensor.dtype != dtype or tensor.stride(-1) != 1 or tensor.get_device() != device:
-            raise KernelError(f"{names.split()[index]} must be {dtype}, contiguous in its last dimension and on "
-                              "the current CUDA device")
+    for tensor in tensors:
+        if tensor.dtype != dtype or tensor.get_device() != device or tensor.stride(-1) != 1:
+            raise KernelError(f"{names}: each must be {dtype}, contiguous in its last dimension and on the "
+                              "current CUDA device")
+
+
+def _here(tensor: torch.Tensor) -> int:
+    """The current device, which ``tensor`` lies on."""
+    device = tensor.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        raise KernelError("the operands must be tensors on the current CUDA device")
+    return device
+
+
+_tree_scratch: dict = {}      # floats by sizes
 
 
 def tree_attention_scratch(dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int,
                            page_size: int) -> int:
     """Floats of scratch that :func:`tree_attention` needs for these sizes, whatever a step brings."""
-    floats = int(lib().hx_tree_attention_scratch_floats(dtype_code(dtype), heads, kv_heads, head_dim,
-                                                        page_size))
-    if floats < 0:
-        raise KernelError(f"no tree attention of {heads} heads of {head_dim} on {kv_heads} with pages "
-                          f"of {page_size}")
+    key = (dtype, heads, kv_heads, head_dim, page_size, torch.cuda.current_device())
+    floats = _tree_scratch.get(key)
+    if floats is None:
+        floats = int(lib().hx_tree_attention_scratch_floats(dtype_code(dtype), heads, kv_heads, head_dim,
+                                                            page_size))
+        if floats < 0:
+            raise KernelError(f"no tree attention of {heads} heads of {head_dim} on {kv_heads} with pages "
+                              f"of {page_size}")
+        _tree_scratch[key] = floats
     return floats
 
 
@@ -1058,7 +1072,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                    request_table_row: torch.Tensor, block_tables: torch.Tensor, out: torch.Tensor,
                    partial: Optional[torch.Tensor], requests: int, heads: int, kv_heads: int,
                    head_dim: int, page_size: int, num_pages: int, scale: float,
-                   status: torch.Tensor) -> None:
+                   status: torch.Tensor, max_nodes: int = 0) -> None:
     """Attention of drafted tokens: request ``r`` brings the tokens ``request_start[r]`` to
     ``request_start[r + 1]``, whose keys and values lie in its pages at the places behind its
     ``request_context[r]`` cached ones, in the order of the tokens.  A token sees every cached
@@ -1067,12 +1081,14 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     :func:`helix_runtime_b200.engine.step.ancestor_words`).  A token that sees nothing gets zeros.
     Rows of ``out`` behind the last request's are left as they are.  ``partial`` (float32,
     :func:`tree_attention_scratch` elements) is made here when it is not given; a call uses it from
-    its launch to its end, so calls that may run at the same time need one each."""
-    code = dtype_code(q.dtype)
-    _need_each(q.dtype, "q k_cache v_cache out", q, k_cache, v_cache, out)
-    _need_each(torch.int64, "visible", visible)
-    _need_each(torch.int32, "request_start request_context request_table_row block_tables status", request_start,
-               request_context, request_table_row, block_tables, status)
+    its launch to its end, so calls that may run at the same time need one each.  ``max_nodes``: the
+    most tokens a request brings, which the kernel is chosen by (any number gives the right result;
+    default: what ``q`` has a request)."""
+    device, code = _here(q), dtype_code(q.dtype)
+    _need_each(device, q.dtype, "q, k_cache, v_cache and out", q, k_cache, v_cache, out)
+    _need_each(device, torch.int64, "visible", visible)
+    _need_each(device, torch.int32, "request_start, request_context, request_table_row, block_tables and status",
+               request_start, request_context, request_table_row, block_tables, status)
     if visible.dim() != 2 or q.dim() != 2 or out.dim() != 2 or block_tables.dim() != 2:
         raise KernelError("visible is [tokens, words]; q, out and block_tables are matrices")
     if (visible.shape[0] < min(q.shape[0], out.shape[0]) or request_start.shape[0] <= requests
@@ -1081,19 +1097,19 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if min(q.shape[1], out.shape[1]) < heads * head_dim or \
             min(k_cache.numel(), v_cache.numel()) < num_pages * kv_heads * page_size * head_dim:
         raise KernelError("q and out hold the heads of a token in a row, the cache num_pages pages")
+    floats = tree_attention_scratch(q.dtype, heads, kv_heads, head_dim, page_size)
     if partial is None:
-        partial = torch.empty(tree_attention_scratch(q.dtype, heads, kv_heads, head_dim, page_size),
-                              dtype=torch.float32, device=q.device)
+        partial = torch.empty(floats, dtype=torch.float32, device=q.device)
     else:
-        _need_each(torch.float32, "partial", partial)
-        if partial.numel() < lib().hx_tree_attention_scratch_floats(code, heads, kv_heads, head_dim, page_size):
+        _need_each(device, torch.float32, "partial", partial)
+        if partial.numel() < floats:
             raise KernelError("partial is smaller than tree_attention_scratch says")
     _check(lib().hx_tree_attention(
         q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), code, visible.data_ptr(),
         visible.stride(0), visible.shape[1], request_start.data_ptr(), request_context.data_ptr(),
         request_table_row.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), out.data_ptr(),
         out.stride(0), partial.data_ptr(), requests, heads, kv_heads, head_dim, page_size, num_pages,
-        scale, status.data_ptr(), _stream()))
+        scale, max_nodes or -(-q.shape[0] // max(1, requests)), status.data_ptr(), _stream()))
 
 
 def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], token_ids: torch.Tensor,
@@ -1117,11 +1133,12 @@ def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], to
     id among the maxima).  Out, all int32: ``path`` ``[requests, width]``, the numbers of the
     tokens that stand, from 0 on, -1 behind them; ``kept`` how many they are; ``next_tokens``, -1
     (and FLAG_NONFINITE) when logits on the way are not finite.  A path that is full ends the walk."""
-    _need_each(torch.float32, "logits temperature uniform", logits, temperature, uniform)
-    _need_each(torch.int32, "token_ids parents request_start path kept next_tokens status", token_ids, parents,
-               request_start, path, kept, next_tokens, status)
+    device = _here(logits)
+    _need_each(device, torch.float32, "logits, temperature and uniform", logits, temperature, uniform)
+    _need_each(device, torch.int32, "token_ids, parents, request_start, path, kept, next_tokens and status",
+               token_ids, parents, request_start, path, kept, next_tokens, status)
     if draft_logits is not None:
-        _need_each(torch.float32, "draft_logits", draft_logits)
+        _need_each(device, torch.float32, "draft_logits", draft_logits)
         if draft_logits.shape != logits.shape:
             raise KernelError("draft_logits has a row of the vocabulary for every row of logits")
     tokens, vocab = logits.shape
@@ -1141,7 +1158,6 @@ def _storage_sizes(storage: torch.Tensor):
     """``[layers, 2, pages, kv_heads, page_size, head_dim]`` of a cache group's storage."""
     if storage.dim() != 6 or storage.shape[1] != 2 or not storage.is_contiguous():
         raise KernelError("storage is [layers, 2, pages, kv_heads, page_size, head_dim], contiguous")
-    _need_each(storage.dtype, "storage", storage)
     return storage.shape
 
 
@@ -1155,7 +1171,8 @@ def keep_rows(storage: torch.Tensor, block_tables: torch.Tensor, request_table_r
     whose path does not ascend, is longer than a row of ``path`` (FLAG_BAD_MOVE) or leads outside its
     pages (FLAG_BAD_PAGE) keeps its rows where they are.  Requests share no page they move rows in."""
     layers, _, pages, kv_heads, page_size, head_dim = _storage_sizes(storage)
-    _need_each(torch.int32, "block_tables request_table_row request_context path kept status", block_tables,
+    _need_each(_here(storage), torch.int32,
+               "block_tables, request_table_row, request_context, path, kept and status", block_tables,
                request_table_row, request_context, path, kept, status)
     if path.dim() != 2 or min(request_table_row.shape[0], request_context.shape[0], path.shape[0],
                               kept.shape[0]) < requests:
@@ -1174,7 +1191,7 @@ def copy_pages(storage: torch.Tensor, source: torch.Tensor, target: torch.Tensor
     pool is left out (FLAG_BAD_PAGE), and so is one whose target another pair writes or reads
     (FLAG_BAD_MOVE); a page copied onto itself stays."""
     layers, _, pages, kv_heads, page_size, head_dim = _storage_sizes(storage)
-    _need_each(torch.int32, "source target status", source, target, status)
+    _need_each(_here(storage), torch.int32, "source, target and status", source, target, status)
     if source.shape != target.shape or source.dim() != 1:
         raise KernelError("source and target are lists of pages of one length")
     _check(lib().hx_copy_pages(

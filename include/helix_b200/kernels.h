@@ -775,13 +775,14 @@ long long hx_tree_attention_scratch_floats(int dtype, int heads, int kv_heads, i
                                            int page_size);
 /* a request's drafted tokens over its cached keys and the drafted ones that a bit mask names;
  * visible: [tokens, ld_visible] 64-bit words, `words` of them a token, bit j of word w = token
- * 64 w + j of the request, whose key lies behind the request_context cached ones */
+ * 64 w + j of the request, whose key lies behind the request_context cached ones; max_nodes: the
+ * most tokens a request brings, which a kernel is chosen by (0: not known) */
 int hx_tree_attention(const void* q, int ldq, const void* k_cache, const void* v_cache, int dtype,
                       const long long* visible, int ld_visible, int words, const int* request_start,
                       const int* request_context, const int* request_table_row,
                       const int* block_tables, int table_stride, void* out, int ldo, float* partial,
                       int requests, int heads, int kv_heads, int head_dim, int page_size,
-                      int num_pages, float scale, int* status, cudaStream_t stream);
+                      int num_pages, float scale, int max_nodes, int* status, cudaStream_t stream);
 /* which drafted tokens stand against the target's logits, by the caller's uniform numbers, and the
  * token that follows the last of them; path: the numbers of those that stand, -1 behind them */
 int hx_verify_drafts(const float* logits, int ld, const float* draft, int ld_draft, int vocab,

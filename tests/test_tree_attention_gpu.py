@@ -127,6 +127,31 @@ def test_values_that_are_not_finite_reach_who_sees_them(dtype, head_dim, page, b
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("head_dim,page,nodes", [(128, 16, 12), (128, 16, 90), (128, 64, 12), (128, 24, 12), (6, 4, 12)])
+def test_cached_values_that_are_not_finite_reach_every_token(dtype, head_dim, page, nodes):
+    """Also where they share a tile of keys with drafted ones, and wherever the work is cut."""
+    for context, place in ((100, 99), (100, 3), (40, 33)):
+        batch = Batch(19, [context], [nodes], 2, 2, head_dim, page, dtype)
+        clean = Batch(19, [context], [nodes], 2, 2, head_dim, page, dtype)
+        clean.run(ops)
+        from plain_tree import to_cache
+        rows = torch.zeros((2, page, head_dim), dtype=dtype)
+        rows[0, place % page, 2] = float("inf")
+        rows[1, place % page, 4] = float("nan")
+        laid = to_cache(rows, dtype).to(batch.v.device)
+        page_id = int(batch.tables[batch.row[0], place // page])
+        batch.v[page_id] = torch.where(laid.ne(0), laid, batch.v[page_id])
+        batch.run(ops)
+        got, want = batch.out[:nodes, :2 * head_dim], clean.out[:nodes, :2 * head_dim]
+        # (a bfloat16 kernel's weight is a sum of two terms, hi + lo, of which lo may be zero or negative:
+        # hi * inf + lo * inf is then not a number.  So what reaches a token is not finite, and no more)
+        reached = ~got[:, 2].isfinite() if dtype == torch.bfloat16 else got[:, 2] == float("inf")
+        assert bool(reached.all()) and bool(got[:, head_dim + 4].isnan().all())
+        kept = [c for c in range(2 * head_dim) if c not in (2, head_dim + 4)]
+        assert torch.equal(got[:, kept], want[:, kept])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_scratch_needs_nothing_and_is_reused(dtype):
     floats = ops.tree_attention_scratch(dtype, 4, 4, 128, 16)
     partial = torch.full((floats + 1,), float("nan"), device="cuda:0")

@@ -39,8 +39,8 @@ def test_entry_points_refuse_sizes_on_the_host():
     def attention(dtype=1, words=1, ld=1, heads=4, kv_heads=2, dim=64, page=16, pages=8, stride=4, scale=1.0,
                   partial=some, status=some, requests=1, k=some):
         return library.hx_tree_attention(some, 256, k, some, dtype, some, ld, words, some, some, some, some, stride,
-                                         some, 256, partial, requests, heads, kv_heads, dim, page, pages, scale, status,
-                                         None)
+                                         some, 256, partial, requests, heads, kv_heads, dim, page, pages, scale, 0,
+                                         status, None)
 
     for changes in (dict(dtype=2), dict(words=0), dict(ld=0), dict(heads=3), dict(heads=0), dict(kv_heads=0),
                     dict(dim=0), dict(dim=7), dict(dim=1026), dict(page=0), dict(pages=0), dict(stride=0),
