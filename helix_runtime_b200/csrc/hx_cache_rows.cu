@@ -3,6 +3,10 @@
 // storage [layer, key|value, page, kv_head, (head_dim / c, slot, c)], see hx_cache_offset.
 //
 // Both are bound by memory: every byte is read once and written once.
+//
+// Neither lets the next kernel in before it has completed.  Attention fetches what earlier steps have left
+// in the cache before it waits for the kernel in front of it, and that one may have been let in
+// early, too: behind a kernel that moves cached rows nothing may start early.
 #include "hx_common.cuh"
 
 namespace {
@@ -18,7 +22,7 @@ template <typename Unit, int UNROLL>
 __global__ __launch_bounds__(THREADS) void copy_pages_kernel(uint8_t* storage, const int* source, const int* target,
                                                              int pairs, int num_pages, long long page_bytes,
                                                              int* status) {
-  hx_pdl_prologue();
+  hx_pdl_wait();      // (and lets nobody in early, see above)
   const int pair = blockIdx.y;
   const size_t plane = static_cast<size_t>(blockIdx.z) * num_pages;
   const int from = source[pair], to = target[pair];
@@ -89,7 +93,7 @@ struct KeepArgs {
 template <typename Unit>
 __global__ __launch_bounds__(THREADS) void keep_rows_kernel(const KeepArgs a) {
   constexpr int LOADS = 4;      // items whose rows are in flight together
-  hx_pdl_prologue();
+  hx_pdl_wait();      // (and lets nobody in early, see above)
   const int request = blockIdx.y;
   const int kept = a.kept[request];
   const int context = a.request_context[request];

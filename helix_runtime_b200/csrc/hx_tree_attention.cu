@@ -377,7 +377,8 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void tree_row_kernel(const TreeArgs
 // ------------------------------------------------------------------ joining parts
 
 constexpr int JOIN_WARPS = 8, JOIN_THREADS = 32 * JOIN_WARPS;
-constexpr int JOIN_ALONE = 4;      // parts that a thread joins by itself
+constexpr int JOIN_FEW = 4;        // parts that a thread joins for many coordinates
+constexpr int JOIN_SOME = 32;      // ... and for few
 constexpr int JOIN_CTAS = 3;       // an SM
 
 // COUNT coordinates of a row out of some parts: sums against the largest of their maxima.
@@ -456,22 +457,22 @@ __device__ __forceinline__ void store_joined(const TreeArgs& a, const TreeCut& c
     if (e < here) out[e] = hx_from_float<T>(joined.acc[e] * inverse);
 }
 
-// Every block makes a list of the cut items and the blocks share them out.  An item of few parts (there
+// Every block makes lists of the cut items and the blocks share them out.  An item of few parts (there
 // are many such items): a thread joins them all, for 16 coordinates of a row, so that maxima and weights
-// are read once for them.  One of more (a long context of few requests): the warps of a block take runs
-// of the parts, a thread 4 coordinates.  Neighbouring lanes have neighbouring rows.  Always joined in
-// ascending order of the keys.
+// are read once for them.  One of some more: the same for 4 coordinates, with more parts in flight.
+// One of many (a long context of few requests): the warps of a block take runs of the parts.
+// Neighbouring lanes have neighbouring rows.  Always joined in ascending order of the keys.
 template <typename T, int ROWS, int VEC>
 __global__ __launch_bounds__(JOIN_THREADS, JOIN_CTAS) void tree_join_kernel(const TreeArgs a, int ctas) {
-  constexpr int ALONE = 16, SHARED = 4;          // coordinates of a thread
-  __shared__ short list[TREE_MOST_CTAS];         // items of few parts from the front, of many from the back
+  constexpr int WIDE = 16, SLIM = 4;      // coordinates of a thread
+  __shared__ short lists[3][TREE_MOST_CTAS];
   __shared__ short parts_of[TREE_MOST_CTAS];
   __shared__ TreeCut cuts[TREE_MOST_CTAS];
-  __shared__ int few_of[JOIN_WARPS], many_of[JOIN_WARPS];
-  __shared__ float met[JOIN_WARPS][SHARED + 2][32];
+  __shared__ int of_warp[3][JOIN_WARPS];
+  __shared__ float met[JOIN_WARPS][SLIM + 2][32];
   hx_pdl_prologue();
   const int D = a.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int few = 0, many = 0;
+  int length[3] = {0, 0, 0};
   for (int base = 0; base < ctas; base += JOIN_THREADS) {
     const int owner = base + threadIdx.x;
     int parts = 0;
@@ -481,60 +482,68 @@ __global__ __launch_bounds__(JOIN_THREADS, JOIN_CTAS) void tree_join_kernel(cons
       cuts[owner] = TreeCut{cut.x, cut.y, cut.z, cut.w};
       parts_of[owner] = static_cast<short>(parts);
     }
-    const unsigned is_few = __ballot_sync(0xffffffffu, parts > 0 && parts <= JOIN_ALONE);
-    const unsigned is_many = __ballot_sync(0xffffffffu, parts > JOIN_ALONE);
-    if (lane == 0) {
-      few_of[warp] = __popc(is_few);
-      many_of[warp] = __popc(is_many);
+    const int which = parts == 0 ? -1 : parts <= JOIN_FEW ? 0 : parts <= JOIN_SOME ? 1 : 2;
+    unsigned mine[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      mine[k] = __ballot_sync(0xffffffffu, which == k);
+      if (lane == 0) of_warp[k][warp] = __popc(mine[k]);
     }
     __syncthreads();
-    const unsigned below = (1u << lane) - 1;
-    int my_few = few + __popc(is_few & below), my_many = many + __popc(is_many & below);
-    for (int w = 0; w < JOIN_WARPS; ++w) {
-      if (w < warp) my_few += few_of[w], my_many += many_of[w];
-      few += few_of[w];
-      many += many_of[w];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      int place = length[k] + __popc(mine[k] & ((1u << lane) - 1));
+      for (int w = 0; w < JOIN_WARPS; ++w) {
+        if (w < warp) place += of_warp[k][w];
+        length[k] += of_warp[k][w];
+      }
+      if (which == k) lists[k][place] = static_cast<short>(owner);
     }
-    if ((is_few >> lane) & 1) list[my_few] = static_cast<short>(owner);
-    if ((is_many >> lane) & 1) list[TREE_MOST_CTAS - 1 - my_many] = static_cast<short>(owner);
     __syncthreads();
   }
-  const int slots = ROWS * ((D + ALONE - 1) / ALONE);      // of an item
-  for (int s = blockIdx.x * JOIN_THREADS + threadIdx.x; s < few * slots; s += gridDim.x * JOIN_THREADS) {
-    const int owner = list[s / slots], at = s % slots, group = at / ROWS, row = at % ROWS;
+  const int thread = blockIdx.x * JOIN_THREADS + threadIdx.x, threads = gridDim.x * JOIN_THREADS;
+  const int wide_slots = ROWS * ((D + WIDE - 1) / WIDE), groups = (D + SLIM - 1) / SLIM;
+  for (int s = thread; s < length[0] * wide_slots; s += threads) {
+    const int owner = lists[0][s / wide_slots], at = s % wide_slots, group = at / ROWS, row = at % ROWS;
     const TreeCut cut = cuts[owner];
     if (row < cut.rows)
-      store_joined<T, ALONE>(a, cut, row, group,
-                             join_parts<ROWS, VEC, ALONE, 2>(a, owner, 0, parts_of[owner], row, group));
+      store_joined<T, WIDE>(a, cut, row, group,
+                            join_parts<ROWS, VEC, WIDE, 2>(a, owner, 0, parts_of[owner], row, group));
+  }
+  for (int s = thread; s < length[1] * ROWS * groups; s += threads) {
+    const int owner = lists[1][s / (ROWS * groups)], at = s % (ROWS * groups), group = at / ROWS, row = at % ROWS;
+    const TreeCut cut = cuts[owner];
+    if (row < cut.rows)
+      store_joined<T, SLIM>(a, cut, row, group,
+                            join_parts<ROWS, VEC, SLIM, 8>(a, owner, 0, parts_of[owner], row, group));
   }
   constexpr int LANE_ROWS = ROWS < 32 ? ROWS : 32, LANE_GROUPS = 32 / LANE_ROWS;      // of a warp
-  const int groups = (D + SHARED - 1) / SHARED;
   const int units = (ROWS / LANE_ROWS) * ((groups + LANE_GROUPS - 1) / LANE_GROUPS);
-  for (int u = blockIdx.x; u < many * units; u += gridDim.x) {
-    const int owner = list[TREE_MOST_CTAS - 1 - u / units], parts = parts_of[owner], unit = u % units;
+  for (int u = blockIdx.x; u < length[2] * units; u += gridDim.x) {
+    const int owner = lists[2][u / units], parts = parts_of[owner], unit = u % units;
     const TreeCut cut = cuts[owner];
     const int row = unit % (ROWS / LANE_ROWS) * LANE_ROWS + lane % LANE_ROWS;
     const int group = unit / (ROWS / LANE_ROWS) * LANE_GROUPS + lane / LANE_ROWS;
     const bool mine = row < cut.rows && group < groups;
-    Joined<SHARED> joined;
+    Joined<SLIM> joined;
     if (mine)
-      joined = join_parts<ROWS, VEC, SHARED, 8>(a, owner, parts * warp / JOIN_WARPS, parts * (warp + 1) / JOIN_WARPS,
-                                                row, group);
+      joined = join_parts<ROWS, VEC, SLIM, 8>(a, owner, parts * warp / JOIN_WARPS, parts * (warp + 1) / JOIN_WARPS,
+                                              row, group);
     met[warp][0][lane] = joined.top;
     met[warp][1][lane] = joined.sum;
 #pragma unroll
-    for (int e = 0; e < SHARED; ++e) met[warp][2 + e][lane] = joined.acc[e];
+    for (int e = 0; e < SLIM; ++e) met[warp][2 + e][lane] = joined.acc[e];
     __syncthreads();
     if (warp == 0 && mine) {
-      Joined<SHARED> total;
+      Joined<SLIM> total;
 #pragma unroll
       for (int w = 0; w < JOIN_WARPS; ++w) {
-        float o[SHARED];
+        float o[SLIM];
 #pragma unroll
-        for (int e = 0; e < SHARED; ++e) o[e] = met[w][2 + e][lane];
+        for (int e = 0; e < SLIM; ++e) o[e] = met[w][2 + e][lane];
         total.add(met[w][0][lane], met[w][1][lane], o);
       }
-      store_joined<T, SHARED>(a, cut, row, group, total);
+      store_joined<T, SLIM>(a, cut, row, group, total);
     }
     __syncthreads();
   }

@@ -38,10 +38,14 @@ struct StreamConfig {
   static constexpr int kRows = 16 * WARPS;
   static constexpr int kHalfBytes = KEYS * D * 2;      // keys (or values) of a chunk
   static constexpr int kSlotBytes = 2 * kHalfBytes;
-  static constexpr int kRing = (WARPS == 1 ? 2 : 3) * (D <= 64 ? 2 : 1);
+#ifndef HX_RING2
+#define HX_RING2 3
+#define HX_MOST2 4
+#endif
+  static constexpr int kRing = (WARPS == 1 ? 2 : HX_RING2) * (D <= 64 ? 2 : 1);
   static constexpr int kSmemBytes = kRing * kSlotBytes;
   static constexpr int kFit = 227 * 1024 / (kSmemBytes + 2048);      // CTAs an SM has shared memory for
-  static constexpr int kMost = WARPS == 1 ? 6 : 4;                   // ... and registers
+  static constexpr int kMost = WARPS == 1 ? 6 : HX_MOST2;                   // ... and registers
   static constexpr int kCtas = kFit < kMost ? kFit : kMost;
 };
 
@@ -114,6 +118,11 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
   using Config = StreamConfig<D, WARPS>;
   constexpr int RING = Config::kRing, ROWS = Config::kRows;
   constexpr int D_STEPS = D / 16, D_TILES = D / 8;
+#ifdef HX_ONE_TERM
+  constexpr bool TWO_TERMS = false;
+#else
+  constexpr bool TWO_TERMS = WARPS == 1;
+#endif
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t full[RING], empty[RING];
   // the run is found from the step's description, which was there before the kernel in front
@@ -193,13 +202,12 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
     }
   };
 
+  if (warp == 0) enter_item();      // (tables are part of the description, too)
   hx_pdl_wait();
   if (threadIdx.x == 0) tree_tell_none<ROWS>(a);
   __syncthreads();
-  if (warp == 0) {
-    enter_item();
+  if (warp == 0)
     while (asked < RING && asked < run.count) ask();
-  }
 
   // where this lane's ldmatrix rows sit in a slot: keys as matrices (keys 0-7, d lo), (keys 0-7, d
   // hi), (keys 8-15, d lo), (keys 8-15, d hi) of 16 keys, values (transposed) as (keys 0-7, d lo),
@@ -331,10 +339,18 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
           const float p1 = fast_exp2(fmaf(s[j][1], scale_log2, -against_low));
           const float p2 = fast_exp2(fmaf(s[j][2], scale_log2, -against_high));
           const float p3 = fast_exp2(fmaf(s[j][3], scale_log2, -against_high));
-          sum_low += p0 + p1;
-          sum_high += p2 + p3;
-          hx_split_bf16(p0, p1, p_hi[j >> 1][2 * (j & 1)], p_lo[j >> 1][2 * (j & 1)]);
-          hx_split_bf16(p2, p3, p_hi[j >> 1][2 * (j & 1) + 1], p_lo[j >> 1][2 * (j & 1) + 1]);
+          if constexpr (TWO_TERMS) {
+            sum_low += p0 + p1;
+            sum_high += p2 + p3;
+            hx_split_bf16(p0, p1, p_hi[j >> 1][2 * (j & 1)], p_lo[j >> 1][2 * (j & 1)]);
+            hx_split_bf16(p2, p3, p_hi[j >> 1][2 * (j & 1) + 1], p_lo[j >> 1][2 * (j & 1) + 1]);
+          } else {
+            const uint32_t low = hx_pack_bf16(p0, p1), high = hx_pack_bf16(p2, p3);
+            sum_low += __uint_as_float(low << 16) + __uint_as_float(low & 0xffff0000u);
+            sum_high += __uint_as_float(high << 16) + __uint_as_float(high & 0xffff0000u);
+            p_hi[j >> 1][2 * (j & 1)] = low;
+            p_hi[j >> 1][2 * (j & 1) + 1] = high;
+          }
         }
         // ---- the weighted values: d tiles 2 m and 2 m + 1
         if (!drafted) {
@@ -346,8 +362,10 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
               hx_ldmatrix_x4_trans(b, v_half + v_offset[h] + m * piece_step);
               hx_mma_bf16(o[2 * m], p_hi[h], b[0], b[1]);
               hx_mma_bf16(o[2 * m + 1], p_hi[h], b[2], b[3]);
-              hx_mma_bf16(o[2 * m], p_lo[h], b[0], b[1]);
-              hx_mma_bf16(o[2 * m + 1], p_lo[h], b[2], b[3]);
+              if (TWO_TERMS) {
+                hx_mma_bf16(o[2 * m], p_lo[h], b[0], b[1]);
+                hx_mma_bf16(o[2 * m + 1], p_lo[h], b[2], b[3]);
+              }
             }
         } else {
           bool found = false;
@@ -363,8 +381,10 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
                 b[e] = finite_part(b[e], 16 * h + 8 * (e & 1) + 2 * quad, first_drafted, there, found);
               hx_mma_bf16(o[2 * m], p_hi[h], b[0], b[1]);
               hx_mma_bf16(o[2 * m + 1], p_hi[h], b[2], b[3]);
-              hx_mma_bf16(o[2 * m], p_lo[h], b[0], b[1]);
-              hx_mma_bf16(o[2 * m + 1], p_lo[h], b[2], b[3]);
+              if (TWO_TERMS) {
+                hx_mma_bf16(o[2 * m], p_lo[h], b[0], b[1]);
+                hx_mma_bf16(o[2 * m + 1], p_lo[h], b[2], b[3]);
+              }
             }
           poisoned |= __any_sync(0xffffffffu, found) != 0;
         }

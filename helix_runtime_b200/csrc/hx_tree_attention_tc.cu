@@ -7,9 +7,14 @@
 //   warp 1      one lane issues S = Q K^T into one of two score buffers in tensor memory;
 //   warp 2      one lane issues O += P V;
 //   warp 3      loads the queries of an item, as soon as the item before has read its own;
-//   warps 4-7   softmax: thread r owns row r.  P goes back over the scores as two bfloat16 terms
-//               (P = hi + lo, 16 bits of each probability, so that the softmax stays a float32
-//               quantity as far as the result can tell); the reference of the exponentials is
+//   warps 4-11  softmax: two threads own a row, one the first 32 scores of a tile, the other the last 32 (with one
+//               thread a row the softmax took 2,000 cycles a tile, a chain of instructions that no
+//               product or copy was long enough to hide: 64 requests x 64 drafts 405 us).  They tell each other their
+//               maxima, so both keep the same reference.  P goes back
+//               over the scores they have read, in bfloat16: each weight is rounded to 8 bits once, as the
+//               output is (a second term, which streaming for few rows has for nothing, would fill the
+//               columns the maxima are told through, and take a third of the products' time).  P is the A
+//               operand of O += P V straight from tensor memory; the reference of the exponentials is
 //               raised when a tile exceeds it by more than 2^8, O stays in tensor memory.
 // Keys and values keep flowing across items: the rings go by TURNS, the key tiles of the CTA's run in
 // order.  Two CTAs share an SM and fill each other's gaps.
@@ -38,8 +43,8 @@
 namespace {
 
 constexpr int BLOCK_M = 128, BLOCK_N = 64;
-constexpr int WARP_PAGES = 0, WARP_SCORES = 1, WARP_OUTPUT = 2, WARP_QUERIES = 3;      // and 4 to 7: softmax
-constexpr int THREADS = 256;
+constexpr int WARP_PAGES = 0, WARP_SCORES = 1, WARP_OUTPUT = 2, WARP_QUERIES = 3;      // and 4 to 11: softmax
+constexpr int THREADS = 384;
 constexpr int GROUP_STRIDE = 128;             // bytes from one 8-row core matrix to the next row group
 constexpr int CHUNK_STRIDE = BLOCK_M * 16;    // bytes from one 16-byte column of Q to the next
 constexpr float RAISE_MAXIMUM_BY = 8.0f;      // log2 units a tile must exceed a row's reference by
@@ -53,7 +58,6 @@ struct TreeTcConfig {
   static constexpr int kHalfBytes = BLOCK_N * D * 2;          // keys (or values) of a tile
   static constexpr int kBarrierBytes = 256;
   static constexpr int kSmemBytes = kQBytes + (kKeyStages + kValueStages) * kHalfBytes + 128 + kBarrierBytes;
-  static constexpr int kLowTermColumn = BLOCK_N / 2;          // P: hi in columns [0, 32), lo after
   static constexpr int kOutputColumn = 2 * BLOCK_N;
   static constexpr int kTmemColumns = 256;
   static_assert(2 * BLOCK_N + D <= kTmemColumns, "tensor memory of a CTA");
@@ -101,13 +105,23 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
       ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
+// A number of this thread's lane to and from a column of tensor memory.
+__device__ __forceinline__ void tmem_store1(uint32_t address, float value) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(address), "r"(__float_as_uint(value)) : "memory");
+}
+__device__ __forceinline__ float tmem_load1(uint32_t address) {
+  uint32_t value;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(value) : "r"(address) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  return __uint_as_float(value);
+}
 // A bfloat16 whose exponent is all ones: an infinity or not a number.
 __device__ __forceinline__ bool not_finite(uint32_t bits16) { return (bits16 & 0x7f80u) == 0x7f80u; }
 
 // What is not finite among the drafted values that a row sees in the segment [c.tile, c.tile + count) is
 // added to the row as stored: whatever their weight, the sum is not finite either.
 template <int D>
-__device__ __noinline__ void add_not_finite(const TreeArgs& a, TreeCursor c, int count, int token, int row,
+__device__ __noinline__ void add_not_finite(const TreeArgs& a, TreeCursor c, int count, int token, int row, int half,
                                             __nv_bfloat16* out, float* part) {
   const int first = max(c.context, c.tile * BLOCK_N);
   const int end = min(c.context + c.nodes, (c.tile + count) * BLOCK_N);
@@ -119,6 +133,7 @@ __device__ __noinline__ void add_not_finite(const TreeArgs& a, TreeCursor c, int
     const int page = a.block_tables[static_cast<size_t>(a.request_table_row[c.request]) * a.table_stride + index];
     if (page < 0 || page >= a.num_pages) continue;
     for (int d = 0; d < D; ++d) {
+      if ((d / 16) % 2 != half) continue;      // (another thread's)
       const float x = __bfloat162float(v[hx_cache_offset(page, c.kv_head(a), key % a.page_size, d, a.kv_heads,
                                                          a.page_size, D, 8)]);
       if (isfinite(x)) continue;
@@ -161,10 +176,11 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   uint64_t* o_full = p_full + 2;               // [2] its output product is done
   uint64_t* q_ready = o_full + 2;              // the queries of a segment are in shared memory
   uint64_t* q_done = q_ready + 1;              // the last score product of a segment has read them
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(q_done + 1);
+  uint64_t* met = q_done + 1;                  // [4] both softmax warps of 32 rows have told
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(met + 4);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_holder + 1);
   volatile int* poisoned = failed + 1;         // the last segment with a drafted value that is not finite
-  static_assert((2 * K_STAGES + 2 * V_STAGES + 8) * 8 + 12 <= Config::kBarrierBytes, "the place of barriers and flags");
+  static_assert((2 * K_STAGES + 2 * V_STAGES + 12) * 8 + 12 <= Config::kBarrierBytes, "the place of barriers and flags");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -184,11 +200,12 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&p_full[b], 4);   // one arrival per softmax warp
+      mbar_init(&p_full[b], 8);   // one arrival per softmax warp
       mbar_init(&o_full[b], 1);
     }
     mbar_init(q_ready, 1);
     mbar_init(q_done, 1);
+    for (int quarter = 0; quarter < 4; ++quarter) mbar_init(&met[quarter], 2);
     *failed = 0;
     *poisoned = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -411,12 +428,12 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
           }
           tc_fence_after();
           const uint64_t desc_v = desc_v0 + stage * (Config::kHalfBytes >> 4);
-          const uint32_t p_hi = tmem_base + b * BLOCK_N, p_lo = p_hi + Config::kLowTermColumn;
+          // (16 columns of P from either half's first column on)
+          const uint32_t probabilities = tmem_base + b * BLOCK_N;
 #pragma unroll
-          for (int g = 0; g < BLOCK_N / 16; ++g) {
-            umma_bf16_a_tmem(target, p_hi + g * 8, desc_v + value_step[g], idesc, (t > 0 || g > 0) ? 1u : 0u);
-            umma_bf16_a_tmem(target, p_lo + g * 8, desc_v + value_step[g], idesc, 1u);
-          }
+          for (int g = 0; g < BLOCK_N / 16; ++g)
+            umma_bf16_a_tmem(target, probabilities + (g >> 1) * (BLOCK_N / 2) + (g & 1) * 8, desc_v + value_step[g],
+                             idesc, (t > 0 || g > 0) ? 1u : 0u);
           umma_commit(&v_done[stage]);
           umma_commit(&o_full[b]);
         }
@@ -426,12 +443,29 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
     }
   } else {
     // ------------------------------------------------------------------ softmax
+    constexpr int HALF = BLOCK_N / 2;
     const int quarter = warp & 3;      // tensor-memory lanes [32 * quarter, 32 * quarter + 32)
+    const int half = (warp - 4) >> 2;  // which 32 columns of a tile, and which half of O's
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t output_base = lane_base + Config::kOutputColumn;
     const float scale_log2 = a.scale * HX_LOG2E;      // positive: it does not change which score is largest
-    const uint64_t factor_pair = pair_of(scale_log2, scale_log2), minus_one = pair_of(-1.0f, -1.0f);
+    const uint64_t factor_pair = pair_of(scale_log2, scale_log2);
+    uint32_t meetings = 0;
+    // This thread's number for the one that the other thread of the row tells, through a column of the score
+    // buffer that neither scores still wanted nor probabilities take.  (The buffer's next scores wait for the
+    // probabilities of both threads, so nothing is overwritten that has not been read.)
+    auto exchange = [&](uint32_t columns, float mine, float& other) {
+      tmem_store1(columns + half * HALF, mine);
+      tmem_store_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&met[quarter]);
+      const bool there = wait_for(&met[quarter], meetings++);
+      tc_fence_after();
+      if (there) other = tmem_load1(columns + (half ^ 1) * HALF);
+      return there;
+    };
     TreeCursor c = at;
     int turn = 0, segment = 0;
     bool ok = true;
@@ -444,7 +478,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       const bool live = quarter * 32 < rows_here;                         // the warp has rows
       const int last_key = c.context + c.nodes - 1;
       float row_max = -INFINITY;      // the reference of this row's exponentials, in log2 units
-      float row_sum = 0.0f;
+      float row_sum = 0.0f;           // of this thread's columns, from the last tile on of both
       for (int t = 0; t < count && ok; ++t, ++turn) {
         const int b = turn & 1;
         ok = wait_for(&s_full[b], static_cast<uint32_t>(turn / 2));
@@ -454,39 +488,39 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
         if (live) {
           tc_fence_after();
           const uint32_t score_base = lane_base + b * BLOCK_N;
-          float p[BLOCK_N];
+          float p[HALF];
           {
-            uint32_t r[4][16];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_load16_issue(score_base + i * 16, r[i]);
+            uint32_t r[2][16];
+            tmem_load16_issue(score_base + half * HALF, r[0]);
+            tmem_load16_issue(score_base + half * HALF + 16, r[1]);
             tmem_load_wait();
 #pragma unroll
-            for (int i = 0; i < BLOCK_N; ++i) p[i] = __uint_as_float(r[i / 16][i % 16]);
+            for (int i = 0; i < HALF; ++i) p[i] = __uint_as_float(r[i / 16][i % 16]);
           }
           if (drafted) {
             const unsigned long long mask = tree_mask(a, c, my_token, key0);
-            uint32_t low = static_cast<uint32_t>(mask), high = static_cast<uint32_t>(mask >> 32);
-            if (page_size == 16) {      // the order of the columns
-              const uint32_t even = __byte_perm(low, high, 0x6420);
-              high = __byte_perm(low, high, 0x7531);
-              low = even;
-            }
+            uint32_t seen = static_cast<uint32_t>(mask >> (HALF * half));
+            if (page_size == 16)      // the order of the columns
+              seen = __byte_perm(static_cast<uint32_t>(mask), static_cast<uint32_t>(mask >> 32),
+                                 half == 0 ? 0x6420 : 0x7531);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (!((low >> i) & 1)) p[i] = -INFINITY;
-              if (!((high >> i) & 1)) p[i + 32] = -INFINITY;
-            }
+            for (int i = 0; i < HALF; ++i)
+              if (!((seen >> i) & 1)) p[i] = -INFINITY;
           }
           float part_max[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) part_max[u] = max_of_3(p[u], p[u + 4], p[u + 8]);
 #pragma unroll
-          for (int i = 12; i + 8 <= BLOCK_N; i += 8)
+          for (int i = 12; i + 8 <= HALF; i += 8)
 #pragma unroll
             for (int u = 0; u < 4; ++u) part_max[u] = max_of_3(part_max[u], p[i + u], p[i + 4 + u]);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) part_max[u] = fmaxf(part_max[u], p[BLOCK_N - 4 + u]);
-          const float tile_max = scale_log2 * fmaxf(max_of_3(part_max[0], part_max[1], part_max[2]), part_max[3]);
+          for (int u = 0; u < 4; ++u) part_max[u] = fmaxf(part_max[u], p[HALF - 4 + u]);
+          const float own_max = scale_log2 * fmaxf(max_of_3(part_max[0], part_max[1], part_max[2]), part_max[3]);
+          float other_max = 0.0f;
+          ok = exchange(score_base + HALF / 2, own_max, other_max);
+          if (!ok) break;
+          const float tile_max = fmaxf(own_max, other_max);
           // a row that has seen nothing yet keeps -inf as its reference and zeros as its probabilities
           const float old_max = row_max;
           // (each row by itself, so that what another row sees does not reach this one, not even by rounding)
@@ -501,87 +535,73 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int d0 = 0; d0 < D; d0 += 32) {
-              const bool both = d0 + 16 < D;
-              uint32_t r0[16], r1[16];
-              tmem_load16_issue(output_base + d0, r0);
-              if (both) tmem_load16_issue(output_base + d0 + 16, r1);
+            for (int d0 = 0; d0 < D; d0 += 16) {
+              if ((d0 / 16) % 2 != half) continue;
+              uint32_t r[16];
+              tmem_load16_issue(output_base + d0, r);
               tmem_load_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                r0[i] = __float_as_uint(__uint_as_float(r0[i]) * correction);
-                if (both) r1[i] = __float_as_uint(__uint_as_float(r1[i]) * correction);
-              }
-              tmem_store16_raw(output_base + d0, r0);
-              if (both) tmem_store16_raw(output_base + d0 + 16, r1);
+              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * correction);
+              tmem_store16_raw(output_base + d0, r);
             }
           }
-          uint64_t part_sum[4] = {0, 0, 0, 0};
+          // P in bfloat16, two keys per column, the earlier key in the lower half; the sum is over the
+          // probabilities as rounded, so that the weights of a row add up to one
+          uint64_t part_sum[2] = {0, 0};
           const float reference = row_max == -INFINITY ? 0.0f : row_max;
           const uint64_t reference_pair = pair_of(-reference, -reference);
+          uint32_t packed[16];
 #pragma unroll
-          for (int i = 0; i < BLOCK_N; i += 2) {
+          for (int i = 0; i < 16; ++i) {
             float x0, x1;
-            halves_of(pair_fma(pair_of(p[i], p[i + 1]), factor_pair, reference_pair), x0, x1);
-            p[i] = fast_exp2(x0);
-            p[i + 1] = fast_exp2(x1);
-            part_sum[(i / 2) % 4] = pair_add(part_sum[(i / 2) % 4], pair_of(p[i], p[i + 1]));
+            halves_of(pair_fma(pair_of(p[2 * i], p[2 * i + 1]), factor_pair, reference_pair), x0, x1);
+            packed[i] = pack_bf16(fast_exp2(x0), fast_exp2(x1));
+            part_sum[i % 2] = pair_add(part_sum[i % 2], pair_of(__uint_as_float(packed[i] << 16),
+                                                                __uint_as_float(packed[i] & 0xffff0000u)));
           }
           {
             float low, high;
-            halves_of(pair_add(pair_add(part_sum[0], part_sum[1]), pair_add(part_sum[2], part_sum[3])), low, high);
+            halves_of(pair_add(part_sum[0], part_sum[1]), low, high);
             row_sum += low + high;
           }
-          // P = hi + lo over the scores just read, two keys per column, the earlier key in the lower half
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float p0 = p[half * 32 + 2 * i], p1 = p[half * 32 + 2 * i + 1];
-              hi[i] = pack_bf16(p0, p1);
-              float rest0, rest1;
-              halves_of(pair_fma(pair_of(__uint_as_float(hi[i] << 16), __uint_as_float(hi[i] & 0xffff0000u)),
-                                 minus_one, pair_of(p0, p1)), rest0, rest1);
-              lo[i] = pack_bf16(rest0, rest1);
-            }
-            tmem_store16_raw(score_base + half * 16, hi);
-            tmem_store16_raw(score_base + Config::kLowTermColumn + half * 16, lo);
+          tmem_store16_raw(score_base + half * HALF, packed);
+          if (t == count - 1) {
+            float other_sum = 0.0f;
+            ok = exchange(score_base + HALF / 2 + 1, row_sum, other_sum);
+            if (!ok) break;
+            row_sum = half == 0 ? row_sum + other_sum : other_sum + row_sum;
           }
           tmem_store_wait();
         }
         if (drafted) {
-          // values behind the last key (whatever an earlier tile left there) and drafted values that
-          // are not finite become zeros
+          // values behind the last key (whatever the page or an earlier tile left there) and drafted values
+          // that are not finite become zeros
           ok = wait_for(&v_full[turn % V_STAGES], static_cast<uint32_t>(turn / V_STAGES));
           if (!ok) break;
           uint8_t* v_half = v_stages + (turn % V_STAGES) * Config::kHalfBytes;
-          const int first_stale = last_key + 1 - key0, first_drafted = max(c.context - key0, 0);
-          bool found = false;
-          for (int i = row; i < BLOCK_N * PIECES; i += 128) {
+          const int there = last_key + 1 - key0, first_drafted = max(c.context - key0, 0);
+          bool wrote = false, found = false;
+          for (int i = half * 128 + row; i < BLOCK_N * PIECES; i += 256) {
             const int piece = i / BLOCK_N, key = i - piece * BLOCK_N;
             if (key < first_drafted) continue;
             uint4* place = reinterpret_cast<uint4*>(v_half + (key / page_size) * page_bytes +
                                                     (piece * page_size + key % page_size) * 16);
-            if (key >= first_stale) {
-              *place = make_uint4(0u, 0u, 0u, 0u);
-              continue;
-            }
             uint4 value = *place;
-            uint32_t* halves = reinterpret_cast<uint32_t*>(&value);
+            uint32_t* pairs = reinterpret_cast<uint32_t*>(&value);
             bool bad = false;
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-              if (not_finite(halves[h])) { halves[h] &= 0xffff0000u; bad = true; }
-              if (not_finite(halves[h] >> 16)) { halves[h] &= 0x0000ffffu; bad = true; }
+              if (not_finite(pairs[h])) { pairs[h] &= 0xffff0000u; bad = true; }
+              if (not_finite(pairs[h] >> 16)) { pairs[h] &= 0x0000ffffu; bad = true; }
             }
             if (bad) {
               *place = value;
-              found = true;
+              wrote = true;
+              found |= key < there;
             }
           }
           if (found) *poisoned = segment;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          if (__any_sync(0xffffffffu, wrote)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         tc_fence_before();
         __syncwarp();
@@ -589,7 +609,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       }
       if (!ok) break;
 
-      // ---- the segment's rows: finished, or this CTA's part of them
+      // ---- the segment's rows: finished, or this CTA's part of them; a thread has half of the coordinates
       ok = wait_for(&o_full[(turn - 1) & 1], static_cast<uint32_t>((turn - 1) / 2));
       if (!ok) break;
       if (live) {
@@ -601,6 +621,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
         float* part = tree_part<BLOCK_M>(a, blockIdx.x, c.tile == 0);
 #pragma unroll
         for (int d0 = 0; d0 < D; d0 += 16) {
+          if ((d0 / 16) % 2 != half) continue;
           float o[16];
           __syncwarp();
           tmem_load16(output_base + d0, o);
@@ -627,18 +648,18 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
             }
           }
         }
-        if (!whole && row < rows_here) {
+        if (!whole && half == 0 && row < rows_here) {
           part[static_cast<size_t>(D) * BLOCK_M + row] = row_max;
           part[static_cast<size_t>(D + 1) * BLOCK_M + row] = row_sum;
         }
         // (told before the arrivals that the last output product waited for)
         if (*poisoned == segment && row < rows_here)
-          add_not_finite<D>(a, c, count, my_token, row, whole ? out : nullptr, whole ? nullptr : part);
+          add_not_finite<D>(a, c, count, my_token, row, half, whole ? out : nullptr, whole ? nullptr : part);
         tc_fence_before();
       }
       left -= count;
       if (left > 0) tree_next_item<BLOCK_N>(a, c);
-      else if (row == 0) tree_tell_cut<BLOCK_M>(a, run, c, count);
+      else if (threadIdx.x == 128) tree_tell_cut<BLOCK_M>(a, run, c, count);
     }
   }
 

@@ -150,13 +150,17 @@ class Batch:
         float32, off by at most (head_dim + 3) u times their magnitudes (the scale, the base-2
         factor and the difference to the maximum are one rounding each), and an exponent's
         error is a weight's relative error, in numerator and denominator: twice that.  Exponential
-        2^-21, sums of n terms n u each, joined parts a few more: (2 n + 64) u.  The tensor cores' weights
-        are two bfloat16 terms, 2^-16.  Last the output's own rounding."""
+        2^-21, sums of n terms n u each, joined parts a few more: (2 n + 64) u.  In bfloat16 a weight is
+        rounded once, by at most d = 2^-8 of itself, and divided by the sum of the rounded ones: sum w (1 + d_j)
+        v / sum w (1 + d_j) is off by at most d (sum w |v| + |output|) / (1 - d).  Last the output's own
+        rounding, again 2^-8 of it."""
         u = 2.0 ** -24
         keys = max(c + n for c, n in zip(self.contexts, self.nodes))
         share = 2 * (self.head_dim + 3) * u * largest + (2 * keys + 64) * u
         if self.dtype == torch.bfloat16:
-            return 2.0 ** -8 * expected.abs() + (share + 2.0 ** -16) * weighed * 1.01
+            d = 2.0 ** -8
+            near = d / (1 - d) * (weighed + expected.abs()) + share * weighed
+            return near + d * (expected.abs() + near)
         return u * expected.abs() + share * weighed
 
     def check(self, out=None):
