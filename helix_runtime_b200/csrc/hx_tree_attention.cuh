@@ -146,6 +146,25 @@ __device__ __forceinline__ void tree_next_item(const TreeArgs& a, TreeCursor& c)
   } while (c.tiles == 0);
 }
 
+// Bounded wait: false when the limit ran out (some seconds).  A poll may sleep for 16 us: without that
+// time the waiting warps of a tcgen05 CTA issued ten times the instructions of those that work, and
+// held them up.
+__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t address = static_cast<uint32_t>(__cvta_generic_to_shared(bar));
+  for (uint32_t poll = 0; poll < 400u * 1000u; ++poll) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(address), "r"(parity), "r"(16u * 1024u)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
 // A CTA's run of the list.  Runs are at least `least` tiles long, so that a short list does not
 // become more parts than it is worth.
 struct TreeRun {
@@ -171,26 +190,35 @@ __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int cta, int ctas
   return run;
 }
 
-// Which of the 64 keys from key0 on does drafted token `token` of the cursor's request see?  Bit i
-// is key key0 + i: a cached key, or a drafted one whose bit is set.
-__device__ __forceinline__ unsigned long long tree_mask(const TreeArgs& a, const TreeCursor& c, int token,
-                                                        int key0) {
+// Which of the 64 keys from key0 on does a drafted token of the cursor's request see?  Bit i is key
+// key0 + i: a cached key, or a drafted one whose bit is set.  `first_word`: the first of the token's
+// words; `word_at` gives the others.
+template <typename Words>
+__device__ __forceinline__ unsigned long long tree_mask_of(const TreeArgs& a, const TreeCursor& c, int key0,
+                                                           unsigned long long first_word, Words word_at) {
   const int cached = c.context - key0;      // of the tile's keys, so many are cached ones
   if (cached >= 64) return ~0ull;
-  const unsigned long long* words = reinterpret_cast<const unsigned long long*>(a.visible) +
-                                    static_cast<size_t>(c.q_begin + token) * a.ld_visible;
   unsigned long long mask;
   if (cached >= 0) {
-    mask = words[0] << cached;
+    mask = first_word << cached;
     if (cached > 0) mask |= (1ull << cached) - 1;
   } else {
     const int first = -cached, word = first >> 6, shift = first & 63;
-    mask = word < a.words ? words[word] >> shift : 0ull;
-    if (shift > 0 && word + 1 < a.words) mask |= words[word + 1] << (64 - shift);
+    mask = word == 0 ? first_word >> shift : word < a.words ? word_at(word) >> shift : 0ull;
+    // (words behind the last token's say nothing)
+    if (shift > 0 && word + 1 < a.words && 64 * (word + 1) < c.nodes) mask |= word_at(word + 1) << (64 - shift);
   }
   const int there = cached + c.nodes;       // keys of the tile that exist
   if (there < 64) mask &= there > 0 ? (1ull << there) - 1 : 0ull;
   return mask;
+}
+__device__ __forceinline__ const unsigned long long* tree_words(const TreeArgs& a, const TreeCursor& c, int token) {
+  return reinterpret_cast<const unsigned long long*>(a.visible) + static_cast<size_t>(c.q_begin + token) * a.ld_visible;
+}
+__device__ __forceinline__ unsigned long long tree_mask(const TreeArgs& a, const TreeCursor& c, int token, int key0) {
+  if (c.context - key0 >= 64) return ~0ull;
+  const unsigned long long* words = tree_words(a, c, token);
+  return tree_mask_of(a, c, key0, words[0], [&](int word) { return words[word]; });
 }
 
 // How the heads of a key/value head and the tokens fill tiles of `rows` rows.

@@ -31,7 +31,6 @@ constexpr int KEYS = 32;
 #endif
 constexpr int LEAST = HX_LEAST;                      // chunks of the shortest run
 constexpr float RAISE_MAXIMUM_BY = 8.0f;      // log2 units a chunk must exceed a row's reference by
-constexpr uint32_t WAIT_LIMIT = 20u * 1000u * 1000u;
 
 template <int D, int WARPS>
 struct StreamConfig {
@@ -53,21 +52,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity) {
-  const uint32_t address = hx_shared_address(bar);
-  for (uint32_t spin = 0; spin < WAIT_LIMIT; ++spin) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(address), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
 }
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
@@ -237,7 +221,11 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
     float o[D_TILES][4];
     float max_low = -INFINITY, max_high = -INFINITY, sum_low = 0.0f, sum_high = 0.0f;
     bool poisoned = false;
+    // the first words of the rows' masks, which are wanted at the item's end
+    unsigned long long first_low = 0, first_high = 0;
     if (live) {
+      first_low = __ldg(tree_words(a, c, token_low));
+      first_high = __ldg(tree_words(a, c, token_high));
       const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + 2 * quad;
       const __nv_bfloat16* q_low = q + static_cast<size_t>(c.q_begin + token_low) * a.ldq + static_cast<size_t>(head_low) * D;
       const __nv_bfloat16* q_high = q + static_cast<size_t>(c.q_begin + token_high) * a.ldq + static_cast<size_t>(head_high) * D;
@@ -256,14 +244,14 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
     for (int t = 0; t < count; ++t, ++i) {
       const int slot = i % RING;
       int arrived = 1;
-      if (lane == 0) arrived = ring_wait(&full[slot], static_cast<uint32_t>(i / RING) & 1u);
+      if (lane == 0) arrived = tree_wait(&full[slot], static_cast<uint32_t>(i / RING) & 1u);
       ok = __shfl_sync(0xffffffffu, arrived, 0) != 0;
       if (!ok) break;
       if constexpr (WARPS > 1) {
         // the slot of the chunk before, which the other warps have had this long to get through with
         if (warp == 0 && i > 0 && asked < run.count) {
           int freed = 1;
-          if (lane == 0) freed = ring_wait(&empty[(i - 1) % RING], static_cast<uint32_t>((i - 1) / RING) & 1u);
+          if (lane == 0) freed = tree_wait(&empty[(i - 1) % RING], static_cast<uint32_t>((i - 1) / RING) & 1u);
           ok = __shfl_sync(0xffffffffu, freed, 0) != 0;
           if (!ok) break;
           ask();
@@ -290,8 +278,12 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
             hx_mma_bf16(s[2 * h + 1], q_frag[k], b[2], b[3]);
           }
         if (drafted) {
-          const uint32_t low = static_cast<uint32_t>(tree_mask(a, c, token_low, key0)) >> (2 * quad);
-          const uint32_t high = static_cast<uint32_t>(tree_mask(a, c, token_high, key0)) >> (2 * quad);
+          const unsigned long long* words_low = tree_words(a, c, token_low);
+          const unsigned long long* words_high = tree_words(a, c, token_high);
+          const uint32_t low = static_cast<uint32_t>(tree_mask_of(
+                                   a, c, key0, first_low, [&](int word) { return words_low[word]; })) >> (2 * quad);
+          const uint32_t high = static_cast<uint32_t>(tree_mask_of(
+                                    a, c, key0, first_high, [&](int word) { return words_high[word]; })) >> (2 * quad);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (!(low >> (8 * j) & 1)) s[j][0] = -INFINITY;
@@ -459,7 +451,7 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
     if (lane == 0) atomicOr(a.status, HX_FLAG_WAIT_TIMEOUT);
     // a CTA does not leave while copies into its shared memory are in flight
     if (threadIdx.x == 0)
-      for (int n = max(0, asked - RING); n < asked; ++n) ring_wait(&full[n % RING], static_cast<uint32_t>(n / RING) & 1u);
+      for (int n = max(0, asked - RING); n < asked; ++n) tree_wait(&full[n % RING], static_cast<uint32_t>(n / RING) & 1u);
     __syncwarp();
   }
 }

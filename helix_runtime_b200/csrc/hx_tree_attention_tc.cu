@@ -29,8 +29,9 @@
 // piece into one stride instead took a copy of 256 bytes 80 cycles of the warp that asks, 6,500 cycles a tile.)
 //
 // Masks matter in the tiles that hold drafted keys, the last one or two of an item.  There values
-// are looked at, too: a drafted value that is not finite would reach rows that do not see it (0 x
-// infinity), so it is taken as zero in the product and added, as what it is, to the rows that do see it.
+// are looked at, too: a probability of zero does not stop one that is not finite (0 x infinity), be it a
+// drafted one that other rows see or what a page holds behind the last key.  Such a value is taken as zero
+// in the product; a drafted one is added, as what it is, to the rows that do see it.
 //
 // Every wait is bounded; a wait that runs out sets a status bit, the CTA lets its copies land, frees its
 // tensor memory and returns.
@@ -115,8 +116,8 @@ __device__ __forceinline__ float tmem_load1(uint32_t address) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
   return __uint_as_float(value);
 }
-// A bfloat16 whose exponent is all ones: an infinity or not a number.
-__device__ __forceinline__ bool not_finite(uint32_t bits16) { return (bits16 & 0x7f80u) == 0x7f80u; }
+// All ones in those of two bfloat16 that are infinite or not a number (all ones in the exponent).
+__device__ __forceinline__ uint32_t exponents_of(uint32_t pair) { return __vcmpeq2(pair & 0x7f807f80u, 0x7f807f80u); }
 
 // What is not finite among the drafted values that a row sees in the segment [c.tile, c.tile + count) is
 // added to the row as stored: whatever their weight, the sum is not finite either.
@@ -186,6 +187,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   const int lane = threadIdx.x & 31;
   const int page_size = a.page_size;
   const int pages_per_tile = BLOCK_N / page_size;
+  const int page_shift = __ffs(page_size) - 1;      // (pages of 8, 16, 32 or 64)
   const uint32_t page_bytes = static_cast<uint32_t>(page_size) * D * 2;
   const uint32_t piece_stride = static_cast<uint32_t>(page_size) * 16;   // next 16-byte piece of a key
 
@@ -222,7 +224,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   // One lane waits and looks at the failure flag, all lanes get the same answer.
   auto wait_for = [&](uint64_t* bar, uint32_t parity) {
     int state = 0;      // 0: go on, 1: this wait ran out, 2: somebody else failed
-    if (lane == 0) state = *failed ? 2 : (mbar_wait(bar, parity & 1u) ? 0 : 1);
+    if (lane == 0) state = *failed ? 2 : (tree_wait(bar, parity & 1u) ? 0 : 1);
     state = __shfl_sync(0xffffffffu, state, 0);
     if (state == 1 && lane == 0) {
       atomicOr(a.status, HX_FLAG_WAIT_TIMEOUT);
@@ -315,9 +317,9 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
     // a CTA does not leave while copies into its shared memory are in flight
     if (*failed) {
       for (int t = max(0, keys_asked - K_STAGES); t < keys_asked; ++t)
-        if (lane == 0) mbar_wait(&k_full[t % K_STAGES], static_cast<uint32_t>(t / K_STAGES) & 1u);
+        if (lane == 0) tree_wait(&k_full[t % K_STAGES], static_cast<uint32_t>(t / K_STAGES) & 1u);
       for (int t = max(0, asked - V_STAGES); t < asked; ++t)
-        if (lane == 0) mbar_wait(&v_full[t % V_STAGES], static_cast<uint32_t>(t / V_STAGES) & 1u);
+        if (lane == 0) tree_wait(&v_full[t % V_STAGES], static_cast<uint32_t>(t / V_STAGES) & 1u);
       __syncwarp();
     }
   } else if (warp == WARP_QUERIES) {
@@ -336,15 +338,19 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
                                static_cast<size_t>(c.q_begin + rows.token0) * a.ldq + static_cast<size_t>(rows.head0) * D;
       // (asynchronous copies: all of a lane's are in flight together, without registers.  Eight at a time
-      // through registers took 25,000 cycles for 128 rows)
-      const int items = (rows_here + 7) / 8 * PIECES * 8;
-      for (int i = lane; i < items; i += 32) {
-        const int block = i >> 3, row_group = block / PIECES, piece = block - row_group * PIECES;
-        const int row = row_group * 8 + (i & 7), token = row / rows.heads;
+      // through registers took 25,000 cycles for 128 rows; one division a copy another 500 each)
+#pragma unroll 2
+      for (int row_group = 0; row_group * 8 < rows_here; ++row_group) {
+        const int row = row_group * 8 + (lane & 7), token = row / rows.heads;
         const bool there = row < rows_here;
-        hx_cp_async_16(smem_u32(q_tile + piece * CHUNK_STRIDE + row_group * GROUP_STRIDE + (i & 7) * 16),
-                       there ? q + static_cast<size_t>(token) * a.ldq + static_cast<size_t>(row - token * rows.heads) * D + piece * 8
-                             : q, there ? 16 : 0);
+        const __nv_bfloat16* from =
+            there ? q + static_cast<size_t>(token) * a.ldq + static_cast<size_t>(row - token * rows.heads) * D : q;
+        const uint32_t target = smem_u32(q_tile + row_group * GROUP_STRIDE + (lane & 7) * 16);
+#pragma unroll
+        for (int j = 0; j < (PIECES + 3) / 4; ++j) {
+          const int piece = 4 * j + (lane >> 3);
+          if (piece < PIECES) hx_cp_async_16(target + piece * CHUNK_STRIDE, from + piece * 8, there ? 16 : 0);
+        }
       }
       hx_cp_async_commit();
       hx_cp_async_wait<0>();
@@ -369,12 +375,12 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       int turn = 0, segment = 0;
       for (int left = run.count; left > 0 && !*failed; ++segment) {
         const int count = min(c.tiles - c.tile, left);
-        bool ok = mbar_wait(q_ready, static_cast<uint32_t>(segment) & 1u);
+        bool ok = tree_wait(q_ready, static_cast<uint32_t>(segment) & 1u);
         for (int t = 0; t < count && ok && !*failed; ++t, ++turn) {
           const int b = turn & 1, stage = turn % K_STAGES;
           // (the buffer held the probabilities of two turns ago, which the output product must have read)
-          ok = mbar_wait(&k_full[stage], static_cast<uint32_t>(turn / K_STAGES) & 1u) &&
-               (turn < 2 || mbar_wait(&o_full[b], static_cast<uint32_t>(turn / 2 - 1) & 1u));
+          ok = tree_wait(&k_full[stage], static_cast<uint32_t>(turn / K_STAGES) & 1u) &&
+               (turn < 2 || tree_wait(&o_full[b], static_cast<uint32_t>(turn / 2 - 1) & 1u));
           if (!ok) break;
           tc_fence_after();
           const uint64_t desc_k = desc_k0 + stage * (Config::kHalfBytes >> 4);
@@ -420,8 +426,8 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
         for (int t = 0; t < count && !*failed; ++t, ++turn) {
           const int b = turn & 1, stage = turn % V_STAGES;
           // (the first probabilities of a segment come when the rows of the one before have left)
-          if (!mbar_wait(&p_full[b], static_cast<uint32_t>(turn / 2) & 1u) ||
-              !mbar_wait(&v_full[stage], static_cast<uint32_t>(turn / V_STAGES) & 1u)) {
+          if (!tree_wait(&p_full[b], static_cast<uint32_t>(turn / 2) & 1u) ||
+              !tree_wait(&v_full[stage], static_cast<uint32_t>(turn / V_STAGES) & 1u)) {
             atomicOr(a.status, HX_FLAG_WAIT_TIMEOUT);
             *failed = 1;
             break;
@@ -476,7 +482,9 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       const int my_token = rows.token0 + min(row, rows_here - 1) / rows.heads;      // (rows behind the last: any)
       const int my_head = rows.head0 + row % rows.heads;
       const bool live = quarter * 32 < rows_here;                         // the warp has rows
-      const int last_key = c.context + c.nodes - 1;
+      // the first word of the row's mask, which is wanted at the item's end, is on its way from its beginning on
+      const unsigned long long* words_of_row = tree_words(a, c, my_token);
+      const unsigned long long first_word = live ? __ldg(words_of_row) : 0ull;
       float row_max = -INFINITY;      // the reference of this row's exponentials, in log2 units
       float row_sum = 0.0f;           // of this thread's columns, from the last tile on of both
       for (int t = 0; t < count && ok; ++t, ++turn) {
@@ -498,7 +506,8 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
             for (int i = 0; i < HALF; ++i) p[i] = __uint_as_float(r[i / 16][i % 16]);
           }
           if (drafted) {
-            const unsigned long long mask = tree_mask(a, c, my_token, key0);
+            const unsigned long long mask =
+                tree_mask_of(a, c, key0, first_word, [&](int word) { return words_of_row[word]; });
             uint32_t seen = static_cast<uint32_t>(mask >> (HALF * half));
             if (page_size == 16)      // the order of the columns
               seen = __byte_perm(static_cast<uint32_t>(mask), static_cast<uint32_t>(mask >> 32),
@@ -534,9 +543,8 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
             ok = wait_for(&o_full[(turn - 1) & 1], static_cast<uint32_t>((turn - 1) / 2));
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
-            for (int d0 = 0; d0 < D; d0 += 16) {
-              if ((d0 / 16) % 2 != half) continue;
+#pragma unroll 1      // (rare: the loop that runs every time keeps the instruction cache)
+            for (int d0 = 16 * half; d0 < D; d0 += 32) {
               uint32_t r[16];
               tmem_load16_issue(output_base + d0, r);
               tmem_load_wait();
@@ -574,31 +582,30 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
           tmem_store_wait();
         }
         if (drafted) {
-          // values behind the last key (whatever the page or an earlier tile left there) and drafted values
-          // that are not finite become zeros
           ok = wait_for(&v_full[turn % V_STAGES], static_cast<uint32_t>(turn / V_STAGES));
           if (!ok) break;
-          uint8_t* v_half = v_stages + (turn % V_STAGES) * Config::kHalfBytes;
-          const int there = last_key + 1 - key0, first_drafted = max(c.context - key0, 0);
+          // a thread has a key and every fourth piece of its value
+          const int number = half * 128 + row, key = number & (BLOCK_N - 1);
           bool wrote = false, found = false;
-          for (int i = half * 128 + row; i < BLOCK_N * PIECES; i += 256) {
-            const int piece = i / BLOCK_N, key = i - piece * BLOCK_N;
-            if (key < first_drafted) continue;
-            uint4* place = reinterpret_cast<uint4*>(v_half + (key / page_size) * page_bytes +
-                                                    (piece * page_size + key % page_size) * 16);
-            uint4 value = *place;
-            uint32_t* pairs = reinterpret_cast<uint32_t*>(&value);
-            bool bad = false;
+          if (key >= c.context - key0) {
+            uint8_t* at_key = v_stages + (turn % V_STAGES) * Config::kHalfBytes + (key >> page_shift) * page_bytes +
+                              (key & (page_size - 1)) * 16;
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              if (not_finite(pairs[h])) { pairs[h] &= 0xffff0000u; bad = true; }
-              if (not_finite(pairs[h] >> 16)) { pairs[h] &= 0x0000ffffu; bad = true; }
-            }
-            if (bad) {
+            for (int j = 0; j < (PIECES + 3) / 4; ++j) {
+              const int piece = 4 * j + number / BLOCK_N;
+              if (piece >= PIECES) break;
+              uint4* place = reinterpret_cast<uint4*>(at_key + piece * piece_stride);
+              uint4 value = *place;
+              if ((exponents_of(value.x) | exponents_of(value.y) | exponents_of(value.z) | exponents_of(value.w)) == 0u)
+                continue;
+              value.x &= ~exponents_of(value.x);
+              value.y &= ~exponents_of(value.y);
+              value.z &= ~exponents_of(value.z);
+              value.w &= ~exponents_of(value.w);
               *place = value;
               wrote = true;
-              found |= key < there;
             }
+            found = wrote && key < c.context + c.nodes - key0;
           }
           if (found) *poisoned = segment;
           if (__any_sync(0xffffffffu, wrote)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -619,9 +626,8 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(c.q_begin + my_token) * a.ldo +
                              static_cast<size_t>(my_head) * D;
         float* part = tree_part<BLOCK_M>(a, blockIdx.x, c.tile == 0);
-#pragma unroll
-        for (int d0 = 0; d0 < D; d0 += 16) {
-          if ((d0 / 16) % 2 != half) continue;
+#pragma unroll 1      // (instructions that are met once an item come at 40 cycles for eight)
+        for (int d0 = 16 * half; d0 < D; d0 += 32) {
           float o[16];
           __syncwarp();
           tmem_load16(output_base + d0, o);

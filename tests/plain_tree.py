@@ -111,11 +111,11 @@ class Batch:
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.scale = 1.0 / math.sqrt(head_dim)
 
-    def run(self, ops, partial=None, out=None):
+    def run(self, ops, partial=None, out=None, max_nodes=0):
         ops.tree_attention(self.q, self.k, self.v, self.visible, self.start, self.context, self.row,
                            self.tables, self.out if out is None else out, partial, self.requests,
                            self.heads, self.kv_heads, self.head_dim, self.page_size, self.num_pages,
-                           self.scale, self.status)
+                           self.scale, self.status, max_nodes)
         return self.out if out is None else out
 
     def expected(self):

@@ -37,9 +37,10 @@ DTYPES = [torch.bfloat16, torch.float32]
     ([5000], [64], 8, 2, 128, 32),                             # one request over all CTAs
 ])
 def test_sizes(dtype, contexts, nodes, heads, kv_heads, head_dim, page):
-    batch = Batch(1, contexts, nodes, heads, kv_heads, head_dim, page, dtype, row_pad=8)
-    batch.run(ops)
-    batch.check()
+    for stale in (float("nan"), 0.5):      # what lies in the pages behind the last key
+        batch = Batch(1, contexts, nodes, heads, kv_heads, head_dim, page, dtype, row_pad=8, stale=stale)
+        batch.run(ops)
+        batch.check()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -50,9 +51,12 @@ def test_many_items_a_run(dtype, page):
     contexts = [int(c) for c in rng.integers(0, 900, 20)]
     nodes = [int(n) for n in rng.integers(1, 20, 20)]
     nodes[7] = 0                       # a request without tokens
-    batch = Batch(2, contexts, nodes, 32, 32, 64, page, dtype)
-    batch.run(ops)
-    batch.check()
+    for stale in (float("nan"), 0.5):
+        batch = Batch(2, contexts, nodes, 32, 32, 64, page, dtype, stale=stale)
+        for most in (1, 64):               # of a kernel's choice: the streaming one, or the tensor cores'
+            batch.out.fill_(7.0)
+            batch.run(ops, max_nodes=most)
+            batch.check()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
