@@ -22,11 +22,13 @@
 // "Table-driven implementation of the exponential function", 1989), whose error of a few 1e-16 is what
 // the sums have anyway, in a dozen instructions.
 //
-// Layout.  A request is a cluster of CTAs; every warp owns a stretch of the vocabulary and reads it
-// from global memory (again from L1 when a child falls), and one exchange of the warps' sums
-// through distributed shared memory a visited token, one more a fallen child, is all that the
-// warps tell each other: each then takes the same decisions from the same numbers.  Only rows of tokens
-// that are walked over are read.
+// Layout.  A request is a cluster of CTAs; every warp owns a stretch of the vocabulary, which it
+// reads from global memory once and from L1 again.  A visited token takes
+// one exchange through distributed shared memory, one more a fallen child: a CTA adds up its warps and tells
+// the others, and then each takes the same decisions from the same numbers.  What a chain of visited tokens
+// takes is latency, so the tree lies in shared memory, the logits of all children are asked for
+// together with the row, and the row that comes next if the first child stands is fetched into the L2
+// meanwhile.  Only rows of tokens that are walked over are read.
 #include "hx_common.cuh"
 
 #include <mutex>
@@ -36,6 +38,7 @@ namespace {
 constexpr int WARPS = 16, THREADS = WARPS * 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr int TABLE = 64;
+constexpr int TREE = 256;      // tokens of a tree that shared memory holds (a larger one is read where it lies)
 
 struct VerifyArgs {
   const float* logits;      // [tokens, ld]
@@ -58,7 +61,8 @@ struct VerifyArgs {
   int* status;
 };
 
-// What a warp tells about its stretch: maximum and sum of exponentials against it, of target and draft.
+// What a warp (and then a CTA) says of its stretch: maximum and sum of exponentials against it, of target
+// and draft.
 struct Told {
   double p_sum, q_sum;
   float p_max, q_max;
@@ -110,7 +114,7 @@ struct Exponential {
     p = fma(rest, p, C1);
     p = fma(rest, p, 1.0);
     const double base = table[n & (TABLE - 1)];
-    return __hiloint2double(__double2hiint(base) + ((n >> 6) << 20), __double2loint(base)) * p;
+    return __hiloint2double(__double2hiint(base) + (n >> 6) * (1 << 20), __double2loint(base)) * p;
   }
 };
 
@@ -120,20 +124,57 @@ __device__ __forceinline__ double warp_sum(double value) {
   return value;
 }
 
+__device__ __forceinline__ void take_larger(float& value, int& id, float other, int other_id) {
+  if (other > value || (other == value && other_id < id)) {
+    value = other;
+    id = other_id;
+  }
+}
+
+// Several of these, all of the same warp or CTA order, as one: sums against the common maxima.
+// Every lane brings one (or none: p_max = -inf, sums zero); all get the result.
+__device__ __forceinline__ Told join_told(Told mine, const double* table, double unit) {
+  float p_top = mine.p_max, q_top = mine.q_max;
+  int best = mine.best;
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) {
+    take_larger(p_top, best, __shfl_xor_sync(0xffffffffu, p_top, offset), __shfl_xor_sync(0xffffffffu, best, offset));
+    q_top = fmaxf(q_top, __shfl_xor_sync(0xffffffffu, q_top, offset));
+  }
+  Told all;
+  all.p_max = p_top;
+  all.q_max = q_top;
+  all.best = best;
+  all.bad = __any_sync(0xffffffffu, mine.bad);
+  all.p_sum = warp_sum(mine.p_sum > 0.0 ? mine.p_sum * Exponential{table, unit, p_top}(mine.p_max) : 0.0);
+  all.q_sum = warp_sum(mine.q_sum > 0.0 ? mine.q_sum * Exponential{table, unit, q_top}(mine.q_max) : 0.0);
+  return all;
+}
+
 __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
   __shared__ double table[TABLE];
-  __shared__ Told told[2][MAX_CLUSTER * WARPS];
+  __shared__ Told of_warp[WARPS], of_cta[2][MAX_CLUSTER];
+  __shared__ double sums_of_warp[WARPS];            // of the last exchange, for the draw
+  __shared__ int parent_of[TREE], id_of[TREE];
+  __shared__ float number_of[TREE];
   hx_pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster_rank(), ctas = cluster_size();
   const int request = blockIdx.x / ctas;
-  const int owners = ctas * WARPS, me = rank * WARPS + warp;
+  const int me = rank * WARPS + warp;
   if (threadIdx.x < TABLE) table[threadIdx.x] = exp2(threadIdx.x * (1.0 / TABLE));
   hx_pdl_wait();
-  cluster_sync();      // every CTA's shared memory is there
-
   const int begin = a.request_start[request];
   const int nodes = a.request_start[request + 1] - begin;
+  const bool held_tree = nodes <= TREE;
+  if (held_tree)
+    for (int j = threadIdx.x; j < nodes; j += THREADS) {
+      parent_of[j] = a.parents[begin + j];
+      id_of[j] = a.ids[begin + j];
+      number_of[j] = a.uniform[begin + j];
+    }
+  cluster_sync();      // every CTA's shared memory is there, and the tree in it
+
   int* path = a.path + static_cast<size_t>(request) * a.ld_path;
   const bool writes = rank == 0 && warp == 0;
   if (nodes <= 0) {      // (the same in the whole cluster)
@@ -151,28 +192,53 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
   const double unit = greedy ? 0.0 : TABLE / (0.693147180559945309 * static_cast<double>(heat));
   const int first = min(static_cast<long long>(me) * a.span, static_cast<long long>(a.vocab));
   const int last = min(static_cast<long long>(first) + a.span, static_cast<long long>(a.vocab));
-  int phase = 0;       // which half of `told` the next exchange uses
+  const bool wide = a.ld % 4 == 0 && a.ld_draft % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 &&
+                    (reinterpret_cast<uintptr_t>(a.draft) & 15) == 0;
+  int phase = 0;       // which half of `of_cta` the next exchange uses
 
-  // One exchange: lane r of a warp writes the warp's words to CTA r; behind the barrier they are
-  // everywhere.  (A half is written again two exchanges later: everyone has passed the barrier between.)
-  auto tell = [&](const Told& mine) {
+  // One exchange: the CTA's warps as one, told to every CTA; all warps of the cluster get the
+  // cluster's.  (A half is written again two exchanges later: everyone has passed the barrier between.)
+  auto tell = [&](const Told& mine, bool plain_sums) {
     phase ^= 1;
-    if (lane < ctas) {
-      const uint32_t place = address_in(&told[phase][me], lane);
-      store_in(place, __double_as_longlong(mine.p_sum));
-      store_in(place + 8, __double_as_longlong(mine.q_sum));
-      store_in(place + 16, static_cast<uint64_t>(__float_as_uint(mine.p_max)) |
-                               static_cast<uint64_t>(__float_as_uint(mine.q_max)) << 32);
-      store_in(place + 24, static_cast<uint64_t>(static_cast<uint32_t>(mine.best)) |
-                               static_cast<uint64_t>(static_cast<uint32_t>(mine.bad)) << 32);
+    if (lane == 0) {
+      of_warp[warp] = mine;
+      sums_of_warp[warp] = mine.p_sum;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      Told one;
+      one.p_sum = one.q_sum = 0.0;
+      one.p_max = one.q_max = -INFINITY;
+      one.best = 0x7fffffff;
+      one.bad = 0;
+      if (lane < WARPS) one = of_warp[lane];
+      Told cta;
+      if (plain_sums) {
+        cta = one;
+        cta.p_sum = warp_sum(one.p_sum);
+      } else {
+        cta = join_told(one, table, unit);
+      }
+      if (lane < ctas) {
+        const uint32_t place = address_in(&of_cta[phase][rank], lane);
+        store_in(place, __double_as_longlong(cta.p_sum));
+        store_in(place + 8, __double_as_longlong(cta.q_sum));
+        store_in(place + 16, static_cast<uint64_t>(__float_as_uint(cta.p_max)) |
+                                 static_cast<uint64_t>(__float_as_uint(cta.q_max)) << 32);
+        store_in(place + 24, static_cast<uint64_t>(static_cast<uint32_t>(cta.best)) |
+                                 static_cast<uint64_t>(static_cast<uint32_t>(cta.bad)) << 32);
+      }
     }
     cluster_sync();
   };
+  auto parent_at = [&](int j) { return held_tree ? parent_of[j] : a.parents[begin + j]; };
+  auto id_at = [&](int j) { return held_tree ? id_of[j] : a.ids[begin + j]; };
+  auto number_at = [&](int j) { return held_tree ? number_of[j] : a.uniform[begin + j]; };
   // the next child of `node` behind `after`, or `nodes`
   auto child_of = [&](int node, int after) {
     for (int base = after + 1; base < nodes; base += 32) {
       const int j = base + lane;
-      const unsigned found = __ballot_sync(0xffffffffu, j < nodes && a.parents[begin + j] == node);
+      const unsigned found = __ballot_sync(0xffffffffu, j < nodes && parent_at(j) == node);
       if (found != 0u) return base + __ffs(found) - 1;
     }
     return nodes;
@@ -186,112 +252,134 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
     const bool drafted = a.draft != nullptr && child < nodes && !greedy;
     const float* draft = drafted ? a.draft + static_cast<size_t>(begin + node) * a.ld_draft : row;
 
-    // ---- this warp's stretch of both rows
+    // calls take(id, p, q) for this lane's tokens of the warp's stretch: four side by side of each 128.  (A
+    // stretch is read two or three times; it stays in L1.  In registers, which it would fit, the exponentials of
+    // a whole stretch are in flight and spill.)
+    auto each = [&](auto take) {
+#pragma unroll 2
+      for (int id = first + 4 * lane; id < last; id += 128) {
+        float p[4], q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (wide && id + 3 < last) {
+          const float4 four = __ldg(reinterpret_cast<const float4*>(row + id));
+          p[0] = four.x; p[1] = four.y; p[2] = four.z; p[3] = four.w;
+          if (drafted) {
+            const float4 other = __ldg(reinterpret_cast<const float4*>(draft + id));
+            q[0] = other.x; q[1] = other.y; q[2] = other.z; q[3] = other.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (id + e < last) {
+              p[e] = __ldg(row + id + e);
+              if (drafted) q[e] = __ldg(draft + id + e);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (id + e < last) take(id + e, p[e], q[e]);
+      }
+    };
+    // lane k: the k-th child (of the first 32) and its logits
+    int my_child = nodes, my_token = -1;
+    float my_p = 0.0f, my_q = 0.0f;
+    if (!greedy && child < nodes) {
+      int count = 0;
+      for (int j = child; j < nodes && count < 32; j = child_of(node, j), ++count)
+        if (lane == count) my_child = j;
+      if (my_child < nodes) my_token = id_at(my_child);
+      if (my_token >= 0 && my_token < a.vocab) {
+        my_p = __ldg(row + my_token);
+        if (drafted) my_q = __ldg(draft + my_token);
+      }
+    }
+    // the rows that come next if the first child stands
+    if (child < nodes && lane < 8 && first + 32 * lane < last) {
+      const size_t ahead = static_cast<size_t>(begin + child);
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.logits + ahead * a.ld + first + 32 * lane));
+      if (drafted) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.draft + ahead * a.ld_draft + first + 32 * lane));
+    }
+
     Told mine;
     mine.p_max = mine.q_max = -INFINITY;
     mine.best = 0x7fffffff;
     bool bad = false;
-    auto take = [&](float p, float q, int id) {
+    each([&](int id, float p, float q) {
       bad |= !isfinite(p) || !(q < INFINITY);      // (a draft may leave tokens out: minus infinity)
       if (p > mine.p_max) {
         mine.p_max = p;
         mine.best = id;
       }
       mine.q_max = fmaxf(mine.q_max, q);
-    };
-#pragma unroll 4
-    for (int id = first + lane; id < last; id += 32) take(row[id], drafted ? draft[id] : 0.0f, id);
+    });
 #pragma unroll
     for (int offset = 16; offset > 0; offset >>= 1) {
-      const float other = __shfl_xor_sync(0xffffffffu, mine.p_max, offset);
-      const int other_best = __shfl_xor_sync(0xffffffffu, mine.best, offset);
-      if (other > mine.p_max || (other == mine.p_max && other_best < mine.best)) {
-        mine.p_max = other;
-        mine.best = other_best;
-      }
+      take_larger(mine.p_max, mine.best, __shfl_xor_sync(0xffffffffu, mine.p_max, offset),
+                  __shfl_xor_sync(0xffffffffu, mine.best, offset));
       mine.q_max = fmaxf(mine.q_max, __shfl_xor_sync(0xffffffffu, mine.q_max, offset));
     }
     mine.bad = __any_sync(0xffffffffu, bad);
     mine.p_sum = mine.q_sum = 0.0;
     if (!greedy && !mine.bad && first < last) {
       const Exponential of_p{table, unit, mine.p_max};
-      // (a stretch that the draft leaves out wholly has no maximum: its sum is zero)
-      const bool any_q = drafted && mine.q_max > -INFINITY;
-      const Exponential of_q{table, unit, any_q ? mine.q_max : 0.0f};
-      for (int id = first + lane; id < last; id += 32) {
-        mine.p_sum += of_p(row[id]);
-        if (any_q) mine.q_sum += of_q(draft[id]);
-      }
-      mine.p_sum = warp_sum(mine.p_sum);
-      mine.q_sum = warp_sum(mine.q_sum);
+      // (a stretch that the draft leaves out wholly has no maximum: its sum is zero against any)
+      const Exponential of_q{table, unit, fmaxf(mine.q_max, -3.0e38f)};
+      double p_sum = 0.0, q_sum = 0.0;
+      each([&](int, float p, float q) {
+        p_sum += of_p(p);
+        if (drafted) q_sum += of_q(q);
+      });
+      mine.p_sum = warp_sum(p_sum);
+      if (drafted) mine.q_sum = warp_sum(q_sum);
     }
-    tell(mine);
-
-    // ---- everybody's: the same sums in the same order in every warp
-    const Told* all = told[phase];
-    float p_top = -INFINITY, q_top = -INFINITY;
-    int best = 0x7fffffff, any_bad = 0;
-    for (int w = lane; w < owners; w += 32) {
-      if (all[w].p_max > p_top || (all[w].p_max == p_top && all[w].best < best)) {
-        p_top = all[w].p_max;
-        best = all[w].best;
-      }
-      q_top = fmaxf(q_top, all[w].q_max);
-      any_bad |= all[w].bad;
-    }
-#pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) {
-      const float other = __shfl_xor_sync(0xffffffffu, p_top, offset);
-      const int other_best = __shfl_xor_sync(0xffffffffu, best, offset);
-      if (other > p_top || (other == p_top && other_best < best)) {
-        p_top = other;
-        best = other_best;
-      }
-      q_top = fmaxf(q_top, __shfl_xor_sync(0xffffffffu, q_top, offset));
-    }
-    any_bad = __any_sync(0xffffffffu, any_bad);
-    if (any_bad || (drafted && q_top == -INFINITY)) {
+    tell(mine, false);
+    Told one;
+    one.p_sum = one.q_sum = 0.0;
+    one.p_max = one.q_max = -INFINITY;
+    one.best = 0x7fffffff;
+    one.bad = 0;
+    if (lane < ctas) one = of_cta[phase][lane];
+    const int first_phase = phase;
+    const Told all = join_told(one, table, unit);
+    if (all.bad || (drafted && all.q_max == -INFINITY)) {
       if (writes && lane == 0) {
         a.next[request] = -1;
         atomicOr(a.status, HX_FLAG_NONFINITE);
       }
       break;
     }
-    const Exponential of_p{table, unit, p_top}, of_q{table, unit, drafted ? q_top : 0.0f};
-    double p_all = 0.0, q_all = 0.0;
-    if (!greedy) {
-      for (int w = lane; w < owners; w += 32) {
-        if (all[w].p_sum > 0.0) p_all += all[w].p_sum * of_p(all[w].p_max);
-        if (all[w].q_sum > 0.0) q_all += all[w].q_sum * of_q(all[w].q_max);
-      }
-      p_all = warp_sum(p_all);
-      q_all = warp_sum(q_all);
-    }
-    const double p_unit = 1.0 / p_all, q_unit = drafted ? 1.0 / q_all : 0.0;
+    const Exponential of_p{table, unit, all.p_max}, of_q{table, unit, drafted ? all.q_max : 0.0f};
+    const double p_unit = 1.0 / all.p_sum, q_unit = drafted ? 1.0 / all.q_sum : 0.0;
 
     // ---- the children, in order
     double b = 0.0, left = 1.0, gone = 0.0;
     int fallen = 0;            // without a draft model: different tokens that fell, whose p is out of `left`
     int fallen_token = -1;     // lane f: the f-th of them
     int stands = -1;
-    for (; child < nodes; child = child_of(node, child)) {
-      const int token = a.ids[begin + child];
+    // lane k: the k-th child's shares, before anything fell
+    const double my_p_share = !greedy && my_token >= 0 ? of_p(my_p) * p_unit : 0.0;
+    const double my_q_share = drafted && my_token >= 0 ? of_q(my_q) * q_unit : 0.0;
+    int order = 0;
+    for (; child < nodes; child = child_of(node, child), ++order) {
+      const int token = id_at(child);
       if (token < 0 || token >= a.vocab) {
         bad_token = 1;      // passed over
         continue;
       }
       if (greedy) {
-        if (token != best) continue;
+        if (token != all.best) continue;
         stands = child;
         break;
       }
-      const double u = a.uniform[begin + child];
-      const double p = of_p(row[token]) * p_unit;
+      const double u = number_at(child);
+      double p = __shfl_sync(0xffffffffu, my_p_share, order & 31), q = __shfl_sync(0xffffffffu, my_q_share, order & 31);
+      if (order >= 32) {
+        p = of_p(__ldg(row + token)) * p_unit;
+        q = drafted ? of_q(__ldg(draft + token)) * q_unit : 0.0;
+      }
       if (drafted) {
         const double rest = 1.0 - gone;
         if (!(rest > 0.0)) continue;      // nothing of q is left to have been drawn from
         const double scale = a.put_back ? 1.0 : 1.0 / rest;
-        const double q = of_q(draft[token]) * q_unit;
         if (u * q * scale * left < p - b * q) {
           stands = child;
           break;
@@ -299,21 +387,19 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
         b += left * scale;
         if (!a.put_back) gone += q;
         double sum = 0.0;
-        for (int id = first + lane; id < last; id += 32) {
-          const double over = of_p(row[id]) * p_unit - b * (of_q(draft[id]) * q_unit);
+        const double b_unit = b * q_unit;
+        each([&](int, float p_logit, float q_logit) {
+          const double over = of_p(p_logit) * p_unit - b_unit * of_q(q_logit);
           if (over > 0.0) sum += over;
-        }
+        });
         mine.p_sum = warp_sum(sum);
-        mine.p_max = p_top;
-        tell(mine);
-        left = 0.0;
-        for (int w = lane; w < owners; w += 32) left += told[phase][w].p_sum;
-        left = warp_sum(left);
+        tell(mine, true);
+        left = warp_sum(lane < ctas ? of_cta[phase][lane].p_sum : 0.0);
       } else {
         // fell already: nothing of it is left
         bool again = __any_sync(0xffffffffu, lane < fallen && fallen_token == token);
         if (fallen > 32)
-          for (int j = child_of(node, node); j < child; j = child_of(node, j)) again |= a.ids[begin + j] == token;
+          for (int j = child_of(node, node); j < child; j = child_of(node, j)) again |= id_at(j) == token;
         if (again) continue;
         if (u * left < p) {
           stands = child;
@@ -333,96 +419,108 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
 
     // ---- none stands: the next token, from what is left
     if (greedy) {
-      if (writes && lane == 0) a.next[request] = best;
+      if (writes && lane == 0) a.next[request] = all.best;
       break;
     }
-    const double u = a.uniform[begin];
+    const double u = number_at(0);
     const bool plain = !(left > 0.0) || (fallen == 0 && b == 0.0);      // (nothing left but by rounding: p itself)
     const bool listed = !plain && fallen > 0;      // the fallen children's tokens weigh nothing
-    // has token base + lane fallen? (the warp asks together)
+    // has the token fallen? (the warp asks together)
     auto fell = [&](int id) {
       bool out = false;
       for (int f = 0; f < min(fallen, 32); ++f) out |= id == __shfl_sync(0xffffffffu, fallen_token, f);
       if (fallen > 32)
-        for (int j = child_of(node, node); j < nodes; j = child_of(node, j)) out |= a.ids[begin + j] == id;
+        for (int j = child_of(node, node); j < nodes; j = child_of(node, j)) out |= id_at(j) == id;
       return out;
     };
-    auto weight = [&](int id) {
-      if (plain || listed) return of_p(row[id]) * p_unit;
-      const double over = of_p(row[id]) * p_unit - b * (of_q(draft[id]) * q_unit);
+    const double b_unit = b * q_unit;
+    auto weight = [&](float p_logit, float q_logit) {
+      const double p = of_p(p_logit) * p_unit;
+      if (plain || listed) return p;
+      const double over = p - b_unit * of_q(q_logit);
       return over > 0.0 ? over : 0.0;
+    };
+    // four tokens of this lane from `id` on, of which the fallen and those behind the stretch weigh nothing
+    auto weights_of = [&](int id, double (&w)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool out = listed && fell(id + e);
+        w[e] = id + e < last && !out ? weight(__ldg(row + id + e), drafted ? __ldg(draft + id + e) : 0.0f) : 0.0;
+      }
     };
     // every warp's sum: p's from the row's first exchange, what is over from that of the last fallen
     // child, otherwise told now
-    const bool first_sums = plain && b == 0.0;
+    const bool first_sums = plain && phase == first_phase;
     if (listed || (plain && !first_sums)) {
       double sum = 0.0;
-      for (int base = first; base < last; base += 32) {
-        const bool out = listed && fell(base + lane);
-        if (base + lane < last && !out) sum += weight(base + lane);
+      for (int base = first; base < last; base += 128) {
+        double w[4];
+        weights_of(base + 4 * lane, w);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
       }
       mine.p_sum = warp_sum(sum);
-      tell(mine);
+      tell(mine, true);
     }
-    auto sum_of = [&](int w) {
-      const Told& of = told[phase][w];
-      return !first_sums ? of.p_sum : of.p_sum > 0.0 ? of.p_sum * of_p(of.p_max) * p_unit : 0.0;
+    // the CTA in which the running sum passes the target, and in it the warp; all add alike and agree
+    auto pick = [&](double sum, int count, double target, double& before) {
+      double inclusive = lane < count ? sum : 0.0;
+#pragma unroll
+      for (int offset = 1; offset < 32; offset <<= 1) {
+        const double other = __shfl_up_sync(0xffffffffu, inclusive, offset);
+        if (lane >= offset) inclusive += other;
+      }
+      const bool some = lane < count && sum > 0.0;
+      const unsigned beyond = __ballot_sync(0xffffffffu, some && target < before + inclusive);
+      const unsigned weighs = __ballot_sync(0xffffffffu, some);
+      // (a sum that falls short by rounding: the last with any weight)
+      const int source = beyond != 0u ? __ffs(beyond) - 1 : 31 - __clz(weighs | 1u);
+      before += __shfl_sync(0xffffffffu, inclusive - (lane < count ? sum : 0.0), source);
+      return source;
     };
-    // the stretch in which the running sum passes the target; all warps add alike and agree on it
-    const int each = (owners + 31) / 32, own_first = min(lane * each, owners), own_last = min(own_first + each, owners);
-    double lane_sum = 0.0;
-    int owner = -1;
-    for (int w = own_first; w < own_last; ++w) {
-      const double sum = sum_of(w);
-      lane_sum += sum;
-      if (sum > 0.0) owner = w;
+    double cta_sum = 0.0;
+    if (lane < ctas) {
+      const Told& of = of_cta[phase][lane];
+      cta_sum = !first_sums ? of.p_sum : of.p_sum > 0.0 ? of.p_sum * of_p(of.p_max) * p_unit : 0.0;
     }
-    double inclusive_sum = lane_sum;
-#pragma unroll
-    for (int offset = 1; offset < 32; offset <<= 1) {
-      const double other = __shfl_up_sync(0xffffffffu, inclusive_sum, offset);
-      if (lane >= offset) inclusive_sum += other;
-    }
-    const double target = u * __shfl_sync(0xffffffffu, inclusive_sum, 31);
-    const unsigned beyond = __ballot_sync(0xffffffffu, owner >= 0 && target < inclusive_sum);
-    const unsigned weighs = __ballot_sync(0xffffffffu, owner >= 0);
-    // (a sum that falls short by rounding: the last stretch with any weight)
-    const int source = beyond != 0u ? __ffs(beyond) - 1 : 31 - __clz(weighs | 1u);
-    double before = inclusive_sum - lane_sum;
-    if (beyond != 0u) {
-      double running = before;
-      for (int w = own_first; w < own_last; ++w) {
-        const double sum = sum_of(w);
-        if (sum > 0.0 && target < running + sum) {
-          owner = w;
-          break;
-        }
-        running += sum;
+    const double target = u * warp_sum(cta_sum);
+    double before = 0.0;
+    if (pick(cta_sum, ctas, target, before) == rank) {
+      double sum = 0.0;
+      if (lane < WARPS) {
+        sum = sums_of_warp[lane];
+        if (first_sums && sum > 0.0) sum *= of_p(of_warp[lane].p_max) * p_unit;
       }
-      before = running;
-    }
-    owner = __shfl_sync(0xffffffffu, owner, source);
-    before = __shfl_sync(0xffffffffu, before, source);
-    if (owner == me) {
-      int chosen = -1, last_with_weight = -1;
-      for (int base = first; base < last && chosen < 0; base += 32) {
-        const int id = base + lane;
-        const bool out = listed && fell(id);
-        const double w = id < last && !out ? weight(id) : 0.0;
-        double inclusive = w;
+      if (pick(sum, WARPS, target, before) == warp) {
+        int chosen = -1, last_with_weight = -1;
+        for (int base = first; base < last && chosen < 0; base += 128) {
+          const int id = base + 4 * lane;
+          double w[4];
+          weights_of(id, w);
+          double inclusive = (w[0] + w[1]) + (w[2] + w[3]);
+          const double own = inclusive;
 #pragma unroll
-        for (int offset = 1; offset < 32; offset <<= 1) {
-          const double other = __shfl_up_sync(0xffffffffu, inclusive, offset);
-          if (lane >= offset) inclusive += other;
+          for (int offset = 1; offset < 32; offset <<= 1) {
+            const double other = __shfl_up_sync(0xffffffffu, inclusive, offset);
+            if (lane >= offset) inclusive += other;
+          }
+          // this lane's first token whose running sum passes the target, and its last with any weight
+          int passes = -1, heavy = -1;
+          double running = before + (inclusive - own);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            running += w[e];
+            if (w[e] > 0.0) heavy = id + e;
+            if (passes < 0 && w[e] > 0.0 && target < running) passes = id + e;
+          }
+          const unsigned passed = __ballot_sync(0xffffffffu, passes >= 0);
+          const unsigned weighs = __ballot_sync(0xffffffffu, heavy >= 0);
+          if (weighs != 0u) last_with_weight = __shfl_sync(0xffffffffu, heavy, 31 - __clz(weighs));
+          if (passed != 0u) chosen = __shfl_sync(0xffffffffu, passes, __ffs(passed) - 1);
+          before += __shfl_sync(0xffffffffu, inclusive, 31);
         }
-        const unsigned passed = __ballot_sync(0xffffffffu, w > 0.0 && target < before + inclusive);
-        const unsigned heavy = __ballot_sync(0xffffffffu, w > 0.0);
-        if (heavy != 0u) last_with_weight = base + 31 - __clz(heavy);
-        if (passed != 0u) chosen = base + __ffs(passed) - 1;
-        before += __shfl_sync(0xffffffffu, inclusive, 31);
+        if (chosen < 0) chosen = last_with_weight;      // the running sum fell short by rounding
+        if (lane == 0) a.next[request] = chosen;
       }
-      if (chosen < 0) chosen = last_with_weight;      // the running sum fell short by rounding
-      if (lane == 0) a.next[request] = chosen;
     }
     break;
   }
@@ -456,10 +554,14 @@ HX_API int hx_verify_drafts(const float* logits, int ld, const float* draft, int
   if (requests == 0) return HX_OK;
   const int sms = hx_device_sm_count();
   HX_REQUIRE(sms > 0, "hx_verify_drafts: the device cannot be asked");
-  // as many CTAs a request as leave two an SM, and no more than have 32 x 4 tokens a warp
-  int ctas = MAX_CLUSTER;
-  while (ctas > 1 && (static_cast<long long>(requests) * ctas > 2ll * sms || vocab <= (ctas / 2) * WARPS * 128)) ctas /= 2;
   HX_REQUIRE(requests <= (1 << 24), "hx_verify_drafts: too many requests");
+#ifndef HX_VC
+#define HX_VC 2
+#endif
+  // as many CTAs a request as fit the GPU at once, two an SM (the walk of the deepest request, whose length is
+  // latency, is what a batch waits for), and no more than have 32 x 4 tokens a warp
+  int ctas = MAX_CLUSTER;
+  while (ctas > 1 && (static_cast<long long>(requests) * ctas > HX_VC * (long long)sms || vocab <= (ctas / 2) * WARPS * 128)) ctas /= 2;
   int span = (vocab + ctas * WARPS - 1) / (ctas * WARPS);
   span = (span + 127) / 128 * 128;
   VerifyArgs a{logits, ld, draft, ld_draft, token_ids, parents, request_start, temperature, uniform, path, ld_path,
