@@ -17,6 +17,7 @@
 //   * tree_tile_kernel: any other page size, float32 or bfloat16, heads up to 256 in steps of 4.
 //     32 rows by 64 keys at a time on the CUDA cores, all in float32;
 //   * tree_row_kernel: what is left (heads up to 1,024, even), a row a warp.
+#include "hx_mma.cuh"
 #include "hx_tree_attention.cuh"
 
 #include <mutex>
@@ -50,14 +51,26 @@ template <> __device__ __forceinline__ float4 load_four<__nv_bfloat16>(const __n
                      __bfloat162float(high.y));
 }
 
-// Scores: a warp has 8 rows, a lane 2 keys; a key's four coordinates are read once for 8 rows, a
-// row's are broadcast.  Values: a lane has 4 (8, above 128) coordinates of the same 8 rows.  Per SM the
-// shared-memory reads of both products take about as long as their multiply-adds, which is the bound.
+// 16 bytes of float32, or four bfloat16 as float32, on their way into shared memory.
+template <typename T> __device__ __forceinline__ void bring_four(float* place, const T* from, bool there);
+template <> __device__ __forceinline__ void bring_four<float>(float* place, const float* from, bool there) {
+  hx_cp_async_16(hx_shared_address(place), from, there ? 16 : 0);
+}
+template <> __device__ __forceinline__ void bring_four<__nv_bfloat16>(float* place, const __nv_bfloat16* from, bool there) {
+  *reinterpret_cast<float4*>(place) = there ? load_four<__nv_bfloat16>(from) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+}
+
+// A warp has 8 rows of the tile.  Scores: a lane has 4 keys (16 apart) of 4 rows, so that 12 reads of 128
+// bytes of shared memory feed 64 multiply-adds of a warp.  Values: a lane has 4 (8, above 128)
+// coordinates of all 8 rows.  Both are bound by the multiply-adds, 3,900 cycles a tile of heads of 112;
+// two CTAs an SM, one of which copies a tile while the other computes.  A thread copies a key's pieces,
+// whose page it has looked up during the tile before.
 template <typename T, int D_MAX>
 __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tree_tile_kernel(
     const TreeArgs a) {
   extern __shared__ float4 tile_shared[];
   constexpr int OUT_PIECES = (D_MAX + 127) / 128;
+  static_assert(TILE_KEYS == 64 && TILE_WARPS * 32 == 2 * TILE_KEYS, "two threads copy a key");
   hx_pdl_prologue();
   const int D = a.head_dim, D4 = D / 4;
   float* q_rows = reinterpret_cast<float*>(tile_shared);
@@ -75,6 +88,10 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
   const T* k_cache = static_cast<const T*>(a.k_cache);
   const T* v_cache = static_cast<const T*>(a.v_cache);
   const float scale_log2 = a.scale * HX_LOG2E;
+  const int my_key = threadIdx.x % TILE_KEYS, my_half = threadIdx.x / TILE_KEYS;      // of a tile's copies
+  const int key_x = lane & 15, row_y = lane >> 4;                                     // of a tile's scores
+  // four coordinates on: the next piece of `chunk`, or further in the same one
+  const int pieces_a_chunk = chunk / 4;
 
   for (int left = run.count; left > 0;) {
     const int count = min(c.tiles - c.tile, left);
@@ -82,6 +99,11 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
     const int rows_here = rows.count, kv_head = rows.kv_head;
     const int last_key = c.context + c.nodes - 1;
     const int* table = a.block_tables + static_cast<size_t>(a.request_table_row[c.request]) * a.table_stride;
+    auto page_of = [&](int key) {
+      const int index = key / a.page_size;
+      return key <= last_key && index < a.table_stride ? table[index] : -1;
+    };
+    int page = page_of(c.tile * TILE_KEYS + my_key);
     __syncthreads();
     for (int i = threadIdx.x; i < TILE_ROWS * D4; i += blockDim.x) {
       const int row = i / D4, d4 = i - row * D4;
@@ -91,98 +113,116 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
                              static_cast<size_t>(rows.head0 + row % rows.heads) * D + 4 * d4);
       reinterpret_cast<float4*>(q_rows)[row * D4 + d4] = value;
     }
-    float row_max[ROWS_A_WARP], row_sum[ROWS_A_WARP];
+    float row_max[4], row_sum[4];      // of the rows whose scores this lane has
+    const unsigned long long* words[4];
+    unsigned long long first_word[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = warp * ROWS_A_WARP + 4 * row_y + j;
+      words[j] = tree_words(a, c, rows.token0 + min(row, rows_here - 1) / rows.heads);
+      first_word[j] = __ldg(words[j]);
+      row_max[j] = -INFINITY;
+      row_sum[j] = 0.0f;
+    }
     float4 acc[ROWS_A_WARP][OUT_PIECES];
 #pragma unroll
-    for (int i = 0; i < ROWS_A_WARP; ++i) {
-      row_max[i] = -INFINITY;
-      row_sum[i] = 0.0f;
+    for (int i = 0; i < ROWS_A_WARP; ++i)
 #pragma unroll
       for (int j = 0; j < OUT_PIECES; ++j) acc[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
     const bool live = warp * ROWS_A_WARP < rows_here;      // this warp has rows
     for (int t = 0; t < count; ++t) {
       const int key0 = (c.tile + t) * TILE_KEYS;
       __syncthreads();      // the last tile has been read (and the queries are written)
       // ---- keys and values of the tile; a key that does not exist or has no page is zeros
-      for (int i = threadIdx.x; i < TILE_KEYS * D4; i += blockDim.x) {
-        const int d4 = i / TILE_KEYS, key = i - d4 * TILE_KEYS;
-        float4 kv = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vv = kv;
-        if (key0 + key <= last_key) {
-          const int index = (key0 + key) / a.page_size;
-          const int page = index < a.table_stride ? table[index] : -1;
-          if (page < 0 || page >= a.num_pages) {
-            if (d4 == 0) atomicOr(a.status, HX_FLAG_BAD_PAGE);
-          } else {
-            const size_t at = hx_cache_offset(page, kv_head, (key0 + key) % a.page_size, 4 * d4, a.kv_heads,
-                                              a.page_size, D, chunk);
-            kv = load_four<T>(k_cache + at);
-            vv = load_four<T>(v_cache + at);
-          }
+      {
+        const int key = key0 + my_key;
+        const bool there = page >= 0 && page < a.num_pages && key <= last_key;
+        if (key <= last_key && !there && my_half == 0) atomicOr(a.status, HX_FLAG_BAD_PAGE);
+        const size_t at = there ? hx_cache_offset(page, kv_head, key % a.page_size, 0, a.kv_heads, a.page_size, D, chunk) : 0;
+        // (coordinates 4 d4: a chunk's first, or further on in it)
+#pragma unroll 4
+        for (int d4 = my_half; d4 < D4; d4 += 2) {
+          const size_t from = at + static_cast<size_t>(d4 / pieces_a_chunk) * a.page_size * chunk + d4 % pieces_a_chunk * 4;
+          bring_four<T>(keys + (d4 * TILE_KEYS + my_key) * 4, k_cache + (there ? from : 0), there);
+          bring_four<T>(values + my_key * (D + 4) + 4 * d4, v_cache + (there ? from : 0), there);
         }
-        reinterpret_cast<float4*>(keys)[d4 * TILE_KEYS + key] = kv;
-        *reinterpret_cast<float4*>(values + key * (D + 4) + 4 * d4) = vv;
+        hx_cp_async_commit();
+        page = t + 1 < count ? page_of(key + TILE_KEYS) : -1;
+        hx_cp_async_wait<0>();
       }
       __syncthreads();
       if (!live) continue;
-      // ---- scores of 8 rows against keys `lane` and `lane + 32`
-      float s[ROWS_A_WARP][2];
+      // ---- scores of rows 4 row_y + j against keys key_x + 16 i
+      float s[4][4];
 #pragma unroll
-      for (int i = 0; i < ROWS_A_WARP; ++i) s[i][0] = s[i][1] = 0.0f;
-      const float4* my_q = reinterpret_cast<const float4*>(q_rows) + warp * ROWS_A_WARP * D4;
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[j][i] = 0.0f;
+      const float4* my_q = reinterpret_cast<const float4*>(q_rows) + (warp * ROWS_A_WARP + 4 * row_y) * D4;
+      const float4* my_k = reinterpret_cast<const float4*>(keys) + key_x;
 #pragma unroll 2
       for (int d4 = 0; d4 < D4; ++d4) {
-        const float4 k0 = reinterpret_cast<const float4*>(keys)[d4 * TILE_KEYS + lane];
-        const float4 k1 = reinterpret_cast<const float4*>(keys)[d4 * TILE_KEYS + lane + 32];
+        float4 k[4], w[4];
 #pragma unroll
-        for (int i = 0; i < ROWS_A_WARP; ++i) {
-          const float4 qi = my_q[i * D4 + d4];
-          s[i][0] = fmaf(qi.x, k0.x, s[i][0]);
-          s[i][1] = fmaf(qi.x, k1.x, s[i][1]);
-          s[i][0] = fmaf(qi.y, k0.y, s[i][0]);
-          s[i][1] = fmaf(qi.y, k1.y, s[i][1]);
-          s[i][0] = fmaf(qi.z, k0.z, s[i][0]);
-          s[i][1] = fmaf(qi.z, k1.z, s[i][1]);
-          s[i][0] = fmaf(qi.w, k0.w, s[i][0]);
-          s[i][1] = fmaf(qi.w, k1.w, s[i][1]);
-        }
+        for (int i = 0; i < 4; ++i) k[i] = my_k[d4 * TILE_KEYS + 16 * i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = my_q[j * D4 + d4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[j][i] = fmaf(w[j].x, k[i].x, s[j][i]);
+            s[j][i] = fmaf(w[j].y, k[i].y, s[j][i]);
+            s[j][i] = fmaf(w[j].z, k[i].z, s[j][i]);
+            s[j][i] = fmaf(w[j].w, k[i].w, s[j][i]);
+          }
       }
-      // ---- the running maximum and sum of every row
+      // ---- the running maximum and sum of every row (sixteen lanes have one)
+      const bool drafted = key0 + TILE_KEYS > c.context;
+      float correction[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = warp * ROWS_A_WARP + 4 * row_y + j;
+        unsigned long long mask = ~0ull;
+        if (drafted)
+          mask = row < rows_here ? tree_mask_of(a, c, key0, first_word[j], [&](int word) { return words[j][word]; }) : 0ull;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[j][i] = (mask >> (key_x + 16 * i)) & 1 ? s[j][i] * scale_log2 : -INFINITY;
+          top = fmaxf(top, s[j][i]);
+        }
+#pragma unroll
+        for (int offset = 8; offset > 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+        const float new_max = fmaxf(row_max[j], top);
+        const float against = new_max == -INFINITY ? 0.0f : new_max;
+        correction[j] = exp2f(row_max[j] - against);
+        row_max[j] = new_max;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = exp2f(s[j][i] - against);
+          sum += p;
+          probabilities[row * TILE_KEYS + key_x + 16 * i] = p;
+        }
+#pragma unroll
+        for (int offset = 8; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+        row_sum[j] = fmaf(row_sum[j], correction[j], sum);
+      }
 #pragma unroll
       for (int i = 0; i < ROWS_A_WARP; ++i) {
-        const int row = warp * ROWS_A_WARP + i;
-        unsigned long long mask = ~0ull;
-        if (key0 + TILE_KEYS > c.context)
-          mask = row < rows_here ? tree_mask(a, c, rows.token0 + row / rows.heads, key0) : 0ull;
-        const float s0 = (mask >> lane) & 1 ? s[i][0] * scale_log2 : -INFINITY;
-        const float s1 = (mask >> (lane + 32)) & 1 ? s[i][1] * scale_log2 : -INFINITY;
-        float top = fmaxf(s0, s1);
-#pragma unroll
-        for (int offset = 16; offset > 0; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
-        const float new_max = fmaxf(row_max[i], top);
-        const float against = new_max == -INFINITY ? 0.0f : new_max;
-        const float p0 = exp2f(s0 - against), p1 = exp2f(s1 - against);
-        const float correction = exp2f(row_max[i] - against);
-        float sum = p0 + p1;
-#pragma unroll
-        for (int offset = 16; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-        row_sum[i] = fmaf(row_sum[i], correction, sum);
-        row_max[i] = new_max;
-        probabilities[row * TILE_KEYS + lane] = p0;
-        probabilities[row * TILE_KEYS + lane + 32] = p1;
+        const float factor = __shfl_sync(0xffffffffu, correction[i % 4], i / 4 * 16);
 #pragma unroll
         for (int j = 0; j < OUT_PIECES; ++j) {
-          acc[i][j].x *= correction;
-          acc[i][j].y *= correction;
-          acc[i][j].z *= correction;
-          acc[i][j].w *= correction;
+          acc[i][j].x *= factor;
+          acc[i][j].y *= factor;
+          acc[i][j].z *= factor;
+          acc[i][j].w *= factor;
         }
       }
       __syncwarp();
       // ---- the weighted values: coordinates 4 lane .. of 8 rows, four keys at a time
       const float4* my_p = reinterpret_cast<const float4*>(probabilities) + warp * ROWS_A_WARP * (TILE_KEYS / 4);
-      // (a drafted key that a row does not see adds nothing to it, not even an infinity times zero)
-      const bool drafted = key0 + TILE_KEYS > c.context;
       const int keys_here = min(TILE_KEYS, last_key + 1 - key0);
       for (int key4 = 0; key4 * 4 < keys_here; ++key4) {
         float4 v[4][OUT_PIECES];
@@ -201,6 +241,7 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
           for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int j = 0; j < OUT_PIECES; ++j) {
+              // (a drafted key that a row does not see adds nothing to it, not even an infinity times zero)
               if (drafted && w[k] == 0.0f) continue;
               acc[i][j].x = fmaf(w[k], v[k][j].x, acc[i][j].x);
               acc[i][j].y = fmaf(w[k], v[k][j].y, acc[i][j].y);
@@ -216,9 +257,11 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
       float* part = tree_part<TILE_ROWS>(a, blockIdx.x, c.tile == 0);
 #pragma unroll
       for (int i = 0; i < ROWS_A_WARP; ++i) {
+        const float top = __shfl_sync(0xffffffffu, row_max[i % 4], i / 4 * 16);
+        const float sum = __shfl_sync(0xffffffffu, row_sum[i % 4], i / 4 * 16);
         const int row = warp * ROWS_A_WARP + i;
-        if (row >= rows_here) break;
-        const float inverse = row_sum[i] > 0.0f ? 1.0f / row_sum[i] : 0.0f;
+        if (row >= rows_here) continue;
+        const float inverse = sum > 0.0f ? 1.0f / sum : 0.0f;
         T* out = static_cast<T*>(a.out) + static_cast<size_t>(c.q_begin + rows.token0 + row / rows.heads) * a.ldo +
                  static_cast<size_t>(rows.head0 + row % rows.heads) * D;
 #pragma unroll
@@ -236,8 +279,8 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
           }
         }
         if (!whole && lane == 0) {
-          part[static_cast<size_t>(D) * TILE_ROWS + row] = row_max[i];
-          part[static_cast<size_t>(D + 1) * TILE_ROWS + row] = row_sum[i];
+          part[static_cast<size_t>(D) * TILE_ROWS + row] = top;
+          part[static_cast<size_t>(D + 1) * TILE_ROWS + row] = sum;
         }
       }
     }
@@ -558,7 +601,9 @@ int launch_tile(const TreeArgs& a, int ctas, cudaStream_t stream) {
   static bool reserved = false;
   std::call_once(once, [] {
     reserved = cudaFuncSetAttribute(tree_tile_kernel<T, D_MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    TileConfig<D_MAX>::floats(D_MAX) * 4) == cudaSuccess;
+                                    TileConfig<D_MAX>::floats(D_MAX) * 4) == cudaSuccess &&
+               cudaFuncSetAttribute(tree_tile_kernel<T, D_MAX>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared) == cudaSuccess;
     if (!reserved) cudaGetLastError();
   });
   HX_REQUIRE(reserved, "hx_tree_attention: cannot reserve shared memory");
