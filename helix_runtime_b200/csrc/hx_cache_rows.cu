@@ -79,6 +79,7 @@ struct KeepArgs {
   const int* kept;
   int kv_heads, page_size, num_pages;
   int pieces;            // units of a row: head_dim / c
+  int planes;
   int* status;
 };
 
@@ -87,12 +88,14 @@ struct KeepArgs {
 // reads its rows before it writes them, in ascending order, overwrites nothing that is still wanted.
 // Leading rows that stay where they are (path[k] = k) are left out.
 //
-// A CTA has a request, a plane and a share of its (head, unit) items; a warp's lanes hold the
-// rows of an item side by side (neighbouring slots of a page are neighbouring units), as many
-// items as fit.
+// A CTA has a request and a share of its (plane, head, unit) items: what it has to find out first (how many
+// rows, which, in which pages: a chain of loads) it finds out once for many of them.  A warp's
+// lanes hold the rows of an item side by side (neighbouring slots of a page are neighbouring units), as
+// many items as fit, and eight such loads are in flight.  A unit is 16 bytes of a sector of 32, so
+// that rows which move alone move twice their bytes.
 template <typename Unit>
 __global__ __launch_bounds__(THREADS) void keep_rows_kernel(const KeepArgs a) {
-  constexpr int LOADS = 4;      // items whose rows are in flight together
+  constexpr int LOADS = 8;      // items whose rows are in flight together
   hx_pdl_wait();      // (and lets nobody in early, see above)
   const int request = blockIdx.y;
   const int kept = a.kept[request];
@@ -135,31 +138,34 @@ __global__ __launch_bounds__(THREADS) void keep_rows_kernel(const KeepArgs a) {
   while (lanes < moved && lanes < 32) lanes *= 2;
   const int lane = threadIdx.x & 31, warps = THREADS / 32;
   const int items = a.kv_heads * a.pieces, items_a_warp = 32 / lanes;
-  const size_t plane = static_cast<size_t>(blockIdx.z) * a.num_pages;
+  const size_t plane_units = static_cast<size_t>(a.num_pages) * items * a.page_size;
   Unit* storage = reinterpret_cast<Unit*>(a.storage);
+  const int all_items = items * a.planes;
   const int stride = gridDim.x * warps * items_a_warp;
   for (int chunk = 0; chunk < moved; chunk += lanes) {
     const int k = first + chunk + lane % lanes;
     const bool mine = k < kept;
     int from_slot = 0, to_slot = 0;
-    size_t from_block = 0, to_block = 0;      // of the page's first item, in units
+    size_t from_block = 0, to_block = 0;      // of the page's first item in the first plane, in units
     if (mine) {
       const int from_page = page_at(context + path[k], from_slot), to_page = page_at(context + k, to_slot);
-      from_block = (plane + from_page) * items * a.page_size + from_slot;
-      to_block = (plane + to_page) * items * a.page_size + to_slot;
+      from_block = static_cast<size_t>(from_page) * items * a.page_size + from_slot;
+      to_block = static_cast<size_t>(to_page) * items * a.page_size + to_slot;
     }
     for (int item = (blockIdx.x * warps + (threadIdx.x >> 5)) * items_a_warp + lane / lanes;
-         __any_sync(0xffffffffu, item < items); item += LOADS * stride) {
+         __any_sync(0xffffffffu, item < all_items); item += LOADS * stride) {
       Unit value[LOADS];
+      size_t place[LOADS];
 #pragma unroll
-      for (int u = 0; u < LOADS; ++u)
-        if (mine && item + u * stride < items)
-          value[u] = storage[from_block + static_cast<size_t>(item + u * stride) * a.page_size];
+      for (int u = 0; u < LOADS; ++u) {
+        const int at = item + u * stride, plane = at / items;
+        place[u] = plane * plane_units + static_cast<size_t>(at - plane * items) * a.page_size;
+        if (mine && at < all_items) value[u] = storage[from_block + place[u]];
+      }
       __syncwarp();
 #pragma unroll
       for (int u = 0; u < LOADS; ++u)
-        if (mine && item + u * stride < items)
-          storage[to_block + static_cast<size_t>(item + u * stride) * a.page_size] = value[u];
+        if (mine && item + u * stride < all_items) storage[to_block + place[u]] = value[u];
     }
     __syncwarp();
   }
@@ -193,7 +199,7 @@ HX_API int hx_keep_rows(void* storage, int dtype, int planes, int num_pages, int
                         const int* request_context, const int* path, int ld_path, int width, const int* kept,
                         int requests, int* status, cudaStream_t stream) {
   HX_REQUIRE(dtype == HX_F32 || dtype == HX_BF16, "hx_keep_rows: unknown dtype %d", dtype);
-  HX_REQUIRE(planes > 0 && planes <= 65535 && num_pages > 0 && kv_heads > 0 && page_size > 0 && head_dim > 0 &&
+  HX_REQUIRE(planes > 0 && num_pages > 0 && kv_heads > 0 && page_size > 0 && head_dim > 0 &&
                  head_dim % 2 == 0 && table_stride > 0,
              "hx_keep_rows: bad cache geometry");
   HX_REQUIRE(requests >= 0 && requests <= 65535 && width > 0 && ld_path >= width, "hx_keep_rows: bad sizes");
@@ -203,10 +209,14 @@ HX_API int hx_keep_rows(void* storage, int dtype, int planes, int num_pages, int
   HX_REQUIRE(static_cast<long long>(kv_heads) * (head_dim / chunk) < (1 << 24), "hx_keep_rows: rows too long");
   if (requests == 0) return HX_OK;
   KeepArgs a{static_cast<uint8_t*>(storage), block_tables, table_stride, request_table_row, request_context, path,
-             ld_path, width, kept, kv_heads, page_size, num_pages, head_dim / chunk, status};
-  // a thread moves about four units of a path of four rows
-  const int items = kv_heads * (head_dim / chunk);
-  const dim3 grid((items + 2 * THREADS - 1) / (2 * THREADS), requests, planes);
+             ld_path, width, kept, kv_heads, page_size, num_pages, head_dim / chunk, planes, status};
+  // eight CTAs an SM together, and no more than have a round of loads each
+  const long long items = static_cast<long long>(kv_heads) * (head_dim / chunk) * planes;
+  HX_REQUIRE(items < (1ll << 30), "hx_keep_rows: too many heads and planes");
+  const int sms = hx_device_sm_count();
+  HX_REQUIRE(sms > 0, "hx_keep_rows: the device cannot be asked");
+  const long long wanted = (8ll * sms + requests - 1) / requests, most = (items + 8 * THREADS / 4 - 1) / (8 * THREADS / 4);
+  const dim3 grid(static_cast<unsigned>(wanted < most ? wanted : most), requests);
   if (unit == 16) hx_launch(keep_rows_kernel<uint4>, grid, THREADS, 0, stream, a);
   else if (unit == 8) hx_launch(keep_rows_kernel<uint2>, grid, THREADS, 0, stream, a);
   else hx_launch(keep_rows_kernel<uint32_t>, grid, THREADS, 0, stream, a);

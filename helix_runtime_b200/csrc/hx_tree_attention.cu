@@ -31,11 +31,9 @@ constexpr int TILE_LEAST = 2;      // key tiles of the shortest run
 
 template <int D_MAX>
 struct TileConfig {
-  // queries [32][D], keys [D / 4][64][4], values [64][D + 4], probabilities [32][64]
-  static constexpr int floats(int d) {
-    return TILE_ROWS * d + TILE_KEYS * d + TILE_KEYS * (d + 4) + TILE_ROWS * TILE_KEYS;
-  }
-  static constexpr int kCtas = floats(D_MAX) * 4 <= 110 * 1024 ? 2 : 1;
+  // queries [32][D], keys [D / 4][64][4] and then, in the same place, values [64][D + 4], probabilities [32][64]
+  static constexpr int floats(int d) { return TILE_ROWS * d + TILE_KEYS * (d + 4) + TILE_ROWS * TILE_KEYS; }
+  static constexpr int kCtas = D_MAX <= 128 ? 4 : 2;
 };
 
 // Four consecutive coordinates of a cached row, wherever the cache's pieces put them.
@@ -63,8 +61,9 @@ template <> __device__ __forceinline__ void bring_four<__nv_bfloat16>(float* pla
 // A warp has 8 rows of the tile.  Scores: a lane has 4 keys (16 apart) of 4 rows, so that 12 reads of 128
 // bytes of shared memory feed 64 multiply-adds of a warp.  Values: a lane has 4 (8, above 128)
 // coordinates of all 8 rows.  Both are bound by the multiply-adds, 3,900 cycles a tile of heads of 112;
-// two CTAs an SM, one of which copies a tile while the other computes.  A thread copies a key's pieces,
-// whose page it has looked up during the tile before.
+// what counts is that enough warps are there to wait for one another: a tile's values take the place of its
+// keys, so that four CTAs share an SM (two, with keys and values side by side and the next ones on
+// their way: 4 requests x 24 drafts 95 us).  A thread copies half a key, whose page it has looked up a tile before.
 template <typename T, int D_MAX>
 __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tree_tile_kernel(
     const TreeArgs a) {
@@ -75,8 +74,8 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
   const int D = a.head_dim, D4 = D / 4;
   float* q_rows = reinterpret_cast<float*>(tile_shared);
   float* keys = q_rows + TILE_ROWS * D;
-  float* values = keys + TILE_KEYS * D;
-  float* probabilities = values + TILE_KEYS * (D + 4);
+  float* values = keys;
+  float* probabilities = keys + TILE_KEYS * (D + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TreeRun run = tree_run<TILE_KEYS>(a, blockIdx.x, gridDim.x, TILE_LEAST);
   if (threadIdx.x == 0) tree_tell_none<TILE_ROWS>(a);
@@ -103,8 +102,23 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
       const int index = key / a.page_size;
       return key <= last_key && index < a.table_stride ? table[index] : -1;
     };
-    int page = page_of(c.tile * TILE_KEYS + my_key);
-    __syncthreads();
+    // the pieces of a key (or value) of this thread; one that does not exist or has no page is zeros
+    auto bring = [&](int key, int page, const T* cache, float* place, int stride) {
+      const bool there = page >= 0 && page < a.num_pages && key <= last_key;
+      const T* from = cache + (there ? hx_cache_offset(page, kv_head, key % a.page_size, 0, a.kv_heads, a.page_size, D, chunk) : 0);
+      const size_t step = there ? static_cast<size_t>(a.page_size) * chunk : 0;
+#pragma unroll 4
+      for (int d4 = my_half; d4 < D4; d4 += 2)      // (coordinates 4 d4: a chunk's first, or further on in it)
+        bring_four<T>(place + d4 * stride, from + d4 / pieces_a_chunk * step + (there ? d4 % pieces_a_chunk * 4 : 0), there);
+      hx_cp_async_commit();
+      return there || key > last_key;
+    };
+    float* my_keys = keys + my_key * 4;
+    float* my_values = values + my_key * (D + 4);
+    int key = c.tile * TILE_KEYS + my_key;      // of the tile that is copied next
+    int page = page_of(key), page_after = count > 1 ? page_of(key + TILE_KEYS) : -1;
+    __syncthreads();      // the last item's tiles have been read
+    if (!bring(key, page, k_cache, my_keys, 4 * TILE_KEYS)) atomicOr(a.status, HX_FLAG_BAD_PAGE);
     for (int i = threadIdx.x; i < TILE_ROWS * D4; i += blockDim.x) {
       const int row = i / D4, d4 = i - row * D4;
       float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -132,26 +146,8 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
     const bool live = warp * ROWS_A_WARP < rows_here;      // this warp has rows
     for (int t = 0; t < count; ++t) {
       const int key0 = (c.tile + t) * TILE_KEYS;
-      __syncthreads();      // the last tile has been read (and the queries are written)
-      // ---- keys and values of the tile; a key that does not exist or has no page is zeros
-      {
-        const int key = key0 + my_key;
-        const bool there = page >= 0 && page < a.num_pages && key <= last_key;
-        if (key <= last_key && !there && my_half == 0) atomicOr(a.status, HX_FLAG_BAD_PAGE);
-        const size_t at = there ? hx_cache_offset(page, kv_head, key % a.page_size, 0, a.kv_heads, a.page_size, D, chunk) : 0;
-        // (coordinates 4 d4: a chunk's first, or further on in it)
-#pragma unroll 4
-        for (int d4 = my_half; d4 < D4; d4 += 2) {
-          const size_t from = at + static_cast<size_t>(d4 / pieces_a_chunk) * a.page_size * chunk + d4 % pieces_a_chunk * 4;
-          bring_four<T>(keys + (d4 * TILE_KEYS + my_key) * 4, k_cache + (there ? from : 0), there);
-          bring_four<T>(values + my_key * (D + 4) + 4 * d4, v_cache + (there ? from : 0), there);
-        }
-        hx_cp_async_commit();
-        page = t + 1 < count ? page_of(key + TILE_KEYS) : -1;
-        hx_cp_async_wait<0>();
-      }
-      __syncthreads();
-      if (!live) continue;
+      hx_cp_async_wait<0>();      // this tile's keys
+      __syncthreads();            // everybody's; and the queries are written
       // ---- scores of rows 4 row_y + j against keys key_x + 16 i
       float s[4][4];
 #pragma unroll
@@ -160,8 +156,8 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
         for (int i = 0; i < 4; ++i) s[j][i] = 0.0f;
       const float4* my_q = reinterpret_cast<const float4*>(q_rows) + (warp * ROWS_A_WARP + 4 * row_y) * D4;
       const float4* my_k = reinterpret_cast<const float4*>(keys) + key_x;
-#pragma unroll 2
-      for (int d4 = 0; d4 < D4; ++d4) {
+#pragma unroll 1
+      for (int d4 = 0; d4 < (live ? D4 : 0); ++d4) {
         float4 k[4], w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) k[i] = my_k[d4 * TILE_KEYS + 16 * i];
@@ -177,9 +173,16 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
             s[j][i] = fmaf(w[j].w, k[i].w, s[j][i]);
           }
       }
+      __syncthreads();      // the keys have been read
+      bring(key, page, v_cache, my_values, 4);
+      const bool more = t + 1 < count;
+      key += TILE_KEYS;
+      page = page_after;
+      if (t + 2 < count) page_after = page_of(key + TILE_KEYS);
       // ---- the running maximum and sum of every row (sixteen lanes have one)
       const bool drafted = key0 + TILE_KEYS > c.context;
       float correction[4];
+      if (live) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = warp * ROWS_A_WARP + 4 * row_y + j;
@@ -220,10 +223,12 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
           acc[i][j].w *= factor;
         }
       }
-      __syncwarp();
+      }
+      hx_cp_async_wait<0>();      // this tile's values
+      __syncthreads();
       // ---- the weighted values: coordinates 4 lane .. of 8 rows, four keys at a time
       const float4* my_p = reinterpret_cast<const float4*>(probabilities) + warp * ROWS_A_WARP * (TILE_KEYS / 4);
-      const int keys_here = min(TILE_KEYS, last_key + 1 - key0);
+      const int keys_here = live ? min(TILE_KEYS, last_key + 1 - key0) : 0;
       for (int key4 = 0; key4 * 4 < keys_here; ++key4) {
         float4 v[4][OUT_PIECES];
 #pragma unroll
@@ -249,6 +254,10 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
               acc[i][j].w = fmaf(w[k], v[k][j].w, acc[i][j].w);
             }
         }
+      }
+      if (more) {
+        __syncthreads();      // the values have been read
+        if (!bring(key, page, k_cache, my_keys, 4 * TILE_KEYS)) atomicOr(a.status, HX_FLAG_BAD_PAGE);
       }
     }
     // ---- the rows, or this CTA's part of them
@@ -592,7 +601,12 @@ __global__ __launch_bounds__(JOIN_THREADS, JOIN_CTAS) void tree_join_kernel(cons
   }
 }
 
-int tile_ctas_an_sm(int head_dim) { return head_dim <= 128 ? 2 : 1; }
+// CTAs of the tile kernel that an SM has registers and shared memory for: heads of 128 leave three.
+int tile_ctas_an_sm(int head_dim) {
+  const int most = head_dim <= 128 ? TileConfig<128>::kCtas : TileConfig<256>::kCtas;
+  const int fit = 227 * 1024 / (TileConfig<128>::floats(head_dim) * 4 + 1024);
+  return fit < most ? fit : most;
+}
 
 template <typename T, int D_MAX>
 int launch_tile(const TreeArgs& a, int ctas, cudaStream_t stream) {

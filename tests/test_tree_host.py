@@ -64,7 +64,7 @@ def test_entry_points_refuse_sizes_on_the_host():
         return library.hx_keep_rows(storage, dtype, planes, pages, kv_heads, page, dim, some, stride, some, some, some,
                                     ld_path, width, some, requests, status, None)
 
-    for changes in (dict(dtype=3), dict(planes=0), dict(planes=65536), dict(pages=0), dict(kv_heads=0), dict(page=0),
+    for changes in (dict(dtype=3), dict(planes=0), dict(planes=2 ** 30), dict(pages=0), dict(kv_heads=0), dict(page=0),
                     dict(dim=0), dict(dim=9), dict(stride=0), dict(ld_path=3), dict(width=0), dict(requests=-1),
                     dict(requests=65536), dict(status=None), dict(storage=some + 8)):
         assert keep(**changes) == -1, changes
