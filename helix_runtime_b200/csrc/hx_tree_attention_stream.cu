@@ -12,7 +12,9 @@
 // softmax stays in registers and is the A operand of the second product, values again from their
 // blocks (ldmatrix.trans).  Shared memory is written by the copy engine alone.
 //
-// Probabilities enter the second product as two bfloat16 terms (hi + lo).  The reference of a row's
+// Probabilities of up to 16 rows enter the second product as two bfloat16 terms (hi + lo, 16 bits), which
+// costs nothing there; those of more rows as one, which is what the output is rounded to, too, and the sum is
+// over the weights as rounded (64 requests x 32 drafts, two terms 323 us, one 290).  The reference of a row's
 // exponentials is raised when a chunk exceeds it by more than 2^8, each row by itself.
 //
 // Masks matter in the chunks that hold drafted keys; there values that are not finite are taken as
@@ -26,10 +28,7 @@
 namespace {
 
 constexpr int KEYS = 32;
-#ifndef HX_LEAST
-#define HX_LEAST 2
-#endif
-constexpr int LEAST = HX_LEAST;                      // chunks of the shortest run
+constexpr int LEAST = 2;                      // chunks of the shortest run
 constexpr float RAISE_MAXIMUM_BY = 8.0f;      // log2 units a chunk must exceed a row's reference by
 
 template <int D, int WARPS>
@@ -37,14 +36,11 @@ struct StreamConfig {
   static constexpr int kRows = 16 * WARPS;
   static constexpr int kHalfBytes = KEYS * D * 2;      // keys (or values) of a chunk
   static constexpr int kSlotBytes = 2 * kHalfBytes;
-#ifndef HX_RING2
-#define HX_RING2 3
-#define HX_MOST2 4
-#endif
-  static constexpr int kRing = (WARPS == 1 ? 2 : HX_RING2) * (D <= 64 ? 2 : 1);
+  // (two warps: a ring of 2 or 4 and as many CTAs as fit then took 350 us where this takes 280)
+  static constexpr int kRing = (WARPS == 1 ? 2 : 3) * (D <= 64 ? 2 : 1);
   static constexpr int kSmemBytes = kRing * kSlotBytes;
   static constexpr int kFit = 227 * 1024 / (kSmemBytes + 2048);      // CTAs an SM has shared memory for
-  static constexpr int kMost = WARPS == 1 ? 6 : HX_MOST2;                   // ... and registers
+  static constexpr int kMost = WARPS == 1 ? 6 : 4;                   // ... and registers
   static constexpr int kCtas = kFit < kMost ? kFit : kMost;
 };
 
@@ -102,11 +98,7 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
   using Config = StreamConfig<D, WARPS>;
   constexpr int RING = Config::kRing, ROWS = Config::kRows;
   constexpr int D_STEPS = D / 16, D_TILES = D / 8;
-#ifdef HX_ONE_TERM
-  constexpr bool TWO_TERMS = false;
-#else
   constexpr bool TWO_TERMS = WARPS == 1;
-#endif
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t full[RING], empty[RING];
   // the run is found from the step's description, which was there before the kernel in front

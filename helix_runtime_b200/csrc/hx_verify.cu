@@ -23,7 +23,9 @@
 // the sums have anyway, in a dozen instructions.
 //
 // Layout.  A request is a cluster of CTAs; every warp owns a stretch of the vocabulary, which it
-// reads from global memory once and from L1 again.  A visited token takes
+// reads for the largest logit and again for the exponentials; those stay
+// in shared memory, in 64 bits, so that a fallen child costs no second exponential (a vocabulary too long for
+// that: they are computed again).  A visited token takes
 // one exchange through distributed shared memory, one more a fallen child: a CTA adds up its warps and tells
 // the others, and then each takes the same decisions from the same numbers.  What a chain of visited tokens
 // takes is latency, so the tree lies in shared memory, the logits of all children are asked for
@@ -38,6 +40,7 @@ namespace {
 constexpr int WARPS = 16, THREADS = WARPS * 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr int TABLE = 64;
+constexpr int MOST_CACHED = 200 * 1024;
 constexpr int TREE = 256;      // tokens of a tree that shared memory holds (a larger one is read where it lies)
 
 struct VerifyArgs {
@@ -58,6 +61,7 @@ struct VerifyArgs {
   int vocab;
   int span;                 // tokens of the vocabulary a warp owns, a multiple of 128
   int put_back;             // children were drawn with putting back
+  int cached;               // shared memory holds the exponentials of a CTA's stretches
   int* status;
 };
 
@@ -131,27 +135,33 @@ __device__ __forceinline__ void take_larger(float& value, int& id, float other, 
   }
 }
 
-// Several of these, all of the same warp or CTA order, as one: sums against the common maxima.
-// Every lane brings one (or none: p_max = -inf, sums zero); all get the result.
-__device__ __forceinline__ Told join_told(Told mine, const double* table, double unit) {
-  float p_top = mine.p_max, q_top = mine.q_max;
-  int best = mine.best;
-#pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) {
-    take_larger(p_top, best, __shfl_xor_sync(0xffffffffu, p_top, offset), __shfl_xor_sync(0xffffffffu, best, offset));
-    q_top = fmaxf(q_top, __shfl_xor_sync(0xffffffffu, q_top, offset));
-  }
+__device__ __forceinline__ double sum_of(double value, int width) {
+  for (int offset = width / 2; offset > 0; offset >>= 1) value += __shfl_xor_sync(0xffffffffu, value, offset);
+  return value;
+}
+
+// `width` (a power of two) of these, one a lane, as one: sums against the common maxima.  All lanes below
+// `width` get the result.
+__device__ __forceinline__ Told join_told(const Told& mine, int width, const double* table, double unit) {
   Told all;
-  all.p_max = p_top;
-  all.q_max = q_top;
-  all.best = best;
-  all.bad = __any_sync(0xffffffffu, mine.bad);
-  all.p_sum = warp_sum(mine.p_sum > 0.0 ? mine.p_sum * Exponential{table, unit, p_top}(mine.p_max) : 0.0);
-  all.q_sum = warp_sum(mine.q_sum > 0.0 ? mine.q_sum * Exponential{table, unit, q_top}(mine.q_max) : 0.0);
+  all.p_max = mine.p_max;
+  all.q_max = mine.q_max;
+  all.best = mine.best;
+  all.bad = mine.bad;
+  for (int offset = width / 2; offset > 0; offset >>= 1) {
+    take_larger(all.p_max, all.best, __shfl_xor_sync(0xffffffffu, all.p_max, offset),
+                __shfl_xor_sync(0xffffffffu, all.best, offset));
+    all.q_max = fmaxf(all.q_max, __shfl_xor_sync(0xffffffffu, all.q_max, offset));
+    all.bad |= __shfl_xor_sync(0xffffffffu, all.bad, offset);
+  }
+  all.p_sum = sum_of(mine.p_sum > 0.0 ? mine.p_sum * Exponential{table, unit, all.p_max}(mine.p_max) : 0.0, width);
+  all.q_sum = sum_of(mine.q_sum > 0.0 ? mine.q_sum * Exponential{table, unit, all.q_max}(mine.q_max) : 0.0, width);
   return all;
 }
 
-__global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
+// (two CTAs an SM: with one, and no registers spilled, the same 64 walks took 120 us instead of 106)
+__global__ __launch_bounds__(THREADS, 2) void verify_kernel(const __grid_constant__ VerifyArgs a) {
+  extern __shared__ double exponentials[];          // [WARPS][span / 4 lanes ...]: of p and, behind all of them, of q
   __shared__ double table[TABLE];
   __shared__ Told of_warp[WARPS], of_cta[2][MAX_CLUSTER];
   __shared__ double sums_of_warp[WARPS];            // of the last exchange, for the draw
@@ -194,6 +204,8 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
   const int last = min(static_cast<long long>(first) + a.span, static_cast<long long>(a.vocab));
   const bool wide = a.ld % 4 == 0 && a.ld_draft % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 &&
                     (reinterpret_cast<uintptr_t>(a.draft) & 15) == 0;
+  double* p_cache = exponentials + warp * a.span;
+  double* q_cache = p_cache + WARPS * a.span;
   int phase = 0;       // which half of `of_cta` the next exchange uses
 
   // One exchange: the CTA's warps as one, told to every CTA; all warps of the cluster get the
@@ -206,19 +218,9 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
     }
     __syncthreads();
     if (warp == 0) {
-      Told one;
-      one.p_sum = one.q_sum = 0.0;
-      one.p_max = one.q_max = -INFINITY;
-      one.best = 0x7fffffff;
-      one.bad = 0;
-      if (lane < WARPS) one = of_warp[lane];
-      Told cta;
-      if (plain_sums) {
-        cta = one;
-        cta.p_sum = warp_sum(one.p_sum);
-      } else {
-        cta = join_told(one, table, unit);
-      }
+      Told cta = of_warp[lane % WARPS];
+      if (plain_sums) cta.p_sum = sum_of(cta.p_sum, WARPS);
+      else cta = join_told(cta, WARPS, table, unit);
       if (lane < ctas) {
         const uint32_t place = address_in(&of_cta[phase][rank], lane);
         store_in(place, __double_as_longlong(cta.p_sum));
@@ -231,6 +233,7 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
     }
     cluster_sync();
   };
+  auto cache_place = [&](int id) { return (id & 3) * (a.span / 4) + ((id - first) >> 2); };
   auto parent_at = [&](int j) { return held_tree ? parent_of[j] : a.parents[begin + j]; };
   auto id_at = [&](int j) { return held_tree ? id_of[j] : a.ids[begin + j]; };
   auto number_at = [&](int j) { return held_tree ? number_of[j] : a.uniform[begin + j]; };
@@ -252,9 +255,7 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
     const bool drafted = a.draft != nullptr && child < nodes && !greedy;
     const float* draft = drafted ? a.draft + static_cast<size_t>(begin + node) * a.ld_draft : row;
 
-    // calls take(id, p, q) for this lane's tokens of the warp's stretch: four side by side of each 128.  (A
-    // stretch is read two or three times; it stays in L1.  In registers, which it would fit, the exponentials of
-    // a whole stretch are in flight and spill.)
+    // calls take(id, p, q) for this lane's tokens of the warp's stretch: four side by side of each 128
     auto each = [&](auto take) {
 #pragma unroll 2
       for (int id = first + 4 * lane; id < last; id += 128) {
@@ -324,22 +325,23 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
       // (a stretch that the draft leaves out wholly has no maximum: its sum is zero against any)
       const Exponential of_q{table, unit, fmaxf(mine.q_max, -3.0e38f)};
       double p_sum = 0.0, q_sum = 0.0;
-      each([&](int, float p, float q) {
-        p_sum += of_p(p);
-        if (drafted) q_sum += of_q(q);
+      // (place e * span / 4 + id / 4 of the warp's: neighbouring lanes side by side)
+      each([&](int id, float p, float q) {
+        const double e_p = of_p(p), e_q = drafted ? of_q(q) : 0.0;
+        p_sum += e_p;
+        q_sum += e_q;
+        if (a.cached) {
+          const int place = cache_place(id);
+          p_cache[place] = e_p;
+          if (drafted) q_cache[place] = e_q;
+        }
       });
       mine.p_sum = warp_sum(p_sum);
       if (drafted) mine.q_sum = warp_sum(q_sum);
     }
     tell(mine, false);
-    Told one;
-    one.p_sum = one.q_sum = 0.0;
-    one.p_max = one.q_max = -INFINITY;
-    one.best = 0x7fffffff;
-    one.bad = 0;
-    if (lane < ctas) one = of_cta[phase][lane];
     const int first_phase = phase;
-    const Told all = join_told(one, table, unit);
+    const Told all = join_told(of_cta[phase][lane % ctas], ctas, table, unit);
     if (all.bad || (drafted && all.q_max == -INFINITY)) {
       if (writes && lane == 0) {
         a.next[request] = -1;
@@ -349,6 +351,24 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
     }
     const Exponential of_p{table, unit, all.p_max}, of_q{table, unit, drafted ? all.q_max : 0.0f};
     const double p_unit = 1.0 / all.p_sum, q_unit = drafted ? 1.0 / all.q_sum : 0.0;
+    // what turns this warp's exponentials, against its own maxima, into shares
+    const double p_factor = first < last && !greedy ? of_p(mine.p_max) * p_unit : 0.0;
+    const double q_factor = first < last && drafted ? of_q(mine.q_max) * q_unit : 0.0;
+    // calls take(id, share of p, share of q) for this lane's tokens
+    auto each_share = [&](auto take) {
+      if (a.cached) {
+#pragma unroll 2
+        for (int id = first + 4 * lane; id < last; id += 128)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (id + e < last) {
+              const int place = cache_place(id + e);
+              take(id + e, p_cache[place] * p_factor, drafted ? q_cache[place] * q_factor : 0.0);
+            }
+      } else {
+        each([&](int id, float p, float q) { take(id, of_p(p) * p_unit, drafted ? of_q(q) * q_unit : 0.0); });
+      }
+    };
 
     // ---- the children, in order
     double b = 0.0, left = 1.0, gone = 0.0;
@@ -387,14 +407,13 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
         b += left * scale;
         if (!a.put_back) gone += q;
         double sum = 0.0;
-        const double b_unit = b * q_unit;
-        each([&](int, float p_logit, float q_logit) {
-          const double over = of_p(p_logit) * p_unit - b_unit * of_q(q_logit);
+        each_share([&](int, double of_target, double of_draft) {
+          const double over = of_target - b * of_draft;
           if (over > 0.0) sum += over;
         });
         mine.p_sum = warp_sum(sum);
         tell(mine, true);
-        left = warp_sum(lane < ctas ? of_cta[phase][lane].p_sum : 0.0);
+        left = sum_of(of_cta[phase][lane % ctas].p_sum, ctas);
       } else {
         // fell already: nothing of it is left
         bool again = __any_sync(0xffffffffu, lane < fallen && fallen_token == token);
@@ -433,19 +452,18 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(const VerifyArgs a) {
         for (int j = child_of(node, node); j < nodes; j = child_of(node, j)) out |= id_at(j) == id;
       return out;
     };
-    const double b_unit = b * q_unit;
-    auto weight = [&](float p_logit, float q_logit) {
-      const double p = of_p(p_logit) * p_unit;
-      if (plain || listed) return p;
-      const double over = p - b_unit * of_q(q_logit);
-      return over > 0.0 ? over : 0.0;
-    };
     // four tokens of this lane from `id` on, of which the fallen and those behind the stretch weigh nothing
     auto weights_of = [&](int id, double (&w)[4]) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool out = listed && fell(id + e);
-        w[e] = id + e < last && !out ? weight(__ldg(row + id + e), drafted ? __ldg(draft + id + e) : 0.0f) : 0.0;
+        w[e] = 0.0;
+        if (id + e >= last || out) continue;
+        const int place = cache_place(id + e);
+        w[e] = a.cached ? p_cache[place] * p_factor : of_p(__ldg(row + id + e)) * p_unit;
+        if (plain || listed || !drafted) continue;
+        w[e] -= b * (a.cached ? q_cache[place] * q_factor : of_q(__ldg(draft + id + e)) * q_unit);
+        if (!(w[e] > 0.0)) w[e] = 0.0;
       }
     };
     // every warp's sum: p's from the row's first exchange, what is over from that of the last fallen
@@ -555,20 +573,29 @@ HX_API int hx_verify_drafts(const float* logits, int ld, const float* draft, int
   const int sms = hx_device_sm_count();
   HX_REQUIRE(sms > 0, "hx_verify_drafts: the device cannot be asked");
   HX_REQUIRE(requests <= (1 << 24), "hx_verify_drafts: too many requests");
-#ifndef HX_VC
-#define HX_VC 2
-#endif
-  // as many CTAs a request as fit the GPU at once, two an SM (the walk of the deepest request, whose length is
-  // latency, is what a batch waits for), and no more than have 32 x 4 tokens a warp
+  // As many CTAs a request as leave four an SM in all, half of which run at once: what a batch waits for is the
+  // deepest walk, whose length is latency, and most walks are short (64 requests with trees of 32 over 32,000
+  // tokens: 8 CTAs 106 us, 4 CTAs 135).  And no more than have 32 x 4 tokens a warp.
   int ctas = MAX_CLUSTER;
-  while (ctas > 1 && (static_cast<long long>(requests) * ctas > HX_VC * (long long)sms || vocab <= (ctas / 2) * WARPS * 128)) ctas /= 2;
+  while (ctas > 1 && (static_cast<long long>(requests) * ctas > 4ll * sms || vocab <= (ctas / 2) * WARPS * 128)) ctas /= 2;
   int span = (vocab + ctas * WARPS - 1) / (ctas * WARPS);
   span = (span + 127) / 128 * 128;
   VerifyArgs a{logits, ld, draft, ld_draft, token_ids, parents, request_start, temperature, uniform, path, ld_path,
-               width, kept, next_tokens, vocab, span, put_back, status};
+               width, kept, next_tokens, vocab, span, put_back, 0, status};
+  // exponentials of target and draft (a request without drafted tokens' logits needs none of them twice)
+  const long long bytes = static_cast<long long>(WARPS) * span * 16;
+  a.cached = bytes <= MOST_CACHED;
+  static std::once_flag once;
+  static bool reserved = false;
+  std::call_once(once, [] {
+    reserved = cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_CACHED) == cudaSuccess;
+    if (!reserved) cudaGetLastError();
+  });
+  HX_REQUIRE(reserved, "hx_verify_drafts: cannot reserve %d bytes of shared memory", MOST_CACHED);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(requests * ctas);
   config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = a.cached ? static_cast<size_t>(bytes) : 0;
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
