@@ -499,6 +499,36 @@ class CacheManager:
         return self._admit_with(request, tokens, self._shared_pages(parent, tokens),
                                 self._state_at(parent, tokens))
 
+    def branch(self, source: Hashable, request: Hashable, tokens: int) -> int:
+        """Admit ``request`` with the first ``tokens`` positions of ``source``, any number of them:
+        whole pages are shared as :meth:`fork` shares them, and of a last page that is only partly
+        theirs it gets a copy (queued on the current stream).  Raises :class:`OutOfPages`, and
+        changes nothing, when a group has no page left for the copy."""
+        parent = self._requests[source]
+        if not 0 < tokens <= parent.length:
+            raise ValueError(f"a branch holds at least one token and no more than the "
+                             f"{parent.length} its source has published")
+        shared, state = self._shared_pages(parent, tokens), self._state_at(parent, tokens)
+        place, partly = divmod(tokens, self.page_size)
+        if partly and any(not group.pool.free_pages for group in self.groups):
+            raise OutOfPages("no page is free for the copy of a partly filled one")
+        slot = self._admit_with(request, tokens, shared, state)
+        if partly:
+            self.extend(request, tokens)
+            for group, old, new in zip(self.groups, parent.tables, self._requests[request].tables):
+                self._copy_page(group, old[place], new[place])
+        return slot
+
+    @staticmethod
+    def _copy_page(group: CacheGroup, source: int, target: int) -> None:
+        if group.storage.is_cuda:
+            from ..ops import library as ops
+            # two pages of the pool, held by different requests: nothing here to be flagged
+            words = torch.tensor([source, target, 0], dtype=torch.int32, device=group.storage.device)
+            ops.copy_pages(group.storage, words[:1], words[1:2], words[2:])
+        else:
+            group.storage[:, :, target] = group.storage[:, :, source]
+
     # ------------------------------------------------------------------ anchors
     #
     # An anchor keeps the whole pages of a prefix alive after the request that computed them

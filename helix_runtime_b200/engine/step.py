@@ -21,7 +21,7 @@ import torch
 from ..cache.manager import CacheManager
 from ..models.decoder import DecoderModel
 from ..ops import library as ops
-from ..parts.base import StepContext, Workspace
+from ..parts.base import DraftedTrees, StepContext, Workspace
 
 
 def ancestor_words(parents: Sequence[int], words: int = 0) -> np.ndarray:
@@ -50,6 +50,11 @@ class StepEntry:
     request: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = ()          # places among ``tokens`` whose logits are asked for
+    # Drafted tokens: ``tokens`` are a tree, token 0 its root and the rest drafts of what follows
+    # their parents (each one's number among ``tokens``, smaller than its own; -1 for token 0).
+    # A token sees the cached ones and its ancestors, and its position is its depth behind them.
+    # Nothing of a tree is published before :meth:`StepFunction.keep` says what stays.
+    parents: Optional[Sequence[int]] = None
 
 
 class StepError(RuntimeError):
@@ -86,6 +91,10 @@ class StepFunction:
         self._device = torch.zeros(cursor, dtype=torch.int32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._uploaded = torch.cuda.Event() if pin else None
+        self._tree_host: Optional[torch.Tensor] = None      # made at the first step of trees
+        self._tree_device: Optional[torch.Tensor] = None
+        # a step of trees whose requests wait for `keep`
+        self._trees: Optional[Tuple[List[StepEntry], StepContext]] = None
         self.last_context: Optional[StepContext] = None
         self.steps_run = 0
         self.tokens_run = 0
@@ -122,6 +131,10 @@ class StepFunction:
         total = sum(len(entry.tokens) for entry in entries)
         if feed_rows is not None and (len(feed_rows) != len(entries) or total != len(entries)):
             raise StepError("a step fed on the device has one token and one row per request")
+        if self._trees is not None and any(self._open_trees()):
+            raise StepError("the last step's drafted trees wait for what is kept of them")
+        masks = self._tree_masks(entries, feed_rows) \
+            if any(entry.parents is not None for entry in entries) else None
         if total > self.max_tokens:
             raise StepError(f"{total} tokens in one step, at most {self.max_tokens}")
         seen = set()
@@ -172,7 +185,10 @@ class StepFunction:
                 self.cache.extend(entry.request, before + count)
                 reserved.append((entry.request, before))
                 token_ids[cursor:cursor + count] = np.asarray(entry.tokens, dtype=np.int32)
-                positions[cursor:cursor + count] = np.arange(before, before + count, dtype=np.int32)
+                if masks is None:
+                    positions[cursor:cursor + count] = np.arange(before, before + count, dtype=np.int32)
+                else:
+                    self._fill_tree(entry, before, cursor, positions, masks[index])
                 token_request[cursor:cursor + count] = index
                 request_slot[index] = self.cache.slot(entry.request)
                 request_start[index] = cursor
@@ -194,6 +210,7 @@ class StepFunction:
             raise
 
         self._device.copy_(self._host, non_blocking=True)
+        trees = None if masks is None else self._upload_trees(cursor, masks)
         if self._uploaded is not None:
             self._uploaded.record()
         self.cache.sync_tables()
@@ -211,9 +228,94 @@ class StepFunction:
             host_request_slots=[int(v) for v in request_slot[:len(entries)]],
             host_request_starts=[int(v) for v in request_start[:len(entries) + 1]],
             host_request_contexts=[int(v) for v in request_context[:len(entries)]],
-            host_query_lengths=[len(entry.tokens) for entry in entries],
+            host_query_lengths=[len(entry.tokens) for entry in entries], trees=trees,
         )
         return ctx, self._view("want_rows", True), n_want, new_lengths
+
+    # ----------------------------------------------------------- drafted trees
+
+    def _tree_masks(self, entries: Sequence[StepEntry], feed_rows) -> List[np.ndarray]:
+        """The entries' masks, all as wide as the largest tree's."""
+        if feed_rows is not None or any(entry.parents is None for entry in entries):
+            raise StepError("a step brings drafted trees for all of its requests or for none")
+        if not self.model.takes_trees:
+            raise StepError("the model has a part that takes no drafted trees")
+        words = max(1, -(-max(len(entry.tokens) for entry in entries) // 64))
+        masks = []
+        for entry in entries:
+            if len(entry.parents) != len(entry.tokens):
+                raise StepError(f"request {entry.request!r} brings {len(entry.tokens)} tokens and "
+                                f"{len(entry.parents)} parents")
+            try:
+                masks.append(ancestor_words(entry.parents, words))
+            except ValueError as error:
+                raise StepError(f"request {entry.request!r}: {error}") from None
+        size = self.max_tokens * (1 + words)
+        if self._tree_host is None or self._tree_host.numel() < size:
+            # places and parents (two int32 an element), then the masks
+            self._tree_host = torch.zeros(size, dtype=torch.int64, pin_memory=self._uploaded is not None)
+            self._tree_device = torch.zeros(size, dtype=torch.int64, device=self.device)
+        return masks
+
+    def _fill_tree(self, entry: StepEntry, before: int, cursor: int, positions: np.ndarray,
+                   mask: np.ndarray) -> None:
+        count, words = mask.shape
+        depth = np.zeros(count, dtype=np.int32)
+        for token in range(1, count):
+            depth[token] = depth[entry.parents[token]] + 1
+        positions[cursor:cursor + count] = before + depth
+        block, cap = self._tree_host.numpy(), self.max_tokens
+        places, parents = block[:cap].view(np.int32).reshape(2, cap)
+        places[cursor:cursor + count] = np.arange(before, before + count, dtype=np.int32)
+        parents[cursor:cursor + count] = np.asarray(entry.parents, dtype=np.int32)
+        block[cap + cursor * words:cap + (cursor + count) * words] = mask.reshape(-1)
+
+    def _upload_trees(self, tokens: int, masks: List[np.ndarray]) -> DraftedTrees:
+        cap, words = self.max_tokens, masks[0].shape[1]
+        used = cap + tokens * words
+        self._tree_device[:used].copy_(self._tree_host[:used], non_blocking=True)
+        places, parents = self._tree_device[:cap].view(torch.int32).view(2, cap)
+        return DraftedTrees(self._tree_device[cap:used].view(tokens, words), places, parents)
+
+    def _open_trees(self) -> List[bool]:
+        """Which requests of the last step of trees are there with tokens not yet published (one
+        that has ended, or whose step failed, has none)."""
+        return [self.cache.has(entry.request)
+                and self.cache.reserved(entry.request) > self.cache.length(entry.request)
+                for entry in self._trees[0]]
+
+    def keep(self, path: torch.Tensor, kept: torch.Tensor) -> List[int]:
+        """Settle the last step's drafted trees: of request ``r`` (in the order of the entries) the
+        ``kept[r]`` tokens ``path[r]`` stay, a branch from the root down, as
+        :meth:`helix_runtime_b200.sampling.sampler.Sampler.verify` names them.  Their keys and
+        values move together, the request's length is published and the other tokens' pages are
+        given back.  Returns the tokens kept of each (waits for the device)."""
+        if self._trees is None:
+            raise StepError("the last step brought no drafted trees")
+        entries, ctx = self._trees
+        live = self._open_trees()
+        if not all(live):
+            # what a request that has ended held may be another's by now
+            kept = kept[:len(entries)] * torch.tensor(live, dtype=kept.dtype, device=kept.device)
+        counts = kept[:len(entries)].tolist()
+        for entry, count in zip(entries, counts):
+            if not 0 <= count <= len(entry.tokens):
+                raise StepError(f"{count} tokens kept of the {len(entry.tokens)} of request "
+                                f"{entry.request!r}")
+        for group in self.cache.groups:
+            ops.keep_rows(group.storage, group.device_tables, ctx.request_slot, ctx.request_context,
+                          path, kept, len(entries), self.status)
+        self._trees = None
+        try:
+            self.raise_on_status()
+        except Exception:
+            self.fail(entries)
+            raise
+        for entry, count, there in zip(entries, counts, live):
+            if there:
+                self.cache.commit(entry.request, self.cache.length(entry.request) + count)
+                self.cache.rollback(entry.request)
+        return counts
 
     def run(self, entries: Sequence[StepEntry], check_status: bool = True) -> Optional[torch.Tensor]:
         """Run one step.  Returns float32 logits ``[wanted, vocab]`` in the order of the entries
@@ -231,10 +333,13 @@ class StepFunction:
 
     def finish(self, entries: Sequence[StepEntry], new_lengths: Sequence[int],
                ctx: StepContext) -> None:
-        """The step succeeded: publish the new lengths."""
-        for entry, length in zip(entries, new_lengths):
-            if self.cache.has(entry.request):    # a request may have ended while in flight
-                self.cache.commit(entry.request, length)
+        """The step succeeded: publish the new lengths (drafted trees wait for :meth:`keep`)."""
+        if ctx.trees is not None:
+            self._trees = (list(entries), ctx)
+        else:
+            for entry, length in zip(entries, new_lengths):
+                if self.cache.has(entry.request):    # a request may have ended while in flight
+                    self.cache.commit(entry.request, length)
         self.last_context = ctx
         self.steps_run += 1
         self.tokens_run += ctx.n_tokens

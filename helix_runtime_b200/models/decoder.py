@@ -6,6 +6,7 @@ schedule entry and returns float32 logits at the wanted rows.
 """
 from __future__ import annotations
 
+import functools
 from typing import Callable, Dict, List, Mapping, Optional, Sequence
 
 import torch
@@ -209,6 +210,13 @@ class DecoderModel:
     def graph_safe(self) -> bool:
         """Whether every part may be recorded into a CUDA graph (see ``Part.graph_safe``)."""
         return all(part.graph_safe for part in self.all_parts())
+
+    @functools.cached_property
+    def takes_trees(self) -> bool:
+        """Whether steps may bring drafted trees: every mixer takes them, and nothing is kept of
+        a request but keys and values."""
+        return all(self.blocks[entry.block].mixer.takes_trees for entry in self.schedule) \
+            and not self.cache_needs()[1]
 
     def tensor_requests(self) -> List[TensorRequest]:
         requests: List[TensorRequest] = []

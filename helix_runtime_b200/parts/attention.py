@@ -411,6 +411,29 @@ class PagedAttention(Mixer):
                                 slopes=self.slopes, chunk=chunk, softcap=self.softcap,
                                 group_heads=group_floats > 0)
 
+    @property
+    def takes_trees(self) -> bool:
+        """Steps of drafted trees: plain softmax attention over all earlier keys, with an encoding
+        that keeps a token's position and its place apart."""
+        cls = type(self)
+        return (cls.forward is PagedAttention.forward and cls.attend is PagedAttention.attend
+                and self.window is None and self.chunk is None and self.conv_taps == 1
+                and not self.shared_values and not self.has_sinks and self.sink_score is None
+                and self.slope_values is None and not self.softcap and self.position.takes_places)
+
+    def attend_trees(self, ctx: StepContext, cache: LayerCache, qkv: torch.Tensor,
+                     context: torch.Tensor) -> None:
+        """:meth:`attend` for drafted tokens, each of which sees the cached ones and its own
+        ancestors among the others."""
+        floats = ops.tree_attention_scratch(ctx.dtype, self.heads, self.kv_heads, self.row_dim,
+                                            cache.page_size)
+        n = ctx.n_tokens
+        ops.tree_attention(qkv[:n], cache.keys, cache.values, ctx.trees.visible, ctx.request_start,
+                           ctx.request_context, ctx.request_slot, cache.block_tables, context[:n],
+                           ctx.workspace.at_least("attention.trees", floats, torch.float32),
+                           ctx.n_requests, self.heads, self.kv_heads, self.row_dim, cache.page_size,
+                           cache.num_pages, self.scale, ctx.status, max_nodes=ctx.max_query_len)
+
     def forward(self, ctx: StepContext, cache: LayerCache, x: torch.Tensor,
                 residual: torch.Tensor) -> None:
         n = ctx.n_tokens
@@ -423,6 +446,10 @@ class PagedAttention(Mixer):
         uncleared = gate_rows = None
         if self.conv_taps > 1:
             uncleared, gate_rows = self.project_filtered(ctx, cache, x, qkv)
+        elif ctx.trees is not None:
+            project(x, self.w_qkv, qkv, n, ops.EPI_STORE, ctx.status, ctx.ordered_sums,
+                    workspace=ctx.workspace)
+            self.position.apply_at(ctx, cache, qkv, self.heads, self.kv_heads, ctx.trees.places)
         elif is_weight_stream(x, self.w_qkv, n):
             # few tokens: split-K into a float32 accumulator that the rotary kernel reads,
             # rounds as the product's store would have, and clears
@@ -437,7 +464,10 @@ class PagedAttention(Mixer):
                     workspace=ctx.workspace)
             self.position.apply(ctx, cache, qkv, self.heads, self.kv_heads)
 
-        self.attend(ctx, cache, qkv, context)
+        if ctx.trees is not None:
+            self.attend_trees(ctx, cache, qkv, context)
+        else:
+            self.attend(ctx, cache, qkv, context)
         restore = getattr(self.position, "restore_values", None)
         if restore is not None:
             restore(ctx, context, self.heads)

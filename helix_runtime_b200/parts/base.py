@@ -114,6 +114,15 @@ class LayerCache:
 
 
 @dataclasses.dataclass
+class DraftedTrees:
+    """What a step of drafted tokens has on top: every request brings a tree (see
+    :class:`helix_runtime_b200.engine.step.StepEntry`)."""
+    visible: torch.Tensor       # [tokens, words] int64: which drafted tokens each one sees
+    places: torch.Tensor        # [capacity] int32 where a token's keys and values are kept
+    parents: torch.Tensor       # [capacity] int32 a token's parent among its request's, -1: none
+
+
+@dataclasses.dataclass
 class StepContext:
     """One step's batch as the parts see it.  N tokens of R requests, flattened."""
     dtype: torch.dtype
@@ -139,6 +148,9 @@ class StepContext:
     host_request_starts: Optional[List[int]] = None
     host_request_contexts: Optional[List[int]] = None
     host_query_lengths: Optional[List[int]] = None      # tokens each request brings
+    # a step of drafted trees: a token's position is its depth behind the cached ones, its place
+    # in the pages its number
+    trees: Optional[DraftedTrees] = None
 
 
 class Part:
@@ -184,6 +196,15 @@ class PositionEncoding(Part):
         instead of ``qkv`` and the accumulator must be left cleared."""
         raise NotImplementedError
 
+    # Whether :meth:`apply_at` is there.
+    takes_places: bool = False
+
+    def apply_at(self, ctx: "StepContext", cache: "LayerCache", qkv: torch.Tensor, heads: int,
+                 kv_heads: int, places: torch.Tensor) -> None:
+        """:meth:`apply` for tokens whose keys and values are kept at ``places`` (device int32)
+        and not at the positions they are encoded by."""
+        raise NotImplementedError
+
     def project_and_apply(self, ctx: "StepContext", cache: "LayerCache", x: torch.Tensor,
                           weight, qkv: torch.Tensor, heads: int, kv_heads: int) -> bool:
         """Optional: the mixer's projection ``qkv[:n] = x[:n] @ weight.T`` and :meth:`apply`
@@ -197,6 +218,8 @@ class Mixer(Part):
     # An entry with ``cache_from`` reads the other entry's keys and values, and its state too
     # unless the mixer keeps its own.
     keeps_own_state: bool = False
+    # Whether ``forward`` takes a step of drafted trees (``ctx.trees``).
+    takes_trees: bool = False
 
     def kv_need(self) -> Optional[KvNeed]:
         return None

@@ -77,6 +77,16 @@ class RotaryTable:
 PAIRINGS = {"adjacent": 0, "half_split": 1}
 
 
+def append_rows(ctx: StepContext, cache: LayerCache, qkv: torch.Tensor, heads: int, kv_heads: int,
+                row_dim: int, places: torch.Tensor, angles: torch.Tensor) -> None:
+    """Store the keys and values of ``qkv[:n_tokens]`` as they are at ``places`` of the entry's
+    pages, when it owns them (``angles``: any table, nothing is turned)."""
+    if cache.owns and cache.keys is not None:
+        ops.rope_append(qkv, places, ctx.token_request, ctx.request_slot, cache.block_tables,
+                        cache.keys, cache.values, angles, angles, ctx.n_tokens, heads, kv_heads,
+                        row_dim, 0, 0, cache.page_size, cache.num_pages, ctx.status)
+
+
 class RotaryEncoding(PositionEncoding):
     def __init__(self, spec: PartSpec, hidden_size: int) -> None:
         super().__init__(spec, hidden_size)
@@ -126,6 +136,22 @@ class RotaryEncoding(PositionEncoding):
                         cache.page_size, cache.num_pages, ctx.status, accum=accum,
                         shared_values=self.shared_values)
 
+    @property
+    def takes_places(self) -> bool:
+        return not self.shared_values
+
+    def apply_at(self, ctx: StepContext, cache: LayerCache, qkv: torch.Tensor, heads: int,
+                 kv_heads: int, places: torch.Tensor) -> None:
+        if self.rotary_dim:
+            # queries and keys alike are turned where they lie: for this pass the keys are
+            # queries, and the values stand where keys that nobody stores would
+            ops.rope_append(qkv, ctx.positions, ctx.token_request, ctx.request_slot,
+                            cache.block_tables, None, None, self.cos, self.sin, ctx.n_tokens,
+                            heads + kv_heads, kv_heads, self.row_dim, self.rotary_dim,
+                            PAIRINGS[self.pairing], cache.page_size, cache.num_pages, ctx.status,
+                            shared_values=True)
+        append_rows(ctx, cache, qkv, heads, kv_heads, self.row_dim, places, self.cos)
+
     def project_and_apply(self, ctx: StepContext, cache: LayerCache, x: torch.Tensor,
                           weight: Weight, qkv: torch.Tensor, heads: int, kv_heads: int) -> bool:
         """Prompt portions in bfloat16: rotation and cache append are the epilogue of the
@@ -154,6 +180,7 @@ class NoPosition(PositionEncoding):
     is the plain cache append.  Parameters: ``head_dim``, ``row_dim`` (default ``head_dim``)."""
 
     pairing = None
+    takes_places = True
 
     def __init__(self, spec: PartSpec, hidden_size: int) -> None:
         super().__init__(spec, hidden_size)
@@ -175,6 +202,10 @@ class NoPosition(PositionEncoding):
                         cache.values if write else None, self._no_angles, self._no_angles,
                         ctx.n_tokens, heads, kv_heads, self.row_dim, 0, 0, cache.page_size,
                         cache.num_pages, ctx.status, accum=accum)
+
+    def apply_at(self, ctx: StepContext, cache: LayerCache, qkv: torch.Tensor, heads: int,
+                 kv_heads: int, places: torch.Tensor) -> None:
+        append_rows(ctx, cache, qkv, heads, kv_heads, self.row_dim, places, self._no_angles)
 
 
 class ComputedRotary(PositionEncoding):

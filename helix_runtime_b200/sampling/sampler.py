@@ -10,12 +10,13 @@ on what else is in the batch or on how the work was cut into steps.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
 from ..ops import library as ops
+from ..parts.base import StepContext
 
 _MASK = (1 << 64) - 1
 
@@ -84,6 +85,34 @@ class Sampler:
     def sample(self, logits: torch.Tensor, temperatures: Sequence[float],
                uniforms: Sequence[float], status: Optional[torch.Tensor]) -> torch.Tensor:
         return self.launch(logits, self.prepare(temperatures, uniforms), status)
+
+    def verify(self, ctx: StepContext, logits: torch.Tensor, temperatures: Sequence[float],
+               uniforms: Sequence[float], draft_logits: Optional[torch.Tensor] = None,
+               replacement: bool = False) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Which tokens of a step of drafted trees stand, and what follows them: the device tensors
+        ``(path, kept, next tokens)`` of :func:`helix_runtime_b200.ops.library.verify_drafts`, with
+        a row a request.  ``logits``: a row for every token of the step, in its order;
+        ``temperatures``: one a request; ``uniforms``: one a token."""
+        requests, tokens = ctx.n_requests, ctx.n_tokens
+        if ctx.trees is None or logits.shape[0] != tokens:
+            raise ValueError("verification takes the logits of all tokens of a step of drafted trees")
+        if len(temperatures) != requests or len(uniforms) != tokens or tokens > self.max_rows:
+            raise ValueError(f"{len(temperatures)} temperatures and {len(uniforms)} uniform numbers for "
+                             f"{requests} requests of {tokens} tokens, at most {self.max_rows}")
+        if self._params_uploaded is not None:
+            self._params_uploaded.synchronize()
+        params = self._host_params.numpy()
+        params[0, :requests] = np.asarray(temperatures, dtype=np.float32)
+        params[1, :tokens] = np.asarray(uniforms, dtype=np.float32)
+        self._device_params.copy_(self._host_params, non_blocking=True)
+        if self._params_uploaded is not None:
+            self._params_uploaded.record()
+        path = torch.empty((requests, ctx.max_query_len), dtype=torch.int32, device=self.device)
+        kept, following = torch.empty((2, requests), dtype=torch.int32, device=self.device)
+        ops.verify_drafts(logits, draft_logits, ctx.token_ids, ctx.trees.parents, ctx.request_start,
+                          self._device_params[0], self._device_params[1], path, kept, following,
+                          requests, ctx.status, replacement=replacement)
+        return path, kept, following
 
     def to_host(self, tokens: torch.Tensor) -> List[int]:
         rows = tokens.shape[0]
