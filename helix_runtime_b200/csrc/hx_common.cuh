@@ -8,6 +8,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 
@@ -38,6 +39,23 @@ void hx_set_error(const char* format, ...);
 void hx_count_launches(int kernels);
 // Streaming multiprocessors of the current device (0 and a message when it cannot be asked).
 int hx_device_sm_count();
+
+// What a kernel needs before its first launch on a device (its shared memory, above all): `prepare` runs
+// until it has gone well once on the current device, whatever others have been used.  False: it has not.
+template <typename Prepare>
+bool hx_once_a_device(std::atomic<unsigned long long>& ready, Prepare prepare) {
+  int device = 0;
+  if (cudaGetDevice(&device) == cudaSuccess && device >= 0 && device < 64) {
+    const unsigned long long bit = 1ull << device;
+    if ((ready.load(std::memory_order_acquire) & bit) != 0) return true;
+    if (prepare()) {
+      ready.fetch_or(bit, std::memory_order_release);
+      return true;
+    }
+  }
+  cudaGetLastError();
+  return false;
+}
 
 #define HX_REQUIRE(cond, ...)            \
   do {                                   \

@@ -20,8 +20,6 @@
 #include "hx_mma.cuh"
 #include "hx_tree_attention.cuh"
 
-#include <mutex>
-
 namespace {
 
 // ------------------------------------------------------------------ 32 rows x 64 keys
@@ -611,14 +609,12 @@ int tile_ctas_an_sm(int head_dim) {
 template <typename T, int D_MAX>
 int launch_tile(const TreeArgs& a, int ctas, cudaStream_t stream) {
   const int bytes = TileConfig<D_MAX>::floats(a.head_dim) * 4;
-  static std::once_flag once;
-  static bool reserved = false;
-  std::call_once(once, [] {
-    reserved = cudaFuncSetAttribute(tree_tile_kernel<T, D_MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    TileConfig<D_MAX>::floats(D_MAX) * 4) == cudaSuccess &&
-               cudaFuncSetAttribute(tree_tile_kernel<T, D_MAX>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                    cudaSharedmemCarveoutMaxShared) == cudaSuccess;
-    if (!reserved) cudaGetLastError();
+  static std::atomic<unsigned long long> ready{0};
+  const bool reserved = hx_once_a_device(ready, [] {
+    return cudaFuncSetAttribute(tree_tile_kernel<T, D_MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                TileConfig<D_MAX>::floats(D_MAX) * 4) == cudaSuccess &&
+           cudaFuncSetAttribute(tree_tile_kernel<T, D_MAX>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                cudaSharedmemCarveoutMaxShared) == cudaSuccess;
   });
   HX_REQUIRE(reserved, "hx_tree_attention: cannot reserve shared memory");
   hx_launch(tree_tile_kernel<T, D_MAX>, ctas, TILE_WARPS * 32, bytes, stream, a);
@@ -695,7 +691,7 @@ HX_API int hx_tree_attention(const void* q, int ldq, const void* k_cache, const 
   HX_REQUIRE(words > 0 && ld_visible >= words, "hx_tree_attention: a token has at least one word of 64 bits");
   HX_REQUIRE(num_pages > 0 && table_stride > 0 && static_cast<long long>(num_pages) * kv_heads < (1ll << 31),
              "hx_tree_attention: bad cache geometry");
-  HX_REQUIRE(scale > 0.0f, "hx_tree_attention: the scale must be positive");
+  HX_REQUIRE(scale > 0.0f && scale <= 3.0e38f, "hx_tree_attention: the scale must be positive and finite");
   HX_REQUIRE(status != nullptr && partial != nullptr, "hx_tree_attention: status word or scratch missing");
   const int size = dtype == HX_BF16 ? 2 : 4;
   const int piece = hx_cache_chunk(size, head_dim) * size;      // bytes the cache is read in

@@ -23,8 +23,6 @@
 #include "hx_mma.cuh"
 #include "hx_tree_attention.cuh"
 
-#include <mutex>
-
 namespace {
 
 constexpr int KEYS = 32;
@@ -451,15 +449,13 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
 template <int D, int WARPS>
 int launch(const TreeArgs& a, cudaStream_t stream) {
   using Config = StreamConfig<D, WARPS>;
-  static std::once_flag once;
-  static bool reserved = false;
-  std::call_once(once, [] {
-    reserved = cudaFuncSetAttribute(tree_stream_kernel<D, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    Config::kSmemBytes) == cudaSuccess &&
-               // (else the driver keeps more of it for L1 than leaves room for kCtas)
-               cudaFuncSetAttribute(tree_stream_kernel<D, WARPS>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                    cudaSharedmemCarveoutMaxShared) == cudaSuccess;
-    if (!reserved) cudaGetLastError();
+  static std::atomic<unsigned long long> ready{0};
+  const bool reserved = hx_once_a_device(ready, [] {
+    return cudaFuncSetAttribute(tree_stream_kernel<D, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                Config::kSmemBytes) == cudaSuccess &&
+           // (else the driver keeps more of it for L1 than leaves room for kCtas)
+           cudaFuncSetAttribute(tree_stream_kernel<D, WARPS>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                cudaSharedmemCarveoutMaxShared) == cudaSuccess;
   });
   HX_REQUIRE(reserved, "hx_tree_attention: cannot reserve %d bytes of shared memory", Config::kSmemBytes);
   const int ctas = hx_device_sm_count() * Config::kCtas;

@@ -39,8 +39,6 @@
 #include "hx_tcgen05.cuh"
 #include "hx_tree_attention.cuh"
 
-#include <mutex>
-
 namespace {
 
 constexpr int BLOCK_M = 128, BLOCK_N = 64;
@@ -150,7 +148,6 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   using Config = TreeTcConfig<D>;
   constexpr int K_STAGES = Config::kKeyStages, V_STAGES = Config::kValueStages;
   constexpr int PIECES = D / 8;
-  hx_pdl_trigger();
 
   // the run is found from the step's description, which was there before the kernel in front
   const TreeRun run = tree_run<BLOCK_N>(a, blockIdx.x, gridDim.x, LEAST);
@@ -213,7 +210,12 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == WARP_SCORES) tmem_alloc(tmem_holder, Config::kTmemColumns);
+  if (warp == WARP_SCORES) {
+    tmem_alloc(tmem_holder, Config::kTmemColumns);
+    // Only now may the kernel behind come in: it could else take the tensor memory that this one still
+    // waits for, and hold it until this one is done.
+    hx_pdl_trigger();
+  }
   hx_pdl_wait();
   if (threadIdx.x == 0) tree_tell_none<BLOCK_M>(a);
   tc_fence_before();
@@ -680,14 +682,12 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
 template <int D>
 int launch(const TreeArgs& a, int ctas, cudaStream_t stream) {
   using Config = TreeTcConfig<D>;
-  static std::once_flag once;
-  static bool reserved = false;
-  std::call_once(once, [] {
-    reserved = cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    Config::kSmemBytes) == cudaSuccess &&
-               cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                    cudaSharedmemCarveoutMaxShared) == cudaSuccess;
-    if (!reserved) cudaGetLastError();
+  static std::atomic<unsigned long long> ready{0};
+  const bool reserved = hx_once_a_device(ready, [] {
+    return cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                Config::kSmemBytes) == cudaSuccess &&
+           cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                cudaSharedmemCarveoutMaxShared) == cudaSuccess;
   });
   HX_REQUIRE(reserved, "hx_tree_attention: cannot reserve %d bytes of shared memory", Config::kSmemBytes);
   hx_launch(tree_attention_tc_kernel<D>, ctas, THREADS, Config::kSmemBytes, stream, a);

@@ -33,7 +33,7 @@
 // meanwhile.  Only rows of tokens that are walked over are read.
 #include "hx_common.cuh"
 
-#include <mutex>
+#include <atomic>
 
 namespace {
 
@@ -585,11 +585,9 @@ HX_API int hx_verify_drafts(const float* logits, int ld, const float* draft, int
   // exponentials of target and draft (a request without drafted tokens' logits needs none of them twice)
   const long long bytes = static_cast<long long>(WARPS) * span * 16;
   a.cached = bytes <= MOST_CACHED;
-  static std::once_flag once;
-  static bool reserved = false;
-  std::call_once(once, [] {
-    reserved = cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_CACHED) == cudaSuccess;
-    if (!reserved) cudaGetLastError();
+  static std::atomic<unsigned long long> ready{0};
+  const bool reserved = hx_once_a_device(ready, [] {
+    return cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_CACHED) == cudaSuccess;
   });
   HX_REQUIRE(reserved, "hx_verify_drafts: cannot reserve %d bytes of shared memory", MOST_CACHED);
   cudaLaunchConfig_t config = {};
