@@ -1034,11 +1034,20 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 # ----------------------------------------------------------------- trees of drafted tokens
 
 def _need_each(device: int, dtype: torch.dtype, names: str, *tensors: torch.Tensor) -> None:
-    """Operands of one dtype on the current device, contiguous in their last dimension."""
+    """Operands of one dtype on the current device, contiguous in their last dimension.  (A call's host time
+    is much of what a small one takes: ``stride(-1)`` costs 0.46 us, ``is_contiguous()`` 0.10.)"""
     for tensor in tensors:
-        if tensor.dtype != dtype or tensor.get_device() != device or tensor.stride(-1) != 1:
+        if (tensor.dtype is not dtype or tensor.get_device() != device
+                or not (tensor.is_contiguous() or tensor.stride(-1) == 1)):
             raise KernelError(f"{names}: each must be {dtype}, contiguous in its last dimension and on the "
                               "current CUDA device")
+
+
+def _need_whole(device: int, dtype: torch.dtype, names: str, *tensors: torch.Tensor) -> None:
+    """Lists and storage of one dtype on the current device, without gaps."""
+    for tensor in tensors:
+        if tensor.dtype is not dtype or tensor.get_device() != device or not tensor.is_contiguous():
+            raise KernelError(f"{names}: each must be {dtype}, contiguous and on the current CUDA device")
 
 
 def _here(tensor: torch.Tensor) -> int:
@@ -1085,31 +1094,34 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     most tokens a request brings, which the kernel is chosen by (any number gives the right result;
     default: what ``q`` has a request)."""
     device, code = _here(q), dtype_code(q.dtype)
-    _need_each(device, q.dtype, "q, k_cache, v_cache and out", q, k_cache, v_cache, out)
+    _need_each(device, q.dtype, "q and out", q, out)
+    _need_whole(device, q.dtype, "k_cache and v_cache", k_cache, v_cache)
     _need_each(device, torch.int64, "visible", visible)
-    _need_each(device, torch.int32, "request_start, request_context, request_table_row, block_tables and status",
-               request_start, request_context, request_table_row, block_tables, status)
+    _need_each(device, torch.int32, "block_tables", block_tables)
+    _need_whole(device, torch.int32, "request_start, request_context, request_table_row and status",
+                request_start, request_context, request_table_row, status)
     if visible.dim() != 2 or q.dim() != 2 or out.dim() != 2 or block_tables.dim() != 2:
         raise KernelError("visible is [tokens, words]; q, out and block_tables are matrices")
-    if (visible.shape[0] < min(q.shape[0], out.shape[0]) or request_start.shape[0] <= requests
-            or min(request_context.shape[0], request_table_row.shape[0]) < requests):
+    (tokens, width), (out_tokens, out_width), (masks, words) = q.shape, out.shape, visible.shape
+    if (masks < min(tokens, out_tokens) or request_start.numel() <= requests
+            or request_context.numel() < requests or request_table_row.numel() < requests):
         raise KernelError("every token has its words, and every request its start, end, context and table")
-    if min(q.shape[1], out.shape[1]) < heads * head_dim or \
+    if min(width, out_width) < heads * head_dim or \
             min(k_cache.numel(), v_cache.numel()) < num_pages * kv_heads * page_size * head_dim:
         raise KernelError("q and out hold the heads of a token in a row, the cache num_pages pages")
     floats = tree_attention_scratch(q.dtype, heads, kv_heads, head_dim, page_size)
     if partial is None:
         partial = torch.empty(floats, dtype=torch.float32, device=q.device)
     else:
-        _need_each(device, torch.float32, "partial", partial)
+        _need_whole(device, torch.float32, "partial", partial)
         if partial.numel() < floats:
             raise KernelError("partial is smaller than tree_attention_scratch says")
     _check(lib().hx_tree_attention(
-        q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), code, visible.data_ptr(),
-        visible.stride(0), visible.shape[1], request_start.data_ptr(), request_context.data_ptr(),
-        request_table_row.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), out.data_ptr(),
-        out.stride(0), partial.data_ptr(), requests, heads, kv_heads, head_dim, page_size, num_pages,
-        scale, max_nodes or -(-q.shape[0] // max(1, requests)), status.data_ptr(), _stream()))
+        q.data_ptr(), q.stride()[0], k_cache.data_ptr(), v_cache.data_ptr(), code, visible.data_ptr(),
+        visible.stride()[0], words, request_start.data_ptr(), request_context.data_ptr(),
+        request_table_row.data_ptr(), block_tables.data_ptr(), block_tables.stride()[0], out.data_ptr(),
+        out.stride()[0], partial.data_ptr(), requests, heads, kv_heads, head_dim, page_size, num_pages,
+        scale, max_nodes or -(-tokens // max(1, requests)), status.data_ptr(), _stream()))
 
 
 def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], token_ids: torch.Tensor,
@@ -1134,31 +1146,36 @@ def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], to
     tokens that stand, from 0 on, -1 behind them; ``kept`` how many they are; ``next_tokens``, -1
     (and FLAG_NONFINITE) when logits on the way are not finite.  A path that is full ends the walk."""
     device = _here(logits)
-    _need_each(device, torch.float32, "logits, temperature and uniform", logits, temperature, uniform)
-    _need_each(device, torch.int32, "token_ids, parents, request_start, path, kept, next_tokens and status",
-               token_ids, parents, request_start, path, kept, next_tokens, status)
+    _need_each(device, torch.float32, "logits", logits)
+    _need_whole(device, torch.float32, "temperature and uniform", temperature, uniform)
+    _need_each(device, torch.int32, "path", path)
+    _need_whole(device, torch.int32, "token_ids, parents, request_start, kept, next_tokens and status",
+                token_ids, parents, request_start, kept, next_tokens, status)
     if draft_logits is not None:
         _need_each(device, torch.float32, "draft_logits", draft_logits)
         if draft_logits.shape != logits.shape:
             raise KernelError("draft_logits has a row of the vocabulary for every row of logits")
-    tokens, vocab = logits.shape
-    if (min(token_ids.shape[0], parents.shape[0], uniform.shape[0]) < tokens or path.dim() != 2
-            or request_start.shape[0] <= requests
-            or min(temperature.shape[0], path.shape[0], kept.shape[0], next_tokens.shape[0]) < requests):
+    if logits.dim() != 2 or path.dim() != 2:
+        raise KernelError("logits and path are matrices")
+    (tokens, vocab), (rows, width) = logits.shape, path.shape
+    if (min(token_ids.numel(), parents.numel(), uniform.numel()) < tokens
+            or request_start.numel() <= requests
+            or min(temperature.numel(), rows, kept.numel(), next_tokens.numel()) < requests):
         raise KernelError("verify_drafts: an operand is too short for the step's tokens and requests")
     _check(lib().hx_verify_drafts(
-        logits.data_ptr(), logits.stride(0), None if draft_logits is None else draft_logits.data_ptr(),
-        0 if draft_logits is None else draft_logits.stride(0), vocab, token_ids.data_ptr(),
+        logits.data_ptr(), logits.stride()[0], None if draft_logits is None else draft_logits.data_ptr(),
+        0 if draft_logits is None else draft_logits.stride()[0], vocab, token_ids.data_ptr(),
         parents.data_ptr(), request_start.data_ptr(), temperature.data_ptr(), uniform.data_ptr(),
-        path.data_ptr(), path.stride(0), path.shape[1], kept.data_ptr(), next_tokens.data_ptr(), requests,
+        path.data_ptr(), path.stride()[0], width, kept.data_ptr(), next_tokens.data_ptr(), requests,
         1 if replacement else 0, status.data_ptr(), _stream()))
 
 
 def _storage_sizes(storage: torch.Tensor):
     """``[layers, 2, pages, kv_heads, page_size, head_dim]`` of a cache group's storage."""
-    if storage.dim() != 6 or storage.shape[1] != 2 or not storage.is_contiguous():
+    sizes = tuple(storage.shape)
+    if len(sizes) != 6 or sizes[1] != 2 or not storage.is_contiguous():
         raise KernelError("storage is [layers, 2, pages, kv_heads, page_size, head_dim], contiguous")
-    return storage.shape
+    return sizes
 
 
 def keep_rows(storage: torch.Tensor, block_tables: torch.Tensor, request_table_row: torch.Tensor,
@@ -1171,16 +1188,19 @@ def keep_rows(storage: torch.Tensor, block_tables: torch.Tensor, request_table_r
     whose path does not ascend, is longer than a row of ``path`` (FLAG_BAD_MOVE) or leads outside its
     pages (FLAG_BAD_PAGE) keeps its rows where they are.  Requests share no page they move rows in."""
     layers, _, pages, kv_heads, page_size, head_dim = _storage_sizes(storage)
-    _need_each(_here(storage), torch.int32,
-               "block_tables, request_table_row, request_context, path, kept and status", block_tables,
-               request_table_row, request_context, path, kept, status)
-    if path.dim() != 2 or min(request_table_row.shape[0], request_context.shape[0], path.shape[0],
-                              kept.shape[0]) < requests:
+    device = _here(storage)
+    _need_each(device, torch.int32, "block_tables and path", block_tables, path)
+    _need_whole(device, torch.int32, "request_table_row, request_context, kept and status", request_table_row,
+                request_context, kept, status)
+    if path.dim() != 2 or block_tables.dim() != 2:
+        raise KernelError("path and block_tables are matrices")
+    rows, width = path.shape
+    if min(request_table_row.numel(), request_context.numel(), rows, kept.numel()) < requests:
         raise KernelError("keep_rows: an operand is too short for the requests")
     _check(lib().hx_keep_rows(
         storage.data_ptr(), dtype_code(storage.dtype), 2 * layers, pages, kv_heads, page_size, head_dim,
-        block_tables.data_ptr(), block_tables.stride(0), request_table_row.data_ptr(),
-        request_context.data_ptr(), path.data_ptr(), path.stride(0), path.shape[1], kept.data_ptr(),
+        block_tables.data_ptr(), block_tables.stride()[0], request_table_row.data_ptr(),
+        request_context.data_ptr(), path.data_ptr(), path.stride()[0], width, kept.data_ptr(),
         requests, status.data_ptr(), _stream()))
 
 
@@ -1191,12 +1211,13 @@ def copy_pages(storage: torch.Tensor, source: torch.Tensor, target: torch.Tensor
     pool is left out (FLAG_BAD_PAGE), and so is one whose target another pair writes or reads
     (FLAG_BAD_MOVE); a page copied onto itself stays."""
     layers, _, pages, kv_heads, page_size, head_dim = _storage_sizes(storage)
-    _need_each(_here(storage), torch.int32, "source, target and status", source, target, status)
-    if source.shape != target.shape or source.dim() != 1:
+    _need_whole(_here(storage), torch.int32, "source, target and status", source, target, status)
+    pairs = source.numel()
+    if target.numel() != pairs or source.dim() != 1 or target.dim() != 1:
         raise KernelError("source and target are lists of pages of one length")
     _check(lib().hx_copy_pages(
         storage.data_ptr(), 2 * layers, pages, kv_heads * page_size * head_dim * storage.element_size(),
-        source.data_ptr(), target.data_ptr(), source.shape[0], status.data_ptr(), _stream()))
+        source.data_ptr(), target.data_ptr(), pairs, status.data_ptr(), _stream()))
 
 
 # ------------------------------------------------------------ residual streams, biased sums

@@ -284,5 +284,9 @@ def test_refusals():
     refused(visible=batch.visible[:2])
     refused(start=batch.start[:1])
     refused(k=batch.k.float())
+    refused(k=batch.k[:1].expand(batch.k.shape))      # one page held, many named
+    refused(context=batch.context[:1, None].expand(4, 1))
+    refused(tables=batch.tables[0])
+    refused(scale=float("inf"))
     refused(q=batch.q.double())
     refused(q=torch.zeros((7, 130), dtype=torch.bfloat16, device="cuda:0")[:, 1:129])      # not aligned

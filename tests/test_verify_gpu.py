@@ -265,6 +265,7 @@ def test_refusals():
     refused(uniform=good["uniform"][:7])
     refused(request_start=good["request_start"][:2])
     refused(temperature=good["temperature"].double())
+    refused(temperature=good["temperature"][:1].expand(2))
     refused(path=good["path"][:1])
     refused(path=good["path"].reshape(-1)[:2])
     refused(path=good["path"][:, :0])
