@@ -2,7 +2,10 @@
 // tokens to where they belong.  Both work on all layers of a group of layers at once:
 // storage [layer, key|value, page, kv_head, (head_dim / c, slot, c)], see hx_cache_offset.
 //
-// Both are bound by memory: every byte is read once and written once.
+// Both are bound by memory: every byte is read once and written once.  Measured (32 layers of 32 heads of 128): 64
+// pages to 64 others 159 us, 6.7 TB/s, as fast as any copy; one page 7 us, the call.  Kept rows of 32 requests, up to 6 each, 48 to
+// 56 us: 16 bytes of each 32-byte sector are wanted, 64 bytes at a time leave memory, and what is
+// wanted moves at 1.9 TB/s; one request's 9 us.
 //
 // Neither lets the next kernel in before it has completed.  Attention fetches what earlier steps have left
 // in the cache before it waits for the kernel in front of it, and that one may have been let in

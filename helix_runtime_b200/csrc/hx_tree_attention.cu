@@ -11,7 +11,7 @@
 // the drafted keys says nothing, and all tokens of a request read the same cached keys.  So a
 // CTA takes the tokens of a request (and the query heads that share a key/value head) as rows of
 // one tile and reads every key once for all of them; a long context is cut over CTAs (see
-// hx_tree_attention.cuh).  Three kernels:
+// hx_tree_attention.cuh).  Four kernels:
 //   * hx_tree_attention_stream.cu: bfloat16, heads of 64 to 128, pages of 8, 16 or 32 keys, few rows;
 //   * hx_tree_attention_tc.cu: the same with many rows, and pages of 64;
 //   * tree_tile_kernel: any other page size, float32 or bfloat16, heads up to 256 in steps of 4.
@@ -60,8 +60,10 @@ template <> __device__ __forceinline__ void bring_four<__nv_bfloat16>(float* pla
 // bytes of shared memory feed 64 multiply-adds of a warp.  Values: a lane has 4 (8, above 128)
 // coordinates of all 8 rows.  Both are bound by the multiply-adds, 3,900 cycles a tile of heads of 112;
 // what counts is that enough warps are there to wait for one another: a tile's values take the place of its
-// keys, so that four CTAs share an SM (two, with keys and values side by side and the next ones on
-// their way: 4 requests x 24 drafts 95 us).  A thread copies half a key, whose page it has looked up a tile before.
+// keys, so that four CTAs share an SM.  4 requests x 24 drafts behind 200 to 1,151 keys, 32 heads of 112, float32: 85 us
+// (1.09 TB/s, 11.1 TFLOP/s; two CTAs, with keys and values side by side and the next ones on their way, 95).  Of a tile's
+// 36,000 cycles, CTAs in step, scores are 12,000, weighted values 11,000, copies 8,500, the softmax 4,000; the
+// same rows spread evenly over the warps took 97 us, 2 keys by 8 rows a lane 90.  A thread copies half a key, whose page it has looked up a tile before.
 template <typename T, int D_MAX>
 __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tree_tile_kernel(
     const TreeArgs a) {
@@ -622,7 +624,10 @@ int launch_tile(const TreeArgs& a, int ctas, cudaStream_t stream) {
   return HX_OK;
 }
 
-// Where the streaming kernel still beats the tcgen05 one (see STREAM figures in hx_tree_attention_stream.cu).
+// Up to here the streaming kernel beats the tcgen05 one, whose tile of 128 rows is mostly empty then (32 heads of 128;
+// streaming against tcgen05): 64 requests x 8 or 16 drafts behind 1,200 keys 214 and 219 us against 259 and 267, x 32
+// drafts 280 against 292; 8 requests behind 640 keys 29, 31 and 38 us against 41, 42 and 43; one request, 32 rows
+// behind 32,701 keys, 45 against 49.  It has no tiles of more rows: a warp's 16 rows fill its registers.
 constexpr int STREAM_MOST_ROWS = 32;
 
 // Which kernel: the tensor cores', the tile kernel, or the row kernel.
