@@ -61,6 +61,9 @@ class DecodeGraphs:
         token): the step's tokens are the ids the previous step sampled in these rows, put in
         place by the first kernel of the graph."""
         from ..ops import library as ops
+        if ctx.trees is not None:
+            raise ValueError("a step of drafted trees is not recorded: its launches depend on more "
+                             "than a graph's key")
         key = self.key_for(ctx, n_want, greedy) + (("fed",) if feed_rows is not None else ())
         graph = self._graphs.get(key)
         if graph is not None:

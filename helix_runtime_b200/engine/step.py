@@ -289,7 +289,8 @@ class StepFunction:
         ``kept[r]`` tokens ``path[r]`` stay, a branch from the root down, as
         :meth:`helix_runtime_b200.sampling.sampler.Sampler.verify` names them.  Their keys and
         values move together, the request's length is published and the other tokens' pages are
-        given back.  Returns the tokens kept of each (waits for the device)."""
+        given back.  Returns the tokens kept of each (waits for the device).  What is no branch of its
+        tree is refused and changes nothing."""
         if self._trees is None:
             raise StepError("the last step brought no drafted trees")
         entries, ctx = self._trees
@@ -298,10 +299,14 @@ class StepFunction:
             # what a request that has ended held may be another's by now
             kept = kept[:len(entries)] * torch.tensor(live, dtype=kept.dtype, device=kept.device)
         counts = kept[:len(entries)].tolist()
-        for entry, count in zip(entries, counts):
-            if not 0 <= count <= len(entry.tokens):
+        for entry, count, row in zip(entries, counts, path[:len(entries)].tolist()):
+            if not 0 <= count <= min(len(entry.tokens), len(row)):
                 raise StepError(f"{count} tokens kept of the {len(entry.tokens)} of request "
                                 f"{entry.request!r}")
+            for token, parent in zip(row[:count], [-1] + row):
+                if not 0 <= token < len(entry.tokens) or entry.parents[token] != parent:
+                    raise StepError(f"what is kept of request {entry.request!r} is no branch of its "
+                                    "tree from the root down")
         for group in self.cache.groups:
             ops.keep_rows(group.storage, group.device_tables, ctx.request_slot, ctx.request_context,
                           path, kept, len(entries), self.status)

@@ -97,38 +97,40 @@ def test_what_is_kept_is_published_and_the_rest_given_back(monkeypatch):
     step = function(cache)
     published(cache, "a", 3)
     published(cache, "b", 8)
-    parents = random_parents(np.random.default_rng(0), 21)
+    parents = [-1, 0, 0, 1, 3, 4] + [5] * 15
     entries = [StepEntry("a", [1] * 21, (), parents), StepEntry("b", [1] * 6, (), parents[:6])]
     free = cache.free_pages()
     ctx, _, _, lengths = step.prepare(entries)
     step.finish(entries, lengths, ctx)
     assert (cache.length("a"), cache.reserved("a")) == (3, 24)
-    path = torch.zeros(2, 6, dtype=torch.int32)
+    path = torch.tensor([[0, 1, 3, 4, 5, 6], [0, 1, 3, 4, 5, -1]], dtype=torch.int32)
     with pytest.raises(StepError, match="wait for"):
         step.prepare([StepEntry("a", [1])])
     with pytest.raises(StepError, match="22 tokens kept"):
         step.keep(path, torch.tensor([22, 1], dtype=torch.int32))
+    with pytest.raises(StepError, match="no branch"):
+        step.keep(path.flip(1), torch.tensor([3, 1], dtype=torch.int32))
     assert not moved
-    assert step.keep(path, torch.tensor([3, 6], dtype=torch.int32)) == [3, 6]
-    assert moved == [([3, 6], 2)]
+    assert step.keep(path, torch.tensor([3, 5], dtype=torch.int32)) == [3, 5]
+    assert moved == [([3, 5], 2)]
     assert (cache.length("a"), cache.reserved("a")) == (6, 6)
-    assert (cache.length("b"), cache.reserved("b")) == (14, 14)
-    assert cache.free_pages() == [free[0] - 1 - 2]      # 6 tokens in two pages, 14 in four
+    assert (cache.length("b"), cache.reserved("b")) == (13, 13)
+    assert cache.free_pages() == [free[0] - 1 - 2]      # 6 tokens in two pages, 13 in four
     cache.check()
     # a request that ended in between keeps nothing, the others do
     ctx, _, _, lengths = step.prepare(entries)
     step.finish(entries, lengths, ctx)
     cache.release("a")
     published(cache, "a", 1)
-    assert step.keep(path, torch.tensor([3, 6], dtype=torch.int32)) == [0, 6]
-    assert moved[-1] == ([0, 6], 2) and cache.length("a") == 1 and cache.length("b") == 20
+    assert step.keep(path, torch.tensor([3, 5], dtype=torch.int32)) == [0, 5]
+    assert moved[-1] == ([0, 5], 2) and cache.length("a") == 1 and cache.length("b") == 18
     # flagged moves publish nothing
     ctx, _, _, lengths = step.prepare(entries)
     step.finish(entries, lengths, ctx)
     step.status.fill_(steps.ops.FLAG_BAD_MOVE)
     with pytest.raises(StepError, match="move in the cache"):
-        step.keep(path, torch.tensor([3, 6], dtype=torch.int32))
-    assert cache.length("b") == cache.reserved("b") == 20 and cache.length("a") == 1
+        step.keep(path, torch.tensor([3, 5], dtype=torch.int32))
+    assert cache.length("b") == cache.reserved("b") == 18 and cache.length("a") == 1
     cache.check()
     step.prepare([StepEntry("a", [1])])
 

@@ -8,6 +8,7 @@ import torch
 
 from conftest import random_tokens
 from engine_harness import Harness, assert_close, tolerance
+from helix_runtime_b200.engine.graphs import DecodeGraphs
 from helix_runtime_b200.engine.step import StepEntry, StepError
 from helix_runtime_b200.ops import library as ops
 from helix_runtime_b200.sampling.sampler import Sampler
@@ -165,6 +166,8 @@ def test_requests_that_end_before_their_trees_are_settled(folders):
     storage = harness.cache.groups[0].storage
     path = torch.tensor([[0, 2, 4, -1, -1]] * 2, dtype=torch.int32, device="cuda:0")
     kept = torch.full((2,), 3, dtype=torch.int32, device="cuda:0")
+    with pytest.raises(ValueError, match="not recorded"):
+        DecodeGraphs(harness.step, None).run(harness.step.last_context, None, 0, True)
     with pytest.raises(StepError, match="6 tokens kept"):
         harness.step.keep(path, kept + 3)
     harness.end("a")
@@ -184,9 +187,18 @@ def test_a_path_that_is_none_publishes_nothing(folders):
     harness.run([("a", [1, 2, 3], ())])
     harness.step.run([StepEntry("a", [4, 5, 6, 7], (), [-1, 0, 0, 1])])
     path = torch.tensor([[0, 3, 1, -1]], dtype=torch.int32, device="cuda:0")
-    with pytest.raises(StepError, match="move in the cache"):
-        harness.step.keep(path, torch.full((1,), 3, dtype=torch.int32, device="cuda:0"))
-    assert harness.cache.length("a") == 3 and harness.cache.reserved("a") == 3
+    before = harness.cache.groups[0].storage.clone()
+    kept = torch.full((1,), 3, dtype=torch.int32, device="cuda:0")
+    for wrong in ([0, 3, 1, -1], [0, 2, 3, -1], [0, 1, 4, -1], [1, 3, -1, -1], [0, 1, -1, -1], [0, 1, 2, 3]):
+        with pytest.raises(StepError, match="no branch"):
+            harness.step.keep(torch.tensor([wrong], dtype=torch.int32, device="cuda:0"), kept)
+    with pytest.raises(StepError, match="3 tokens kept"):
+        harness.step.keep(path[:, :2].contiguous(), kept)
+    assert torch.equal(harness.cache.groups[0].storage.view(torch.int32), before.view(torch.int32))
+    assert harness.cache.length("a") == 3 and harness.cache.reserved("a") == 7
+    path = torch.tensor([[0, 1, 3, -1]], dtype=torch.int32, device="cuda:0")
+    assert harness.step.keep(path, kept) == [3]
+    assert harness.cache.length("a") == 6 and harness.cache.reserved("a") == 6
     harness.cache.check()
     assert harness.run([("a", [4], [0])]) is not None
 
