@@ -56,14 +56,54 @@ template <> __device__ __forceinline__ void bring_four<__nv_bfloat16>(float* pla
   *reinterpret_cast<float4*>(place) = there ? load_four<__nv_bfloat16>(from) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 }
 
+// a += w x and b += w y, one instruction.
+__device__ __forceinline__ void two_fma(float w, float x, float y, float& a, float& b) {
+  asm("{\n\t.reg .b64 w, v, s;\n\t"
+      "mov.b64 w, {%2, %2};\n\tmov.b64 v, {%3, %4};\n\tmov.b64 s, {%0, %1};\n\t"
+      "fma.rn.f32x2 s, w, v, s;\n\tmov.b64 {%0, %1}, s;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(w), "f"(x), "f"(y));
+}
+
+// acc[i] += a tile's values by the probabilities of row i: coordinates 4 lane .. of a warp's rows.  MASKED: a
+// (drafted) key that a row does not see adds nothing to it, not even an infinity times zero.
+template <bool MASKED, int PIECES>
+__device__ __forceinline__ void tile_weigh(float4 (&acc)[ROWS_A_WARP][PIECES], const float4* my_p, const float* values,
+                                           int D, int lane, int keys) {
+  for (int key4 = 0; key4 * 4 < keys; ++key4) {
+    float4 v[4][PIECES];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) {
+        const int d = 4 * lane + 128 * j;
+        if (d < D) v[k][j] = *reinterpret_cast<const float4*>(values + (4 * key4 + k) * (D + 4) + d);
+      }
+#pragma unroll
+    for (int i = 0; i < ROWS_A_WARP; ++i) {
+      const float4 p = my_p[i * (TILE_KEYS / 4) + key4];
+      const float w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          if (MASKED && w[k] == 0.0f) continue;
+          two_fma(w[k], v[k][j].x, v[k][j].y, acc[i][j].x, acc[i][j].y);
+          two_fma(w[k], v[k][j].z, v[k][j].w, acc[i][j].z, acc[i][j].w);
+        }
+    }
+  }
+}
+
 // A warp has 8 rows of the tile.  Scores: a lane has 4 keys (16 apart) of 4 rows, so that 12 reads of 128
 // bytes of shared memory feed 64 multiply-adds of a warp.  Values: a lane has 4 (8, above 128)
 // coordinates of all 8 rows.  Both are bound by the multiply-adds, 3,900 cycles a tile of heads of 112;
 // what counts is that enough warps are there to wait for one another: a tile's values take the place of its
-// keys, so that four CTAs share an SM.  4 requests x 24 drafts behind 200 to 1,151 keys, 32 heads of 112, float32: 85 us
-// (1.09 TB/s, 11.1 TFLOP/s; two CTAs, with keys and values side by side and the next ones on their way, 95).  Of a tile's
-// 36,000 cycles, CTAs in step, scores are 12,000, weighted values 11,000, copies 8,500, the softmax 4,000; the
-// same rows spread evenly over the warps took 97 us, 2 keys by 8 rows a lane 90.  A thread copies half a key, whose page it has looked up a tile before.
+// keys, so that four CTAs share an SM.  4 requests x 24 drafts behind 700 keys, 32 heads of 112, float32: 79 us
+// (1.1 TB/s, 12 TFLOP/s).  Two CTAs, with keys and values side by side and the next ones on their way, took 95, the
+// same rows spread evenly over the warps 97, 2 keys by 8 rows a lane 90; weighted values without a question for masks where no key is
+// drafted, two multiply-adds an instruction, 79 instead of 84 (the same for the scores took registers it has not: 90).  Of a tile's
+// 35,000 cycles, CTAs in step, scores are 12,000, weighted values 10,000, copies 8,500, the softmax 4,000.  A thread copies half a key, whose page it has looked up a tile before.
 template <typename T, int D_MAX>
 __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tree_tile_kernel(
     const TreeArgs a) {
@@ -128,13 +168,8 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
       reinterpret_cast<float4*>(q_rows)[row * D4 + d4] = value;
     }
     float row_max[4], row_sum[4];      // of the rows whose scores this lane has
-    const unsigned long long* words[4];
-    unsigned long long first_word[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int row = warp * ROWS_A_WARP + 4 * row_y + j;
-      words[j] = tree_words(a, c, rows.token0 + min(row, rows_here - 1) / rows.heads);
-      first_word[j] = __ldg(words[j]);
       row_max[j] = -INFINITY;
       row_sum[j] = 0.0f;
     }
@@ -188,7 +223,7 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
         const int row = warp * ROWS_A_WARP + 4 * row_y + j;
         unsigned long long mask = ~0ull;
         if (drafted)
-          mask = row < rows_here ? tree_mask_of(a, c, key0, first_word[j], [&](int word) { return words[j][word]; }) : 0ull;
+          mask = row < rows_here ? tree_mask(a, c, rows.token0 + row / rows.heads, key0) : 0ull;
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -229,32 +264,8 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
       // ---- the weighted values: coordinates 4 lane .. of 8 rows, four keys at a time
       const float4* my_p = reinterpret_cast<const float4*>(probabilities) + warp * ROWS_A_WARP * (TILE_KEYS / 4);
       const int keys_here = live ? min(TILE_KEYS, last_key + 1 - key0) : 0;
-      for (int key4 = 0; key4 * 4 < keys_here; ++key4) {
-        float4 v[4][OUT_PIECES];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int j = 0; j < OUT_PIECES; ++j) {
-            const int d = 4 * lane + 128 * j;
-            if (d < D) v[k][j] = *reinterpret_cast<const float4*>(values + (4 * key4 + k) * (D + 4) + d);
-          }
-#pragma unroll
-        for (int i = 0; i < ROWS_A_WARP; ++i) {
-          const float4 p = my_p[i * (TILE_KEYS / 4) + key4];
-          const float w[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int j = 0; j < OUT_PIECES; ++j) {
-              // (a drafted key that a row does not see adds nothing to it, not even an infinity times zero)
-              if (drafted && w[k] == 0.0f) continue;
-              acc[i][j].x = fmaf(w[k], v[k][j].x, acc[i][j].x);
-              acc[i][j].y = fmaf(w[k], v[k][j].y, acc[i][j].y);
-              acc[i][j].z = fmaf(w[k], v[k][j].z, acc[i][j].z);
-              acc[i][j].w = fmaf(w[k], v[k][j].w, acc[i][j].w);
-            }
-        }
-      }
+      if (drafted) tile_weigh<true>(acc, my_p, values, D, lane, keys_here);
+      else tile_weigh<false>(acc, my_p, values, D, lane, keys_here);
       if (more) {
         __syncthreads();      // the values have been read
         if (!bring(key, page, k_cache, my_keys, 4 * TILE_KEYS)) atomicOr(a.status, HX_FLAG_BAD_PAGE);
