@@ -12,10 +12,10 @@
 // softmax stays in registers and is the A operand of the second product, values again from their
 // blocks (ldmatrix.trans).  Shared memory is written by the copy engine alone.
 //
-// Probabilities of up to 16 rows enter the second product as two bfloat16 terms (hi + lo, 16 bits), which
-// costs nothing there; those of more rows as one, which is what the output is rounded to, too, and the sum is
-// over the weights as rounded (64 requests x 32 drafts, two terms 323 us, one 290).  The reference of a row's
-// exponentials is raised when a chunk exceeds it by more than 2^8, each row by itself.
+// Probabilities enter the second product as two bfloat16 terms (hi + lo, 16 bits), which costs nothing for up to
+// 16 rows; for more, one term alone (2^-8 of each weight off) would save a tenth (64 requests x 32 drafts, two
+// terms 323 us, one 290).  The reference of a row's exponentials is raised when a chunk exceeds it by more than 2^8,
+// each row by itself.
 //
 // Measured (32 heads of 128, pages of 16): 64 requests x 16 drafts behind 1,200 keys 219 us, 5.8 TB/s of the 6.55 that a
 // copy reaches: memory.  8 x 32 behind 640 keys 38 us, 2.3 TB/s: a run of 4 chunks a CTA is too short to hide how
@@ -100,7 +100,6 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
   using Config = StreamConfig<D, WARPS>;
   constexpr int RING = Config::kRing, ROWS = Config::kRows;
   constexpr int D_STEPS = D / 16, D_TILES = D / 8;
-  constexpr bool TWO_TERMS = WARPS == 1;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t full[RING], empty[RING];
   // the run is found from the step's description, which was there before the kernel in front
@@ -325,18 +324,10 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
           const float p1 = fast_exp2(fmaf(s[j][1], scale_log2, -against_low));
           const float p2 = fast_exp2(fmaf(s[j][2], scale_log2, -against_high));
           const float p3 = fast_exp2(fmaf(s[j][3], scale_log2, -against_high));
-          if constexpr (TWO_TERMS) {
-            sum_low += p0 + p1;
-            sum_high += p2 + p3;
-            hx_split_bf16(p0, p1, p_hi[j >> 1][2 * (j & 1)], p_lo[j >> 1][2 * (j & 1)]);
-            hx_split_bf16(p2, p3, p_hi[j >> 1][2 * (j & 1) + 1], p_lo[j >> 1][2 * (j & 1) + 1]);
-          } else {
-            const uint32_t low = hx_pack_bf16(p0, p1), high = hx_pack_bf16(p2, p3);
-            sum_low += __uint_as_float(low << 16) + __uint_as_float(low & 0xffff0000u);
-            sum_high += __uint_as_float(high << 16) + __uint_as_float(high & 0xffff0000u);
-            p_hi[j >> 1][2 * (j & 1)] = low;
-            p_hi[j >> 1][2 * (j & 1) + 1] = high;
-          }
+          sum_low += p0 + p1;
+          sum_high += p2 + p3;
+          hx_split_bf16(p0, p1, p_hi[j >> 1][2 * (j & 1)], p_lo[j >> 1][2 * (j & 1)]);
+          hx_split_bf16(p2, p3, p_hi[j >> 1][2 * (j & 1) + 1], p_lo[j >> 1][2 * (j & 1) + 1]);
         }
         // ---- the weighted values: d tiles 2 m and 2 m + 1
         if (!drafted) {
@@ -348,10 +339,8 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
               hx_ldmatrix_x4_trans(b, v_half + v_offset[h] + m * piece_step);
               hx_mma_bf16(o[2 * m], p_hi[h], b[0], b[1]);
               hx_mma_bf16(o[2 * m + 1], p_hi[h], b[2], b[3]);
-              if (TWO_TERMS) {
-                hx_mma_bf16(o[2 * m], p_lo[h], b[0], b[1]);
-                hx_mma_bf16(o[2 * m + 1], p_lo[h], b[2], b[3]);
-              }
+              hx_mma_bf16(o[2 * m], p_lo[h], b[0], b[1]);
+              hx_mma_bf16(o[2 * m + 1], p_lo[h], b[2], b[3]);
             }
         } else {
           bool found = false;
@@ -367,10 +356,8 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
                 b[e] = finite_part(b[e], 16 * h + 8 * (e & 1) + 2 * quad, first_drafted, there, found);
               hx_mma_bf16(o[2 * m], p_hi[h], b[0], b[1]);
               hx_mma_bf16(o[2 * m + 1], p_hi[h], b[2], b[3]);
-              if (TWO_TERMS) {
-                hx_mma_bf16(o[2 * m], p_lo[h], b[0], b[1]);
-                hx_mma_bf16(o[2 * m + 1], p_lo[h], b[2], b[3]);
-              }
+              hx_mma_bf16(o[2 * m], p_lo[h], b[0], b[1]);
+              hx_mma_bf16(o[2 * m + 1], p_lo[h], b[2], b[3]);
             }
           poisoned |= __any_sync(0xffffffffu, found) != 0;
         }

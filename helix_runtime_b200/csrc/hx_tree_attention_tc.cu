@@ -11,9 +11,10 @@
 //               thread a row the softmax took 2,000 cycles a tile, a chain of instructions that no
 //               product or copy was long enough to hide: 64 requests x 64 drafts 405 us).  They tell each other their
 //               maxima, so both keep the same reference.  P goes back
-//               over the scores they have read, in bfloat16: each weight is rounded to 8 bits once, as the
-//               output is (a second term, which streaming for few rows has for nothing, would fill the
-//               columns the maxima are told through, and take a third of the products' time).  P is the A
+//               over the scores they have read as two bfloat16 terms (hi + lo, 16 bits of each weight, as in
+//               the kernels of prompts and single tokens: one term alone is 2^-8 of each weight off, as much again as the
+//               output's rounding).  They fill the score buffer, also the columns that the maxima are told
+//               through, so the low terms wait until the other thread has read.  P is the A
 //               operand of O += P V straight from tensor memory; the reference of the exponentials is
 //               raised when a tile exceeds it by more than 2^8, O stays in tensor memory.
 // Keys and values keep flowing across items: the rings go by TURNS, the key tiles of the CTA's run in
@@ -441,12 +442,14 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
           }
           tc_fence_after();
           const uint64_t desc_v = desc_v0 + stage * (Config::kHalfBytes >> 4);
-          // (16 columns of P from either half's first column on)
+          // (from either half's first column on 16 columns of P's high terms, and 16 of its low ones)
           const uint32_t probabilities = tmem_base + b * BLOCK_N;
 #pragma unroll
-          for (int g = 0; g < BLOCK_N / 16; ++g)
-            umma_bf16_a_tmem(target, probabilities + (g >> 1) * (BLOCK_N / 2) + (g & 1) * 8, desc_v + value_step[g],
-                             idesc, (t > 0 || g > 0) ? 1u : 0u);
+          for (int g = 0; g < BLOCK_N / 16; ++g) {
+            const uint32_t high = probabilities + (g >> 1) * (BLOCK_N / 2) + (g & 1) * 8;
+            umma_bf16_a_tmem(target, high, desc_v + value_step[g], idesc, (t > 0 || g > 0) ? 1u : 0u);
+            umma_bf16_a_tmem(target, high + BLOCK_N / 4, desc_v + value_step[g], idesc, 1u);
+          }
           umma_commit(&v_done[stage]);
           umma_commit(&o_full[b]);
         }
@@ -465,19 +468,29 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
     const float scale_log2 = a.scale * HX_LOG2E;      // positive: it does not change which score is largest
     const uint64_t factor_pair = pair_of(scale_log2, scale_log2);
     uint32_t meetings = 0;
-    // This thread's number for the one that the other thread of the row tells, through a column of the score
-    // buffer that neither scores still wanted nor probabilities take.  (The buffer's next scores wait for the
-    // probabilities of both threads, so nothing is overwritten that has not been read.)
-    auto exchange = [&](uint32_t columns, float mine, float& other) {
-      tmem_store1(columns + half * HALF, mine);
-      tmem_store_wait();
+    // The two warps of 32 rows meet: each arrives, and waits for both.
+    auto arrive = [&]() {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&met[quarter]);
+    };
+    auto meet = [&]() {
       const bool there = wait_for(&met[quarter], meetings++);
       tc_fence_after();
-      if (there) other = tmem_load1(columns + (half ^ 1) * HALF);
       return there;
+    };
+    // This thread's number for the one that the other thread of the row tells, through a column of the score
+    // buffer whose score has been read.  The arrival behind it says that the other's has been read, too: before
+    // anything else goes into that column (the low terms of the probabilities, the next scores, which wait for
+    // them) the threads have met once more.
+    auto exchange = [&](uint32_t columns, float mine, float& other) {
+      tmem_store1(columns + half * HALF, mine);
+      tmem_store_wait();
+      arrive();
+      if (!meet()) return false;
+      other = tmem_load1(columns + (half ^ 1) * HALF);
+      arrive();
+      return true;
     };
     TreeCursor c = at;
     int turn = 0, segment = 0;
@@ -560,32 +573,35 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
               tmem_store16_raw(output_base + d0, r);
             }
           }
-          // P in bfloat16, two keys per column, the earlier key in the lower half; the sum is over the
-          // probabilities as rounded, so that the weights of a row add up to one
+          // P = hi + lo, two keys per column, the earlier key in the lower half
           uint64_t part_sum[2] = {0, 0};
           const float reference = row_max == -INFINITY ? 0.0f : row_max;
           const uint64_t reference_pair = pair_of(-reference, -reference);
-          uint32_t packed[16];
+          uint32_t high[16], low[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float x0, x1;
             halves_of(pair_fma(pair_of(p[2 * i], p[2 * i + 1]), factor_pair, reference_pair), x0, x1);
-            packed[i] = pack_bf16(fast_exp2(x0), fast_exp2(x1));
-            part_sum[i % 2] = pair_add(part_sum[i % 2], pair_of(__uint_as_float(packed[i] << 16),
-                                                                __uint_as_float(packed[i] & 0xffff0000u)));
+            x0 = fast_exp2(x0);
+            x1 = fast_exp2(x1);
+            part_sum[i % 2] = pair_add(part_sum[i % 2], pair_of(x0, x1));
+            hx_split_bf16(x0, x1, high[i], low[i]);
           }
           {
-            float low, high;
-            halves_of(pair_add(part_sum[0], part_sum[1]), low, high);
-            row_sum += low + high;
+            float even, odd;
+            halves_of(pair_add(part_sum[0], part_sum[1]), even, odd);
+            row_sum += even + odd;
           }
-          tmem_store16_raw(score_base + half * HALF, packed);
+          tmem_store16_raw(score_base + half * HALF, high);
+          ok = meet();
+          if (!ok) break;
           if (t == count - 1) {
             float other_sum = 0.0f;
-            ok = exchange(score_base + HALF / 2 + 1, row_sum, other_sum);
+            ok = exchange(score_base + HALF / 2 + 1, row_sum, other_sum) && meet();
             if (!ok) break;
             row_sum = half == 0 ? row_sum + other_sum : other_sum + row_sum;
           }
+          tmem_store16_raw(score_base + half * HALF + HALF / 2, low);
           tmem_store_wait();
         }
         if (drafted) {

@@ -290,3 +290,29 @@ def test_refusals():
     refused(scale=float("inf"))
     refused(q=batch.q.double())
     refused(q=torch.zeros((7, 130), dtype=torch.bfloat16, device="cuda:0")[:, 1:129])      # not aligned
+
+
+@pytest.mark.parametrize("head_dim,page,rows", [(128, 16, 16), (128, 16, 32), (64, 8, 32), (64, 32, 32), (128, 16, 128),
+                                                (128, 32, 128), (112, 64, 128), (64, 8, 128)])
+def test_weights_keep_sixteen_bits(head_dim, page, rows):
+    """A weight enters the products as two bfloat16 terms whichever kernel takes the step, as it does in the
+    kernels of prompts and single tokens: what follows its parent is scored alike however many others are drafted.
+
+    The tolerance.  With d = 2^-8 the first term leaves at most d of a weight and the second at most d of that: a
+    weight is off by 2^-16 of itself.  The sum of the weights takes them as they are.  The tensor cores' sums
+    may cut where float32 rounds, u = 2^-23 a step: head_dim products of a score (and three
+    roundings of its scale and reference) in numerator and denominator, two terms of a key in the numerator and
+    one in the denominator; exponentials, correction of the reference and joined parts 64 u.  Last the output's rounding,
+    2^-8 of it.  Of many outputs some are nearly zero beside what was weighed, and there one term alone (2^-8 of each
+    weight) is off by a multiple of this."""
+    batch = Batch(20, [40, 9, 300], [12, 30, 3], 4, 2, head_dim, page, torch.bfloat16)
+    batch.q_host = batch.q_host * 0.25
+    batch.q *= 0.25
+    batch.run(ops, max_nodes=rows // 2)
+    expected, weighed, largest = batch.expected()
+    u, keys = 2.0 ** -23, 303
+    near = weighed * (2.0 ** -16 + 2 * (head_dim + 3) * u * largest + (4 * keys + 64) * u)
+    allowed = near + 2.0 ** -8 * (expected.abs() + near)
+    off = (batch.out[:batch.tokens, :4 * head_dim].double().cpu() - expected).abs()
+    assert bool((off <= allowed).all()), f"{int((off > allowed).sum())} of {off.numel()} outputs are further off"
+    assert int(batch.status.item()) == 0
