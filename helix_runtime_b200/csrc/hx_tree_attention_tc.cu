@@ -183,8 +183,11 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
   uint64_t* met = q_done + 1;                  // [4] both softmax warps of 32 rows have told
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(met + 4);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  volatile int* poisoned = failed + 1;         // the last segment with a drafted value that is not finite
-  static_assert((2 * K_STAGES + 2 * V_STAGES + 12) * 8 + 12 <= Config::kBarrierBytes, "the place of barriers and flags");
+  // [2] the last even and the last odd segment with a drafted value that is not finite.  (A warp without rows may
+  // already look at the first tiles of segment n + 1 while others write rows of segment n, but comes no
+  // further: their probabilities of n + 1 are wanted for its products.)
+  volatile int* poisoned = failed + 1;
+  static_assert((2 * K_STAGES + 2 * V_STAGES + 12) * 8 + 16 <= Config::kBarrierBytes, "the place of barriers and flags");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
     mbar_init(q_done, 1);
     for (int quarter = 0; quarter < 4; ++quarter) mbar_init(&met[quarter], 2);
     *failed = 0;
-    *poisoned = -1;
+    poisoned[0] = poisoned[1] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -630,7 +633,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
             }
             found = wrote && key < c.context + c.nodes - key0;
           }
-          if (found) *poisoned = segment;
+          if (found) poisoned[segment & 1] = segment;
           if (__any_sync(0xffffffffu, wrote)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         tc_fence_before();
@@ -682,7 +685,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
           part[static_cast<size_t>(D + 1) * BLOCK_M + row] = row_sum;
         }
         // (told before the arrivals that the last output product waited for)
-        if (*poisoned == segment && row < rows_here)
+        if (poisoned[segment & 1] == segment && row < rows_here)
           add_not_finite<D>(a, c, count, my_token, row, half, whole ? out : nullptr, whole ? nullptr : part);
         tc_fence_before();
       }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from helix_runtime_b200.ops import library as ops
-from plain_tree import Batch, ancestors, random_parents
+from plain_tree import Batch, ancestors, from_cache, random_parents, to_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -315,4 +315,48 @@ def test_weights_keep_sixteen_bits(head_dim, page, rows):
     allowed = near + 2.0 ** -8 * (expected.abs() + near)
     off = (batch.out[:batch.tokens, :4 * head_dim].double().cpu() - expected).abs()
     assert bool((off <= allowed).all()), f"{int((off > allowed).sum())} of {off.numel()} outputs are further off"
+    assert int(batch.status.item()) == 0
+
+
+def put(batch, cache, token, coordinate, number):
+    """``number`` into one coordinate of the drafted token ``token`` of every request, in every key/value head."""
+    page, dtype = batch.page_size, cache.dtype
+    for r, context in enumerate(batch.contexts):
+        place = context + token
+        page_id = int(batch.tables[batch.row[r], place // page])
+        held = from_cache(cache[page_id]).clone()
+        held[:, place % page, coordinate] = number
+        cache[page_id] = to_cache(held, dtype)
+
+
+@pytest.mark.parametrize("head_dim,page", [(128, 16), (64, 32), (112, 64), (80, 8)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("contexts,heads,extra", [
+    ([1 + 7 * (i % 8) for i in range(48)], 32, 0),       # short requests: a CTA has many items of one tile
+    ([1 + 7 * (i % 8) for i in range(48)], 32, 33),      # ... of one or two, half of the warps with rows
+    ([0, 700, 20], 4, 0),                                # items cut over CTAs
+    ([700, 64, 1], 4, 90),
+])
+def test_tensor_memory_values_that_are_not_finite_in_every_item(head_dim, page, bad, contexts, heads, extra):
+    """A drafted token whose values overflowed in all heads: every item of a CTA has such a value, and each
+    reaches, coordinate by coordinate, the tokens that see it and no other."""
+    nodes = 12 + extra
+    parents = [-1, 0, 0, 1, 1, 2, 2, 3, 3, 5, 5, 6] + [4] * extra
+    seen = [ancestors(parents)] * len(contexts)
+    args = (23, contexts, [nodes] * len(contexts), heads, heads, head_dim, page, torch.bfloat16)
+    clean = Batch(*args, seen=seen)
+    clean.run(ops, max_nodes=128)
+    batch = Batch(*args, seen=seen)
+    put(batch, batch.v, 2, 1, bad)
+    hit = torch.zeros((len(contexts), nodes, heads, head_dim), dtype=torch.bool, device=batch.out.device)
+    hit[:, [2, 5, 6, 9, 10, 11], :, 1] = True
+    hit = hit.view(batch.tokens, heads * head_dim)
+    want = clean.out[:batch.tokens]
+    assert bool(want.isfinite().all())
+    for _ in range(5):
+        batch.out.fill_(7.0)
+        batch.run(ops, max_nodes=128)
+        got = batch.out[:batch.tokens]
+        assert bool((got[hit].isnan() if bad != bad else got[hit] == bad).all())
+        assert torch.equal(got[~hit], want[~hit])
     assert int(batch.status.item()) == 0
