@@ -281,7 +281,7 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
         const float sum = __shfl_sync(0xffffffffu, row_sum[i % 4], i / 4 * 16);
         const int row = warp * ROWS_A_WARP + i;
         if (row >= rows_here) continue;
-        const float inverse = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inverse = tree_inverse(sum);
         T* out = static_cast<T*>(a.out) + static_cast<size_t>(c.q_begin + rows.token0 + row / rows.heads) * a.ldo +
                  static_cast<size_t>(rows.head0 + row % rows.heads) * D;
 #pragma unroll
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(ROW_WARPS * 32) void tree_row_kernel(const TreeArgs
         }
       }
       const bool whole = c.tile == 0 && count == c.tiles;
-      const float inverse = row_sum > 0.0f ? 1.0f / row_sum : 0.0f;
+      const float inverse = tree_inverse(row_sum);
       T* out = static_cast<T*>(a.out) + static_cast<size_t>(c.q_begin + token) * a.ldo +
                static_cast<size_t>(head) * D;
       float* part = tree_part<ROW_WARPS>(a, blockIdx.x, c.tile == 0);
@@ -449,7 +449,9 @@ template <int COUNT>
 struct Joined {
   float top = -INFINITY, sum = 0.0f, acc[COUNT] = {};
   __device__ __forceinline__ void add(float m, float l, const float (&o)[COUNT]) {
-    if (m == -INFINITY) return;      // no part, or one whose row saw nothing
+    // no part, or one whose row saw nothing.  (Scores that are no numbers leave no maximum either, but a sum
+    // that is none: it goes on into the row's.)
+    if (m == -INFINITY && !(l != l)) return;
     const float new_top = fmaxf(top, m);
     const float keep = exp2f(top - new_top), take = exp2f(m - new_top);
     top = new_top;
@@ -472,6 +474,7 @@ __device__ __forceinline__ Joined<COUNT> join_parts(const TreeArgs& a, int owner
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
       m[u] = -INFINITY;
+      l[u] = 0.0f;
       if (base + u < end) {
         const int index = base + u;
         const float* part = a.partial + (index == 0 ? 2ll * owner + 1 : 2ll * (owner + index)) * stride;
@@ -499,7 +502,7 @@ __device__ __forceinline__ Joined<COUNT> join_parts(const TreeArgs& a, int owner
 template <typename T, int COUNT>
 __device__ __forceinline__ void store_joined(const TreeArgs& a, const TreeCut& cut, int row, int group,
                                              const Joined<COUNT>& joined) {
-  const float inverse = joined.sum > 0.0f ? 1.0f / joined.sum : 0.0f;
+  const float inverse = tree_inverse(joined.sum);
   T* out = static_cast<T*>(a.out) + static_cast<size_t>(cut.token + row / cut.heads) * a.ldo +
            static_cast<size_t>(cut.head0 + row % cut.heads) * a.head_dim + group * COUNT;
   const int here = a.head_dim - group * COUNT;

@@ -165,6 +165,9 @@ __device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
+// One over a row's sum of weights; a row that saw nothing becomes zeros, one whose scores are no numbers stays none.
+__device__ __forceinline__ float tree_inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+
 // A CTA's run of the list.  Runs are at least `least` tiles long, so that a short list does not
 // become more parts than it is worth.
 struct TreeRun {

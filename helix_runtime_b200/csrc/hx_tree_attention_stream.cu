@@ -396,8 +396,8 @@ __global__ __launch_bounds__(WARPS * 32, StreamConfig<D, WARPS>::kCtas) void tre
       }
       const bool whole = c.tile == 0 && count == c.tiles;
       if (whole) {
-        const float inverse_low = sum_low > 0.0f ? 1.0f / sum_low : 0.0f;
-        const float inverse_high = sum_high > 0.0f ? 1.0f / sum_high : 0.0f;
+        const float inverse_low = tree_inverse(sum_low);
+        const float inverse_high = tree_inverse(sum_high);
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + 2 * quad;
         __nv_bfloat16* out_low = out + static_cast<size_t>(c.q_begin + token_low) * a.ldo + static_cast<size_t>(head_low) * D;
         __nv_bfloat16* out_high = out + static_cast<size_t>(c.q_begin + token_high) * a.ldo + static_cast<size_t>(head_high) * D;

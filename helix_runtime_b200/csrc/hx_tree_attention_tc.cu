@@ -648,7 +648,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
       if (live) {
         tc_fence_after();
         const bool whole = c.tile == 0 && count == c.tiles;
-        const float inverse = row_sum > 0.0f ? 1.0f / row_sum : 0.0f;
+        const float inverse = tree_inverse(row_sum);
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(c.q_begin + my_token) * a.ldo +
                              static_cast<size_t>(my_head) * D;
         float* part = tree_part<BLOCK_M>(a, blockIdx.x, c.tile == 0);
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
           __syncwarp();
           tmem_load16(output_base + d0, o);
           if (row < rows_here) {
-            if (row_max == -INFINITY) {
+            if (row_sum == 0.0f) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = 0.0f;
             }

@@ -360,3 +360,56 @@ def test_tensor_memory_values_that_are_not_finite_in_every_item(head_dim, page, 
         assert bool((got[hit].isnan() if bad != bad else got[hit] == bad).all())
         assert torch.equal(got[~hit], want[~hit])
     assert int(batch.status.item()) == 0
+
+
+# A call of each kernel: its type, heads and pages, and the rows (tokens times query heads of a key/value
+# head) that the call is told a request has at most.
+KERNELS = [
+    ("streaming, one warp", torch.bfloat16, 128, 16, 1),
+    ("streaming, two warps", torch.bfloat16, 128, 16, 32),
+    ("streaming, two warps", torch.bfloat16, 64, 8, 32),
+    ("tensor memory", torch.bfloat16, 128, 16, 128),
+    ("tensor memory", torch.bfloat16, 64, 32, 128),
+    ("tensor memory", torch.bfloat16, 112, 64, 128),
+    ("tensor memory", torch.bfloat16, 80, 8, 128),
+    ("tiles", torch.bfloat16, 64, 24, 1),
+    ("tiles", torch.float32, 128, 16, 1),
+    ("tiles", torch.float32, 256, 16, 1),
+    ("rows", torch.bfloat16, 300, 8, 1),
+    ("rows", torch.float32, 6, 4, 1),
+]
+
+
+@pytest.mark.parametrize("kernel,dtype,head_dim,page,rows", KERNELS)
+@pytest.mark.parametrize("contexts", [[0, 0], [20, 20], [300, 300], [320, 320], [1500, 40]])
+def test_a_query_that_is_no_number_says_so(kernel, dtype, head_dim, page, rows, contexts):
+    """Whatever the length, so whether or not its keys are cut over CTAs; no other row is touched."""
+    nodes, heads = [9, 5], 4
+    clean = Batch(21, contexts, nodes, heads, 2, head_dim, page, dtype)
+    clean.run(ops, max_nodes=max(1, rows // 2))
+    batch = Batch(21, contexts, nodes, heads, 2, head_dim, page, dtype)
+    bad = torch.zeros(batch.out.shape, dtype=torch.bool, device=batch.out.device)
+    for token, head in ((0, 0), (4, 3), (8, 1), (13, 2)):
+        batch.q[token, head * head_dim + 1] = float("nan")
+        bad[token, head * head_dim:(head + 1) * head_dim] = True
+    batch.run(ops, max_nodes=max(1, rows // 2))
+    assert bool(batch.out[bad].isnan().all())
+    assert torch.equal(batch.out[~bad], clean.out[~bad])
+
+
+@pytest.mark.parametrize("kernel,dtype,head_dim,page,rows", KERNELS)
+@pytest.mark.parametrize("contexts", [[0, 0], [20, 40], [320, 700]])
+def test_a_drafted_key_that_is_no_number_reaches_who_sees_it(kernel, dtype, head_dim, page, rows, contexts):
+    heads, nodes = 4, 12
+    seen = [ancestors([-1, 0, 0, 1, 1, 2, 2, 3, 3, 5, 5, 6])] * 2
+    args = (24, contexts, [nodes] * 2, heads, heads, head_dim, page, dtype)
+    clean = Batch(*args, seen=seen)
+    clean.run(ops, max_nodes=rows)
+    batch = Batch(*args, seen=seen)
+    put(batch, batch.k, 2, 0, float("nan"))
+    batch.run(ops, max_nodes=rows)
+    branch = [r * nodes + n for r in range(2) for n in (2, 5, 6, 9, 10, 11)]
+    others = [n for n in range(2 * nodes) if n not in branch]
+    width = heads * head_dim
+    assert bool(batch.out[branch, :width].isnan().all())
+    assert torch.equal(batch.out[others, :width], clean.out[others, :width])
