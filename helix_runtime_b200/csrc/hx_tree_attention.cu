@@ -65,8 +65,12 @@ __device__ __forceinline__ void two_fma(float w, float x, float y, float& a, flo
       : "f"(w), "f"(x), "f"(y));
 }
 
+// A weight that stands for a key which its row does not see (weights themselves are never negative).
+constexpr uint32_t NOT_SEEN = 0x80000000u;
+
 // acc[i] += a tile's values by the probabilities of row i: coordinates 4 lane .. of a warp's rows.  MASKED: a
-// (drafted) key that a row does not see adds nothing to it, not even an infinity times zero.
+// (drafted) key that a row does not see adds nothing to it, not even an infinity times zero.  One that it sees
+// adds what its weight makes of it, also a weight of zero, as in tiles without drafted keys.
 template <bool MASKED, int PIECES>
 __device__ __forceinline__ void tile_weigh(float4 (&acc)[ROWS_A_WARP][PIECES], const float4* my_p, const float* values,
                                            int D, int lane, int keys) {
@@ -87,7 +91,7 @@ __device__ __forceinline__ void tile_weigh(float4 (&acc)[ROWS_A_WARP][PIECES], c
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-          if (MASKED && w[k] == 0.0f) continue;
+          if (MASKED && __float_as_uint(w[k]) == NOT_SEEN) continue;
           two_fma(w[k], v[k][j].x, v[k][j].y, acc[i][j].x, acc[i][j].y);
           two_fma(w[k], v[k][j].z, v[k][j].w, acc[i][j].z, acc[i][j].w);
         }
@@ -221,13 +225,17 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = warp * ROWS_A_WARP + 4 * row_y + j;
-        unsigned long long mask = ~0ull;
-        if (drafted)
-          mask = row < rows_here ? tree_mask(a, c, rows.token0 + row / rows.heads, key0) : 0ull;
+        unsigned seen = ~0u;      // bit 16 (i % 2) + i / 2 of it: the row sees key key_x + 16 i
+        if (drafted) {
+          const unsigned long long mask =
+              (row < rows_here ? tree_mask(a, c, rows.token0 + row / rows.heads, key0) : 0ull) >> key_x;
+          seen = (static_cast<unsigned>(mask) & 0x00010001u) | (static_cast<unsigned>(mask >> 32) & 0x00010001u) << 1;
+        }
+        auto sees = [&](int i) { return (seen >> (16 * (i % 2) + i / 2)) & 1; };
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[j][i] = (mask >> (key_x + 16 * i)) & 1 ? s[j][i] * scale_log2 : -INFINITY;
+          s[j][i] = sees(i) ? s[j][i] * scale_log2 : -INFINITY;
           top = fmaxf(top, s[j][i]);
         }
 #pragma unroll
@@ -241,7 +249,7 @@ __global__ __launch_bounds__(TILE_WARPS * 32, TileConfig<D_MAX>::kCtas) void tre
         for (int i = 0; i < 4; ++i) {
           const float p = exp2f(s[j][i] - against);
           sum += p;
-          probabilities[row * TILE_KEYS + key_x + 16 * i] = p;
+          probabilities[row * TILE_KEYS + key_x + 16 * i] = sees(i) ? p : __uint_as_float(NOT_SEEN);
         }
 #pragma unroll
         for (int offset = 8; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);

@@ -413,3 +413,32 @@ def test_a_drafted_key_that_is_no_number_reaches_who_sees_it(kernel, dtype, head
     width = heads * head_dim
     assert bool(batch.out[branch, :width].isnan().all())
     assert torch.equal(batch.out[others, :width], clean.out[others, :width])
+
+
+@pytest.mark.parametrize("kernel,dtype,head_dim,page,rows",
+                         [case for case in KERNELS if case[0] != "tensor memory"])
+@pytest.mark.parametrize("context,place", [(0, 2), (60, 62), (64, 66), (100, 102), (100, 99), (100, 3), (40, 33),
+                                           (64, 63)])
+def test_a_weight_of_zero_does_not_hide_a_value(kernel, dtype, head_dim, page, rows, context, place):
+    """A key that a token sees with a score so low that its weight is zero in 32 bits, and a value that is not finite:
+    the output is not finite, wherever a tile of keys begins.  Who does not see it gets what it got."""
+    nodes, heads = 12, 2
+    parents = [-1, 0, 0, 1, 1, 2, 2, 3, 3, 5, 5, 6]
+    seen = [ancestors(parents)]
+    outs = []
+    for value in (0.0, float("inf")):
+        batch = Batch(22, [context], [nodes], heads, heads, head_dim, page, dtype, seen=seen)
+        batch.q.copy_(batch.q.abs())
+        page_id = int(batch.tables[batch.row[0], place // page])
+        for cache, number in ((batch.k, -1e4), (batch.v, value)):
+            held = from_cache(cache[page_id]).clone()
+            held[:, place % page] = number
+            cache[page_id] = to_cache(held, dtype)
+        batch.run(ops, max_nodes=rows)
+        assert int(batch.status.item()) == 0
+        outs.append(batch.out[:nodes, :heads * head_dim].clone())
+    sees = [n for n in range(nodes) if place < context or seen[0][n, place - context]]
+    others = [n for n in range(nodes) if n not in sees]
+    assert bool(outs[0].isfinite().all())
+    assert not bool(outs[1][sees].isfinite().any())
+    assert torch.equal(outs[1][others], outs[0][others])
