@@ -345,7 +345,7 @@ __global__ __launch_bounds__(THREADS, 2) void verify_kernel(const __grid_constan
       if (drafted) mine.q_sum = warp_sum(q_sum);
     }
     tell(mine, false);
-    const int first_phase = phase;
+    bool row_sums = true;      // what was told last is the row's own sums (and not what a fallen child leaves)
     const Told all = join_told(of_cta[phase][lane % ctas], ctas, table, unit);
     if (all.bad || (drafted && all.q_max == -INFINITY)) {
       if (writes && lane == 0) {
@@ -418,6 +418,7 @@ __global__ __launch_bounds__(THREADS, 2) void verify_kernel(const __grid_constan
         });
         mine.p_sum = warp_sum(sum);
         tell(mine, true);
+        row_sums = false;
         left = sum_of(of_cta[phase][lane % ctas].p_sum, ctas);
       } else {
         // fell already: nothing of it is left
@@ -473,7 +474,7 @@ __global__ __launch_bounds__(THREADS, 2) void verify_kernel(const __grid_constan
     };
     // every warp's sum: p's from the row's first exchange, what is over from that of the last fallen
     // child, otherwise told now
-    const bool first_sums = plain && phase == first_phase;
+    const bool first_sums = plain && row_sums;
     if (listed || (plain && !first_sums)) {
       double sum = 0.0;
       for (int base = first; base < last; base += 128) {

@@ -271,3 +271,23 @@ def test_refusals():
     refused(path=good["path"][:, :0])
     refused(kept=good["kept"][:1])
     refused(requests=-1)
+
+
+@pytest.mark.parametrize("replacement", [False, True])
+@pytest.mark.parametrize("vocab", [300, 5000, 130000])
+@pytest.mark.parametrize("fallen", [1, 2, 3, 4, 5, 8])
+def test_nothing_is_left_of_the_distribution(fallen, vocab, replacement):
+    """Target and draft agree on a few tokens, and the children are others, which weigh nothing in either: each
+    falls, the first takes all of the target with it, and the next token is the target's own sample."""
+    heavy = [vocab - 90, vocab - 60, vocab - 7]
+    drafts = Drafts(16, [fallen + 1] * 3, vocab, replacement=replacement, heat=0.01,
+                    parents=[[-1] + [0] * fallen] * 3)
+    drafts.logits[:] = -1000.0
+    drafts.logits[:, heavy] = [0.5, 0.5, 0.5]
+    drafts.draft[:] = drafts.logits
+    drafts.ids[:] = np.arange(drafts.ids.size)
+    for request, number in enumerate((0.1, 0.5, 0.9)):
+        drafts.uniform[request * (fallen + 1)] = number
+    drafts.run()
+    assert drafts.next[:3].tolist() == heavy
+    assert drafts.kept[:3].tolist() == [1, 1, 1] and int(drafts.status.item()) == 0
