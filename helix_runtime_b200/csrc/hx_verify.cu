@@ -377,8 +377,20 @@ __global__ __launch_bounds__(THREADS, 2) void verify_kernel(const __grid_constan
 
     // ---- the children, in order
     double b = 0.0, left = 1.0, gone = 0.0;
-    int fallen = 0;            // without a draft model: different tokens that fell, whose p is out of `left`
+    // without putting back: different tokens that fell.  (Without a draft model their p is out of `left`, with one their
+    // q is in `gone`; a token that is drafted again takes nothing more.)
+    int fallen = 0;
     int fallen_token = -1;     // lane f: the f-th of them
+    auto fell_before = [&](int child, int token) {
+      bool again = __any_sync(0xffffffffu, lane < fallen && fallen_token == token);
+      if (fallen > 32)
+        for (int j = child_of(node, node); j < child; j = child_of(node, j)) again |= id_at(j) == token;
+      return again;
+    };
+    auto remember = [&](int token) {
+      if (lane == fallen) fallen_token = token;
+      ++fallen;
+    };
     int stands = -1;
     // lane k: the k-th child's shares, before anything fell
     const double my_p_share = !greedy && my_token >= 0 ? of_p(my_p) * p_unit : 0.0;
@@ -405,12 +417,16 @@ __global__ __launch_bounds__(THREADS, 2) void verify_kernel(const __grid_constan
         const double rest = 1.0 - gone;
         if (!(rest > 0.0)) continue;      // nothing of q is left to have been drawn from
         const double scale = a.put_back ? 1.0 : 1.0 / rest;
-        if (u * q * scale * left < p - b * q) {
+        const bool again = !a.put_back && fell_before(child, token);
+        if (!again && u * q * scale * left < p - b * q) {
           stands = child;
           break;
         }
         b += left * scale;
-        if (!a.put_back) gone += q;
+        if (!a.put_back && !again) {
+          gone += q;
+          remember(token);
+        }
         double sum = 0.0;
         each_share([&](int, double of_target, double of_draft) {
           const double over = of_target - b * of_draft;
@@ -421,18 +437,13 @@ __global__ __launch_bounds__(THREADS, 2) void verify_kernel(const __grid_constan
         row_sums = false;
         left = sum_of(of_cta[phase][lane % ctas].p_sum, ctas);
       } else {
-        // fell already: nothing of it is left
-        bool again = __any_sync(0xffffffffu, lane < fallen && fallen_token == token);
-        if (fallen > 32)
-          for (int j = child_of(node, node); j < child; j = child_of(node, j)) again |= id_at(j) == token;
-        if (again) continue;
+        if (fell_before(child, token)) continue;      // nothing of it is left
         if (u * left < p) {
           stands = child;
           break;
         }
         left -= p;
-        if (lane == fallen) fallen_token = token;
-        ++fallen;
+        remember(token);
       }
     }
     if (stands >= 0) {
@@ -449,7 +460,7 @@ __global__ __launch_bounds__(THREADS, 2) void verify_kernel(const __grid_constan
     }
     const double u = number_at(0);
     const bool plain = !(left > 0.0) || (fallen == 0 && b == 0.0);      // (nothing left but by rounding: p itself)
-    const bool listed = !plain && fallen > 0;      // the fallen children's tokens weigh nothing
+    const bool listed = !plain && !drafted && fallen > 0;      // the fallen children's tokens weigh nothing
     // has the token fallen? (the warp asks together)
     auto fell = [&](int id) {
       bool out = false;

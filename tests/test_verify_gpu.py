@@ -291,3 +291,15 @@ def test_nothing_is_left_of_the_distribution(fallen, vocab, replacement):
     drafts.run()
     assert drafts.next[:3].tolist() == heavy
     assert drafts.kept[:3].tolist() == [1, 1, 1] and int(drafts.status.item()) == 0
+
+
+@pytest.mark.parametrize("vocab", [12, 300])
+def test_a_token_drafted_twice_without_putting_back(vocab):
+    """It cannot have been drawn a second time: nothing of the draft is left of it, and nothing more goes."""
+    for seed in range(40, 52):
+        drafts = Drafts(seed, [9, 9], vocab, noise=2.0, parents=[[-1] + [0] * 8] * 2)
+        drafts.ids[3] = drafts.ids[2] = drafts.ids[1]
+        drafts.ids[[12, 16]] = drafts.ids[10]
+        drafts.uniform[1:9] = 1.0 - 2.0 ** -24
+        drafts.uniform[[10, 11, 12, 13]] = 1.0 - 2.0 ** -24
+        drafts.run().check()
