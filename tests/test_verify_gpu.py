@@ -303,3 +303,24 @@ def test_a_token_drafted_twice_without_putting_back(vocab):
         drafts.uniform[1:9] = 1.0 - 2.0 ** -24
         drafts.uniform[[10, 11, 12, 13]] = 1.0 - 2.0 ** -24
         drafts.run().check()
+
+
+@pytest.mark.parametrize("mode", ["without", "with", "lookup"])
+@pytest.mark.parametrize("nodes,vocab", [([257], 90), ([300, 40, 256], 70), ([701, 1], 500)])
+def test_trees_past_the_shared_tables(mode, nodes, vocab):
+    """Trees of which shared memory holds no copy, walked over their whole depth."""
+    for seed, noise in ((30, 0.7), (31, 0.0)):
+        parents = [[-1] + [j - 1 if j % 3 else max(0, j - 4) for j in range(1, n)] for n in nodes]
+        drafts = Drafts(seed, nodes, vocab, draft=mode != "lookup", replacement=mode == "with", noise=noise,
+                        parents=parents)
+        drafts.run().check()
+    if mode != "lookup":      # (the last drafts are the target's: every first child stands, half of the tokens are on the way)
+        assert int(drafts.kept[0]) >= nodes[0] // 2
+
+
+@pytest.mark.parametrize("mode", ["without", "with", "lookup"])
+@pytest.mark.parametrize("vocab", [102400, 102401, 130000, 262147])
+def test_vocabularies_whose_exponentials_are_computed_again(mode, vocab):
+    for seed in (32, 33):
+        Drafts(seed, [6, 9, 4], vocab, draft=mode != "lookup", replacement=mode == "with", heat=[0.8, 1.1, 0.0],
+               pad=seed % 2 * 3).run().check()
