@@ -231,6 +231,11 @@ class CacheManager:
         """Positions the request has pages for: its length plus what steps in flight add."""
         return self._requests[request].reserved
 
+    def admission(self, request: Hashable) -> Optional[object]:
+        """The request as it was admitted (None: it is not there): a later one of the same name is
+        another object."""
+        return self._requests.get(request)
+
     def live_requests(self) -> List[Hashable]:
         return list(self._requests)
 

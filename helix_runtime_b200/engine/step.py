@@ -57,6 +57,15 @@ class StepEntry:
     parents: Optional[Sequence[int]] = None
 
 
+@dataclasses.dataclass
+class OpenTrees:
+    """A step of drafted trees whose requests wait for :meth:`StepFunction.keep`."""
+    entries: List[StepEntry]
+    ctx: StepContext
+    admissions: List[object]          # each entry's request as admitted, see CacheManager.admission
+    lengths: List[int]                # up to where each has reserved
+
+
 class StepError(RuntimeError):
     """The batch is not runnable (bad token, too long, unknown request) or a kernel failed."""
 
@@ -93,8 +102,7 @@ class StepFunction:
         self._uploaded = torch.cuda.Event() if pin else None
         self._tree_host: Optional[torch.Tensor] = None      # made at the first step of trees
         self._tree_device: Optional[torch.Tensor] = None
-        # a step of trees whose requests wait for `keep`
-        self._trees: Optional[Tuple[List[StepEntry], StepContext]] = None
+        self._trees: Optional[OpenTrees] = None
         self.last_context: Optional[StepContext] = None
         self.steps_run = 0
         self.tokens_run = 0
@@ -131,8 +139,10 @@ class StepFunction:
         total = sum(len(entry.tokens) for entry in entries)
         if feed_rows is not None and (len(feed_rows) != len(entries) or total != len(entries)):
             raise StepError("a step fed on the device has one token and one row per request")
-        if self._trees is not None and any(self._open_trees()):
-            raise StepError("the last step's drafted trees wait for what is kept of them")
+        if self._trees is not None:
+            if any(self._open_trees()):
+                raise StepError("the last step's drafted trees wait for what is kept of them")
+            self._trees = None
         masks = self._tree_masks(entries, feed_rows) \
             if any(entry.parents is not None for entry in entries) else None
         if total > self.max_tokens:
@@ -278,11 +288,13 @@ class StepFunction:
         return DraftedTrees(self._tree_device[cap:used].view(tokens, words), places, parents)
 
     def _open_trees(self) -> List[bool]:
-        """Which requests of the last step of trees are there with tokens not yet published (one
-        that has ended, or whose step failed, has none)."""
-        return [self.cache.has(entry.request)
-                and self.cache.reserved(entry.request) > self.cache.length(entry.request)
-                for entry in self._trees[0]]
+        """Which requests of the last step of trees still hold what it reserved for them (one that
+        has ended, though another of its name may be there, or whose step was given up does not)."""
+        open_trees = self._trees
+        return [admission is not None and self.cache.admission(entry.request) is admission
+                and self.cache.reserved(entry.request) == length
+                for entry, admission, length in zip(open_trees.entries, open_trees.admissions,
+                                                    open_trees.lengths)]
 
     def keep(self, path: torch.Tensor, kept: torch.Tensor) -> List[int]:
         """Settle the last step's drafted trees: of request ``r`` (in the order of the entries) the
@@ -293,7 +305,7 @@ class StepFunction:
         tree is refused and changes nothing."""
         if self._trees is None:
             raise StepError("the last step brought no drafted trees")
-        entries, ctx = self._trees
+        entries, ctx = self._trees.entries, self._trees.ctx
         live = self._open_trees()
         if not all(live):
             # what a request that has ended held may be another's by now
@@ -340,7 +352,9 @@ class StepFunction:
                ctx: StepContext) -> None:
         """The step succeeded: publish the new lengths (drafted trees wait for :meth:`keep`)."""
         if ctx.trees is not None:
-            self._trees = (list(entries), ctx)
+            self._trees = OpenTrees(list(entries), ctx,
+                                    [self.cache.admission(entry.request) for entry in entries],
+                                    list(new_lengths))
         else:
             for entry, length in zip(entries, new_lengths):
                 if self.cache.has(entry.request):    # a request may have ended while in flight
@@ -361,6 +375,8 @@ class StepFunction:
                 self.cache.rollback(entry.request,
                                     None if keep_lengths is None else keep_lengths[index],
                                     after=after)
+        if self._trees is not None and not any(self._open_trees()):
+            self._trees = None
 
     @staticmethod
     def describe_status(flags: int) -> str:

@@ -201,3 +201,59 @@ def test_branches_that_are_refused_change_nothing():
     stateful.branch("a", "b", 10)
     assert stateful.state(0)[stateful.slot("b")].tolist() == [7.0] * 4
     stateful.check()
+
+
+def recorder(monkeypatch):
+    """Calls of the operator that moves rows, in place of it: context and kept rows of each request."""
+    moved = []
+    monkeypatch.setattr(steps.ops, "keep_rows",
+                        lambda storage, tables, rows, context, path, kept, requests, status:
+                        moved.append((context[:requests].tolist(), kept[:requests].tolist())))
+    return moved
+
+
+def test_a_tree_that_is_given_up_is_forgotten(monkeypatch):
+    """Plain tokens of its request, queued ahead, are not taken for it, and it can no longer be kept."""
+    moved = recorder(monkeypatch)
+    path, one = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for count in (1, 3):
+        cache = manager()
+        step = function(cache)
+        published(cache, "a", 3)
+        tree = [StepEntry("a", [1] * count, (), list(range(-1, count - 1)))]
+        ctx, _, _, lengths = step.prepare(tree)
+        step.finish(tree, lengths, ctx)
+        step.fail(tree)
+        with pytest.raises(StepError, match="no drafted trees"):
+            step.keep(path, one)
+        plain = [StepEntry("a", [2] * count)]
+        first = step.prepare(plain)
+        with pytest.raises(StepError, match="no drafted trees"):
+            step.keep(path, one)
+        step.prepare([StepEntry("a", [0])], feed_rows=[0])      # queued behind it
+        with pytest.raises(StepError, match="no drafted trees"):
+            step.keep(path, one)
+        step.finish(plain, first[3], first[0])
+        assert cache.length("a") == 3 + count and cache.reserved("a") == 4 + count
+        cache.check()
+    assert not moved
+
+
+def test_a_request_of_the_same_name_has_no_tree(monkeypatch):
+    """What another request of that name has reserved is not the tree's of the one that ended."""
+    moved = recorder(monkeypatch)
+    cache = manager()
+    step = function(cache)
+    published(cache, "a", 3)
+    published(cache, "b", 3)
+    tree = [StepEntry("a", [1] * 4, (), [-1, 0, 0, 0]), StepEntry("b", [1] * 4, (), [-1, 0, 0, 0])]
+    ctx, _, _, lengths = step.prepare(tree)
+    step.finish(tree, lengths, ctx)
+    cache.release("a")
+    published(cache, "a", 3)
+    cache.extend("a", 7)
+    path = torch.tensor([[0, 2], [0, 2]], dtype=torch.int32)
+    assert step.keep(path, torch.tensor([2, 2], dtype=torch.int32)) == [0, 2]
+    assert moved == [([3, 3], [0, 2])]
+    assert (cache.length("a"), cache.reserved("a")) == (3, 7) and cache.length("b") == 5
+    cache.check()
