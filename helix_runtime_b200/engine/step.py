@@ -59,11 +59,13 @@ class StepEntry:
 
 @dataclasses.dataclass
 class OpenTrees:
-    """A step of drafted trees whose requests wait for :meth:`StepFunction.keep`."""
+    """A step of drafted trees whose requests wait for :meth:`StepFunction.keep`, from its
+    preparation on: what they are moved by lies where the next step's description would."""
     entries: List[StepEntry]
     ctx: StepContext
     admissions: List[object]          # each entry's request as admitted, see CacheManager.admission
     lengths: List[int]                # up to where each has reserved
+    run: bool = False
 
 
 class StepError(RuntimeError):
@@ -240,6 +242,10 @@ class StepFunction:
             host_request_contexts=[int(v) for v in request_context[:len(entries)]],
             host_query_lengths=[len(entry.tokens) for entry in entries], trees=trees,
         )
+        if trees is not None:
+            self._trees = OpenTrees(list(entries), ctx,
+                                    [self.cache.admission(entry.request) for entry in entries],
+                                    list(new_lengths))
         return ctx, self._view("want_rows", True), n_want, new_lengths
 
     # ----------------------------------------------------------- drafted trees
@@ -305,8 +311,13 @@ class StepFunction:
         tree is refused and changes nothing."""
         if self._trees is None:
             raise StepError("the last step brought no drafted trees")
+        if not self._trees.run:
+            raise StepError("the step of the drafted trees has not run")
         entries, ctx = self._trees.entries, self._trees.ctx
         live = self._open_trees()
+        for entry, there, context in zip(entries, live, ctx.host_request_contexts):
+            if there and self.cache.length(entry.request) != context:
+                raise StepError(f"an earlier step of request {entry.request!r} has not been published")
         if not all(live):
             # what a request that has ended held may be another's by now
             kept = kept[:len(entries)] * torch.tensor(live, dtype=kept.dtype, device=kept.device)
@@ -352,9 +363,8 @@ class StepFunction:
                ctx: StepContext) -> None:
         """The step succeeded: publish the new lengths (drafted trees wait for :meth:`keep`)."""
         if ctx.trees is not None:
-            self._trees = OpenTrees(list(entries), ctx,
-                                    [self.cache.admission(entry.request) for entry in entries],
-                                    list(new_lengths))
+            if self._trees is not None and self._trees.ctx is ctx:
+                self._trees.run = True
         else:
             for entry, length in zip(entries, new_lengths):
                 if self.cache.has(entry.request):    # a request may have ended while in flight

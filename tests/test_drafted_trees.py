@@ -257,3 +257,51 @@ def test_a_request_of_the_same_name_has_no_tree(monkeypatch):
     assert moved == [([3, 3], [0, 2])]
     assert (cache.length("a"), cache.reserved("a")) == (3, 7) and cache.length("b") == 5
     cache.check()
+
+
+def test_no_step_is_prepared_over_a_tree_that_waits(monkeypatch):
+    """From its preparation on: a step queued behind it would overwrite what its rows are moved by."""
+    moved = recorder(monkeypatch)
+    cache = manager(num_pages=20)
+    step = function(cache)
+    published(cache, "a", 3)
+    published(cache, "b", 9)
+    tree = [StepEntry("a", [1] * 4, (), [-1, 0, 0, 0])]
+    ctx, _, _, lengths = step.prepare(tree)
+    path, two = torch.tensor([[0, 2]], dtype=torch.int32), torch.tensor([2], dtype=torch.int32)
+    with pytest.raises(StepError, match="wait for"):
+        step.prepare([StepEntry("b", [1])])
+    with pytest.raises(StepError, match="not run"):
+        step.keep(path, two)
+    assert cache.reserved("b") == 9 and ctx.request_context[0] == 3
+    step.finish(tree, lengths, ctx)
+    assert step.keep(path, two) == [2]
+    assert moved == [([3], [2])] and cache.length("a") == 5
+    # a preparation that fails, and a tree given up before it has run, leave the way free
+    with pytest.raises(OutOfPages):
+        step.prepare([StepEntry("b", [1] * 100, (), list(range(-1, 99)))])
+    tree = [StepEntry("a", [1] * 4, (), [-1, 0, 0, 0])]
+    step.prepare(tree)
+    step.fail(tree)
+    step.prepare([StepEntry("b", [1])])
+    cache.check()
+
+
+def test_a_tree_waits_for_the_steps_in_front_of_it(monkeypatch):
+    """Its rows lie behind tokens that an earlier step has reserved and not yet published."""
+    moved = recorder(monkeypatch)
+    cache = manager()
+    step = function(cache)
+    published(cache, "a", 3)
+    plain, tree = [StepEntry("a", [1, 2])], [StepEntry("a", [1] * 4, (), [-1, 0, 0, 0])]
+    earlier = step.prepare(plain)
+    ctx, _, _, lengths = step.prepare(tree)
+    step.finish(tree, lengths, ctx)
+    path, two = torch.tensor([[0, 2]], dtype=torch.int32), torch.tensor([2], dtype=torch.int32)
+    with pytest.raises(StepError, match="earlier step"):
+        step.keep(path, two)
+    assert not moved and cache.length("a") == 3
+    step.finish(plain, earlier[3], earlier[0])
+    assert step.keep(path, two) == [2]
+    assert cache.length("a") == cache.reserved("a") == 7
+    cache.check()
