@@ -324,3 +324,36 @@ def test_vocabularies_whose_exponentials_are_computed_again(mode, vocab):
     for seed in (32, 33):
         Drafts(seed, [6, 9, 4], vocab, draft=mode != "lookup", replacement=mode == "with", heat=[0.8, 1.1, 0.0],
                pad=seed % 2 * 3).run().check()
+
+
+@pytest.mark.parametrize("heat", [1.0, 0.8])
+def test_the_exponential_is_as_exact_as_64_bits(heat):
+    """Two tokens, and numbers next to the first one's share: as near as a few roundings in 64 bits allow.
+
+    With logits x <= 0 and 0 the first token follows when u is below e / (1 + e), e = exp(x / T).  In units of
+    2^-53 the factor 64 / (T ln 2) and its product with x are off by 1.5 + 1.5, so e by 3 |x| / T; table, polynomial
+    and their product add 4, the sums, the share and the product with u 8.  Among many x those are taken whose share lies
+    beyond that, and up to 30 times as far, from a float32 u; which side it lies on is told in 80 bits."""
+    if np.finfo(np.longdouble).eps > 1e-18:
+        pytest.skip("no 80-bit numbers here")
+    rng = np.random.default_rng(17)
+    low, high, found = 2.0 ** -53, 30 * 2.0 ** -53, []
+    wide_heat = np.longdouble(np.float32(heat))
+    for _ in range(20):
+        x = (-2.0 * rng.random(1 << 20)).astype(np.float32)
+        scaled = x.astype(np.longdouble) / wide_heat
+        share = np.exp(scaled) / (1 + np.exp(scaled))
+        u = share.astype(np.float32)
+        away = np.abs((u.astype(np.longdouble) - share) / share) / (3 * np.abs(scaled) + 12)
+        near = (away > low) & (away < high)
+        found += list(zip(x[near], u[near], (u.astype(np.longdouble) >= share)[near]))
+    assert len(found) > 20
+    x, u, wanted = (np.array(column) for column in zip(*found))
+    requests = len(found)
+    drafts = Drafts(18, [1] * requests, 2, draft=False, heat=heat)
+    drafts.logits[:] = 0.0
+    drafts.logits[:, 0] = x
+    drafts.uniform = u.astype(np.float32)
+    drafts.run()
+    assert np.array_equal(drafts.next[:requests].cpu().numpy(), wanted.astype(np.int32))
+    assert int(drafts.status.item()) == 0
