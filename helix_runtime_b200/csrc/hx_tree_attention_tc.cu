@@ -469,7 +469,7 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t output_base = lane_base + Config::kOutputColumn;
     const float scale_log2 = a.scale * HX_LOG2E;      // positive: it does not change which score is largest
-    const uint64_t factor_pair = pair_of(scale_log2, scale_log2);
+    const uint64_t factor_pair = pair_of(scale_log2, scale_log2), minus_one = pair_of(-1.0f, -1.0f);
     uint32_t meetings = 0;
     // The two warps of 32 rows meet: each arrives, and waits for both.
     auto arrive = [&]() {
@@ -585,10 +585,13 @@ __global__ __launch_bounds__(THREADS, CTAS_AN_SM) void tree_attention_tc_kernel(
           for (int i = 0; i < 16; ++i) {
             float x0, x1;
             halves_of(pair_fma(pair_of(p[2 * i], p[2 * i + 1]), factor_pair, reference_pair), x0, x1);
-            x0 = fast_exp2(x0);
-            x1 = fast_exp2(x1);
-            part_sum[i % 2] = pair_add(part_sum[i % 2], pair_of(x0, x1));
-            hx_split_bf16(x0, x1, high[i], low[i]);
+            const uint64_t weights = pair_of(fast_exp2(x0), fast_exp2(x1));
+            part_sum[i % 2] = pair_add(part_sum[i % 2], weights);
+            halves_of(weights, x0, x1);
+            high[i] = pack_bf16(x0, x1);
+            halves_of(pair_fma(pair_of(__uint_as_float(high[i] << 16), __uint_as_float(high[i] & 0xffff0000u)), minus_one,
+                               weights), x0, x1);
+            low[i] = pack_bf16(x0, x1);
           }
           {
             float even, odd;
