@@ -101,9 +101,10 @@ __device__ __forceinline__ void tile_weigh(float4 (&acc)[ROWS_A_WARP][PIECES], c
 
 // A warp has 8 rows of the tile.  Scores: a lane has 4 keys (16 apart) of 4 rows, so that 12 reads of 128
 // bytes of shared memory feed 64 multiply-adds of a warp.  Values: a lane has 4 (8, above 128)
-// coordinates of all 8 rows.  Both are bound by the multiply-adds, 3,900 cycles a tile of heads of 112;
-// what counts is that enough warps are there to wait for one another: a tile's values take the place of its
-// keys, so that four CTAs share an SM.  4 requests x 24 drafts behind 700 keys, 32 heads of 112, float32: 79 us
+// coordinates of all 8 rows.  A tile of heads of 112 is 3,900 cycles of multiply-adds, 15,600 for an SM's four
+// CTAs, of the 35,000 that these take: the rest is what its phases wait for, copies, shared memory and one another, as the
+// CTAs run in step.  What counts is that enough warps are there to fill such waits: a tile's values take the place of its
+// keys, so that four CTAs share an SM.  4 requests x 24 drafts behind 700 keys, 32 heads of 112, float32: 80 us
 // (1.1 TB/s, 12 TFLOP/s).  Two CTAs, with keys and values side by side and the next ones on their way, took 95, the
 // same rows spread evenly over the warps 97, 2 keys by 8 rows a lane 90; weighted values without a question for masks where no key is
 // drafted, two multiply-adds an instruction, 79 instead of 84 (the same for the scores took registers it has not: 90).  Of a tile's
@@ -647,9 +648,9 @@ int launch_tile(const TreeArgs& a, int ctas, cudaStream_t stream) {
 }
 
 // Up to here the streaming kernel beats the tcgen05 one, whose tile of 128 rows is mostly empty then (32 heads of 128;
-// streaming against tcgen05): 64 requests x 8 or 16 drafts behind 1,200 keys 214 and 219 us against 259 and 267, x 32
-// drafts 280 against 292; 8 requests behind 640 keys 29, 31 and 38 us against 41, 42 and 43; one request, 32 rows
-// behind 32,701 keys, 45 against 49.  It has no tiles of more rows: a warp's 16 rows fill its registers.
+// streaming against tcgen05): 64 requests x 8 or 16 drafts behind 1,200 keys 215 and 219 us against 321 and 332, x 32
+// drafts 306 to 331 against 345 to 358; 8 requests behind 640 keys 33, 31 and 40 us against 49, 44 and 45; one request, 32 rows
+// behind 32,701 keys, 56 against 53 to 58.  It has no tiles of more rows: a warp's 16 rows fill its registers.
 constexpr int STREAM_MOST_ROWS = 32;
 
 // Which kernel: the tensor cores', the tile kernel, or the row kernel.

@@ -14,11 +14,11 @@
 //
 // Probabilities enter the second product as two bfloat16 terms (hi + lo, 16 bits), which costs nothing for up to
 // 16 rows; for more, one term alone (2^-8 of each weight off) would save a tenth (64 requests x 32 drafts, two
-// terms 323 us, one 290).  The reference of a row's exponentials is raised when a chunk exceeds it by more than 2^8,
+// terms 306 to 331 us, one 290).  The reference of a row's exponentials is raised when a chunk exceeds it by more than 2^8,
 // each row by itself.
 //
 // Measured (32 heads of 128, pages of 16): 64 requests x 16 drafts behind 1,200 keys 219 us, 5.8 TB/s of the 6.55 that a
-// copy reaches: memory.  8 x 32 behind 640 keys 38 us, 2.3 TB/s: a run of 4 chunks a CTA is too short to hide how
+// copy reaches: memory.  8 x 32 behind 640 keys 40 us, 2.3 TB/s: a run of 4 chunks a CTA is too short to hide how
 // it starts (5,000 cycles) and is joined.  One request x 8 behind 509 keys 17 us: two launches and the call.
 //
 // Masks matter in the chunks that hold drafted keys; there values that are not finite are taken as

@@ -34,10 +34,10 @@
 // drafted one that other rows see or what a page holds behind the last key.  Such a value is taken as zero
 // in the product; a drafted one is added, as what it is, to the rows that do see it.
 //
-// Measured (32 heads of 128): one request x 64 drafts behind 32,701 keys, 4 query heads a key/value head, 75 us, 459
-// TFLOP/s: a chain of 2,400 cycles a tile (scores, softmax, output product, one behind the other), which two CTAs an SM
-// fill to a half; tensor memory has no room for a third.  64 requests x 64 drafts behind 1,200 keys, as many key/value heads, 333 us,
-// 4.0 TB/s.
+// Measured (32 heads of 128): one request x 64 drafts behind 32,701 keys, 4 query heads a key/value head, 85 to 91 us, 380
+// to 400 TFLOP/s: scores, softmax and output product of a tile are one behind the other, 2,900 cycles a tile and SM with two
+// CTAs an SM (the tensor pipe is active 30 % of the time); tensor memory has no room for a third.  64 requests x 64 drafts behind
+// 1,200 keys, as many key/value heads, 376 to 390 us, 3.4 TB/s.  With one term of a weight these took 78 and 333 us.
 //
 // Every wait is bounded; a wait that runs out sets a status bit, the CTA lets its copies land, frees its
 // tensor memory and returns.

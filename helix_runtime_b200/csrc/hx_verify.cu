@@ -32,7 +32,7 @@
 // together with the row, and the row that comes next if the first child stands is fetched into the L2
 // meanwhile.  Only rows of tokens that are walked over are read.
 //
-// Measured (32,000 tokens): 64 requests x 32 drafts, with the drafts' logits, 104 to 118 us by the walks drawn; one request x 8 16
+// Measured (32,000 tokens): 64 requests x 32 drafts, with the drafts' logits, 100 to 118 us by the walks drawn; one request x 8 16
 // to 32; 32 x 16 without a draft model 27 to 34.  A visited token takes about 13,000 cycles (two passes over its
 // stretch, an exchange, and one more with each child that falls), the deepest walk of a batch sets the time.  Its bytes,
 // 25 MB, would take 4 us.

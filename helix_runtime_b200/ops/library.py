@@ -1144,7 +1144,9 @@ def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], to
     ``temperature`` (float32 ``[requests]``; 0: greedy, then a draft stands when it is the lowest
     id among the maxima).  Out, all int32: ``path`` ``[requests, width]``, the numbers of the
     tokens that stand, from 0 on, -1 behind them; ``kept`` how many they are; ``next_tokens``, -1
-    (and FLAG_NONFINITE) when logits on the way are not finite.  A path that is full ends the walk."""
+    (and FLAG_NONFINITE) when logits on the way are not finite.  A path that is full ends the walk.
+    Where the children that fell leave nothing of the distribution (tokens that the draft does not
+    give, say), the next token is the target's own sample."""
     device = _here(logits)
     _need_each(device, torch.float32, "logits", logits)
     _need_whole(device, torch.float32, "temperature and uniform", temperature, uniform)
